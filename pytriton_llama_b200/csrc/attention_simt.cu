@@ -466,6 +466,13 @@ int attention_merge_bf16(void* out, const float* part_acc, const float* part_ml,
                        dim3((unsigned)((pairs + kMergeWarps - 1) / kMergeWarps)), dim3(kMergeWarps * 32), 0, as_stream(stream),
                        (__nv_bfloat16*)out, part_acc, part_ml, out_stride, nq, d, splits, items, tokens);
 }
+int attention_merge_f32(void* out, const float* part_acc, const float* part_ml, int tokens, int out_stride,
+                        int nq, int d, int splits, const int* items, void* stream) {
+  const long long pairs = (long long)tokens * nq;
+  return launch_kernel("attention_merge", attention_merge_kernel<float>,
+                       dim3((unsigned)((pairs + kMergeWarps - 1) / kMergeWarps)), dim3(kMergeWarps * 32), 0, as_stream(stream),
+                       (float*)out, part_acc, part_ml, out_stride, nq, d, splits, items, tokens);
+}
 
 }  // namespace ptl
 

@@ -13,6 +13,7 @@ import ctypes
 import os
 from typing import Optional, Tuple
 
+import numpy as np
 import torch
 
 from . import build
@@ -89,6 +90,10 @@ _SIGNATURES = {
     "ptl_moe_grouped": [_ptr, _c_int, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f, _c_f, _c_f, _ptr],
     "ptl_moe_combine_norm": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_f, _ptr],
     "ptl_moe_combine": [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _ptr],
+    "ptl_rope_kv8_write": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ll, _ptr],
+    "ptl_read_kv8": [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr],
+    "ptl_attention8_simt": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                            _c_int, _c_f, _c_int, _c_int, _c_int, _ptr],
     "ptl_paged_attention_simt": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int,
                                  _c_int, _c_int, _c_int, _c_int, _c_f, _c_int, _c_int, _c_int, _ptr],
 }
@@ -201,6 +206,10 @@ def load_library() -> ctypes.CDLL:
     lib.ptl_sample_cluster.restype = _c_int
     lib.ptl_sample_work_words.argtypes = []
     lib.ptl_sample_work_words.restype = _c_int
+    lib.ptl_token_scores.argtypes = [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _ptr]
+    lib.ptl_token_scores.restype = _c_int
+    lib.ptl_copy_pages.argtypes = [_ptr, _ptr, _c_int, _ptr, _ptr, _c_int, _ptr, _ptr]
+    lib.ptl_copy_pages.restype = _c_int
     lib.ptl_softcap.argtypes = [_ptr, _c_ll, _c_f, _ptr]
     lib.ptl_softcap.restype = _c_int
     lib.ptl_prefill_attention_opts_bf16.argtypes = [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
@@ -361,6 +370,7 @@ class CudaOps:
         "add_tanh_norm": "norm", "linear_add_tanh_norm": "product", "combine_experts_tanh_norm": "experts", "linear_relu2": "product",
         "linear_each": "product", "token_shift": "elementwise", "wkv_scan": "recurrent", "state_space_scan": "recurrent",
         "gated_group_norm": "norm", "gated_lru": "recurrent",
+        "rope_kv8_write": "rope", "read_kv8": "attention", "paged_attention8": "attention", "copy_pages": "cache", "token_scores": "sampling",
         "head_norm_rotate_store": "rope", "pool_blocks": "attention", "post_norm_add": "norm", "mean_of_normed": "norm",
     }
 
@@ -877,6 +887,142 @@ class CudaOps:
         self._attention_tensor_cores(out, qkv, cache, block_table, tok_req, positions, nq, nkv, d, page_size, scale,
                                      window, hints, rope=(inv_freq, slots if write else None))
         return out
+
+    # ------------------------------------------------------------------ keys and values in 8 bits
+    KV8_BLOCK = 16         # positions that share a scale
+
+    def _want_kv8(self, codes: torch.Tensor, words: torch.Tensor, nkv: int, d: int, page_size: int) -> None:
+        self._want(codes, "codes", torch.uint8)
+        self._want(words, "words", torch.int32)
+        if page_size % self.KV8_BLOCK:
+            raise KernelError(f"8-bit cache: pages of {page_size} positions are no whole blocks of {self.KV8_BLOCK}")
+        if d % 16 or d <= 0 or d > 256:
+            raise KernelError(f"8-bit cache: head size {d} is no multiple of 16 up to 256")
+        if codes.dim() < 1 or codes[0].numel() != 2 * nkv * page_size * d or codes.shape[0] == 0:
+            raise KernelError(f"8-bit cache: pages of {tuple(codes.shape)} do not fit {nkv} heads of {d} and {page_size} positions")
+        if tuple(words.shape) != (codes.shape[0], nkv, page_size // self.KV8_BLOCK, 2):
+            raise KernelError(f"8-bit cache: words {tuple(words.shape)}, expected {(codes.shape[0], nkv, page_size // self.KV8_BLOCK, 2)}")
+
+    def rope_kv8_write(self, qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optional[torch.Tensor], rot: int,
+                       slots: torch.Tensor, codes: torch.Tensor, words: torch.Tensor, nq: int, nkv: int, d: int, page_size: int) -> None:
+        """``rope_kv_write`` for a cache that holds keys and values in 8 bits: q is turned in place, k (turned, in qkv's type)
+        and v go to their slots; qkv's k and v columns stay as they are.
+
+        ``codes`` uint8 [pages, 2 (k, v), nkv, page_size, d] and ``words`` int32 [pages, nkv, page_size / 16, 2 (k, v)], where a
+        word has the exponent E of 16 positions' scale in bits 0..7 and a mark for each token with a value that is no
+        finite number in bits 16..31.  A code u stands for (u - 127.5) * 2^(E - 133), at most half a step from what was
+        written; E 0: all zeros.  A token at the first of the 16 positions starts them anew, a later one raises E where it
+        has to, and the codes that are there go by it: what is held does not depend on the steps that the tokens came in.
+        Rows of the same 16 positions stand next to each other, no slot twice (a request's tokens do); rows with a slot that is
+        negative or behind the pool write nothing."""
+        self._want(qkv, "qkv")
+        self._want(positions, "positions", torch.int32)
+        self._want(slots, "slots", torch.int32)
+        self._want_kv8(codes, words, nkv, d, page_size)
+        if qkv.dim() != 2 or qkv.shape[1] != (nq + 2 * nkv) * d:
+            raise KernelError(f"qkv is {tuple(qkv.shape)}, expected rows of {(nq + 2 * nkv) * d} elements")
+        if positions.numel() < qkv.shape[0] or slots.numel() < qkv.shape[0]:
+            raise KernelError("rope_kv8_write: fewer positions or slots than rows")
+        if inv_freq is not None:
+            self._want(inv_freq, "inv_freq", torch.float32)
+            if inv_freq.numel() < rot // 2:
+                raise KernelError("inv_freq shorter than half the rotary width")
+        fn = getattr(self.lib, "ptl_rope_kv8_write" + _suffix(qkv.dtype))
+        self._check(fn(_p(qkv), _p(positions), _p(inv_freq), _p(slots), _p(codes), _p(words), qkv.shape[0], nq, nkv, d, rot, page_size,
+                       codes.shape[0] * page_size, self._stream()), kernels=1 if qkv.shape[0] else 0)
+
+    def read_kv8(self, codes: torch.Tensor, words: torch.Tensor, block_table: torch.Tensor, contexts, dtype: torch.dtype) -> torch.Tensor:
+        """What an 8-bit cache holds of the first ``contexts[r]`` (host integers) positions of the requests in the table's rows,
+        request after request: [tokens, 2 (k, v), nkv, d].  bfloat16 holds every value exactly.  A marked token reads as NaN, a
+        position without a page as 0."""
+        if codes.dim() != 5:
+            raise KernelError(f"codes are {tuple(codes.shape)}, expected [pages, 2, heads, positions, d]")
+        pages, _, nkv, page_size, d = codes.shape
+        self._want_kv8(codes, words, nkv, d, page_size)
+        self._want(block_table, "block_table", torch.int32)
+        contexts = np.ascontiguousarray(np.asarray(contexts, dtype=np.int64).reshape(-1))
+        if block_table.dim() != 2 or contexts.size > block_table.shape[0]:
+            raise KernelError(f"read_kv8: {contexts.size} requests, the table has {tuple(block_table.shape)} entries")
+        for r, n in enumerate(contexts):
+            if not 0 <= n <= block_table.shape[1] * page_size:
+                raise KernelError(f"read_kv8: a request of {n} tokens does not fit its row of the table")
+        contexts = contexts.astype(np.int32)
+        total = int(contexts.sum(dtype=np.int64))
+        out = self.empty((total, 2, nkv, d), dtype)
+        fn = getattr(self.lib, "ptl_read_kv8" + _suffix(dtype))
+        self._check(fn(_p(out), _p(codes), _p(words), _p(block_table), contexts.ctypes.data, contexts.size, block_table.shape[1], nkv, d,
+                       page_size, pages, self._stream()), kernels=1 if total else 0)
+        return out
+
+    def paged_attention8(self, q: torch.Tensor, codes: torch.Tensor, words: torch.Tensor, block_table: torch.Tensor, tok_req: torch.Tensor,
+                         positions: torch.Tensor, nq: int, nkv: int, d: int, page_size: int, scale: float, window: int = 0,
+                         hints=None) -> torch.Tensor:
+        """``paged_attention`` over an 8-bit cache (``rope_kv8_write``).  q is [T, >= nq*d] (the q part of a qkv buffer is fine);
+        returns [T, nq*d].  A token that was written with a number that is not finite gives NaN to the rows that see it and
+        to no other; a position without a page is not seen; a row without a request or without keys is zeros."""
+        self._want(q, "q")
+        self._want_kv8(codes, words, nkv, d, page_size)
+        for name, t in (("block_table", block_table), ("tok_req", tok_req), ("positions", positions)):
+            self._want(t, name, torch.int32)
+        tokens = q.shape[0]
+        if q.dim() != 2 or q.shape[1] < nq * d or nq <= 0 or nq % nkv:
+            raise KernelError(f"paged_attention8: q {tuple(q.shape)} for {nq} heads of {d} over {nkv} kv heads")
+        if block_table.dim() != 2:
+            raise KernelError(f"paged_attention8: the block table is {tuple(block_table.shape)}, expected a row per request")
+        if tok_req.numel() < tokens or positions.numel() < tokens:
+            raise KernelError("paged_attention8: fewer requests or positions than rows")
+        if window < 0:
+            raise KernelError(f"paged_attention8: a window of {window} positions")
+        out = self.empty((tokens, nq * d), q.dtype)
+        longest = getattr(hints, "max_ctx_len", 0) or block_table.shape[1] * page_size
+        if window:
+            longest = min(longest, window)
+        # blocks of 128 keys' turns: split until they fill the machine a few times
+        splits = max(1, min(-(-longest // 256), 148 * 8 // max(1, tokens * nq), 64))
+        part_acc = part_ml = None
+        if splits > 1:
+            part_acc = self.empty((tokens, nq, splits, d), torch.float32)
+            part_ml = self.empty((tokens, nq, splits, 2), torch.float32)
+        fn = getattr(self.lib, "ptl_attention8_simt" + _suffix(q.dtype))
+        self._check(fn(_p(out), _p(part_acc), _p(part_ml), _p(q), _p(codes), _p(words), _p(block_table), _p(tok_req), _p(positions), tokens,
+                       q.shape[1], nq * d, block_table.shape[1], nq, nkv, d, page_size, float(scale), int(window), splits, codes.shape[0],
+                       self._stream()), kernels=(2 if splits > 1 else 1) if tokens else 0)
+        return out
+
+    # ------------------------------------------------------------------ pages
+    def copy_pages(self, tensors, src, dst) -> None:
+        """tensor[dst[i]] = tensor[src[i]] for every i and every one of ``tensors`` (any types, rows of any size, at least as many
+        rows as the largest index says), in one launch.  ``src`` and ``dst`` are host integers; no row is written twice, and none that is
+        read is written."""
+        src = np.ascontiguousarray(np.asarray(src, dtype=np.int64).reshape(-1))
+        dst = np.ascontiguousarray(np.asarray(dst, dtype=np.int64).reshape(-1))
+        if src.size != dst.size:
+            raise KernelError(f"copy_pages: {src.size} rows to read, {dst.size} to write")
+        tensors = list(tensors)
+        if not src.size or not tensors:
+            return
+        seen = np.unique(dst)
+        if seen.size != dst.size:
+            raise KernelError("copy_pages: a row is written twice")
+        if np.isin(src, seen, assume_unique=False).any():
+            raise KernelError("copy_pages: a row that is read is written too")
+        low, high = int(min(src.min(), dst.min())), int(max(src.max(), dst.max()))
+        for t in tensors:
+            self._want(t, "a tensor of pages")
+            if t.dim() < 1 or low < 0 or high >= t.shape[0] or high > 0x7fffffff:
+                raise KernelError(f"copy_pages: rows {low}..{high} of a tensor {tuple(t.shape)}")
+        starts = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel()]
+        starts.sort()
+        if any(a[1] > b[0] for a, b in zip(starts, starts[1:])):
+            raise KernelError("copy_pages: two tensors share memory")
+        held = [t for t in tensors if t.numel()]
+        n = len(held)
+        base = (_ptr * n)(*(t.data_ptr() for t in held))
+        row = (_c_ll * n)(*(t.numel() // t.shape[0] * t.element_size() for t in held))
+        src32, dst32 = src.astype(np.int32), dst.astype(np.int32)
+        launches = _c_int(0)
+        rc = self.lib.ptl_copy_pages(base, row, n, src32.ctypes.data, dst32.ctypes.data, src32.size, ctypes.byref(launches), self._stream())
+        self._check(rc, kernels=launches.value)
 
     def begin_forward(self) -> None:
         """Called by the model at the start of every forward pass: what was worked out for the last
@@ -2351,6 +2497,29 @@ class CudaOps:
         self._check(self.lib.ptl_token_logprob(_p(out), _p(logits), _p(tokens), _p(scratch[0]), _p(scratch[1]), rows, vocab, vocab,
                                                self._stream()), kernels=2)
         return out
+
+    SCORES_MAX_TOP = 32
+
+    def token_scores(self, logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
+        """(log softmax(logits[row])[tokens[row]] [rows], the entropy of softmax(logits[row]) in nats [rows], the log-probabilities of the
+        ``top`` most likely tokens [rows, k] and the tokens, int32 [rows, k]), k = min(top, vocabulary), best first, of
+        equal logits the lowest index first; ``top`` up to 32.  A token outside the vocabulary has -inf.  A row without a
+        distribution (a NaN, +inf, or -inf only) has NaN log-probabilities and entropy; its alternatives are the largest logits, NaN last."""
+        self._want(logits, "logits", torch.float32)
+        self._want(tokens, "tokens", torch.int32)
+        if logits.dim() != 2 or logits.shape[1] == 0:
+            raise KernelError(f"token_scores: logits are {tuple(logits.shape)}, expected [rows, vocabulary]")
+        rows, vocab = logits.shape
+        if tokens.numel() != rows:
+            raise KernelError(f"token_scores: {tokens.numel()} tokens for {rows} rows")
+        if not 0 <= top <= self.SCORES_MAX_TOP:
+            raise KernelError(f"token_scores: {top} alternatives, at most {self.SCORES_MAX_TOP}")
+        k = min(int(top), vocab)
+        scores = self.empty((2, rows), torch.float32)
+        best, ids = self.empty((rows, k), torch.float32), self.empty((rows, k), torch.int32)
+        self._check(self.lib.ptl_token_scores(_p(scores[0]), _p(scores[1]), _p(best), _p(ids), _p(logits), _p(tokens), rows, vocab, k,
+                                              self._stream()), kernels=1 if rows else 0)
+        return scores[0], scores[1], best, ids
 
     def sample_tokens(self, logits: torch.Tensor, temperature: Optional[torch.Tensor], top_p: Optional[torch.Tensor],
                       u: Optional[torch.Tensor], out: Optional[torch.Tensor] = None, logprobs: bool = False):
