@@ -35,6 +35,10 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--triton_weight", action="store_true", default=True, help="kept for lite_llama's name; no effect")
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
     ap.add_argument("--page_size", type=int, default=16)
+    ap.add_argument("--cache_bits", type=int, choices=[8], help="hold keys and values in 8 bits (default: in the compute type)")
+    ap.add_argument("--n", type=int, default=1, help="completions of --prompt_ids, one to a line, each with its mean log-probability")
+    ap.add_argument("--top_logprobs", type=int, default=0,
+                    help="with --prompt_ids: print every generated token with that many of the most likely ones, and the entropy")
     ap.add_argument("--device", default="cuda")
     ap.add_argument("--stats", action="store_true",
                     help="time every step on the device (steps then run uncaptured, one at a time) and print, after each "
@@ -72,7 +76,7 @@ def main(argv: Optional[List[str]] = None) -> int:
         checkpoints_dir=str(folder), tokenizer_path=str(folder) if _has_tokenizer(folder) else None,
         max_gpu_num_blocks=args.max_gpu_num_blocks, max_seq_len=args.max_seq_len,
         load_model=args.load_model, triton_weight=args.triton_weight, compiled_model=args.compiled_model,
-        device=args.device, dtype=args.dtype, page_size=args.page_size, seed=args.seed, timing=args.stats)
+        device=args.device, dtype=args.dtype, page_size=args.page_size, cache_bits=args.cache_bits, seed=args.seed, timing=args.stats)
     engine = generator.llm.engine
     if args.stats and engine.memory_report:
         print(f"[stats] cache pool: {json.dumps(engine.memory_report)}", file=sys.stderr)
@@ -86,6 +90,22 @@ def main(argv: Optional[List[str]] = None) -> int:
             if batch[0]:
                 print(" ".join(str(t) for t in batch[0]), end=" ", flush=True)
         print()
+        show_stats()
+
+    def run_scored(ids: List[int]) -> None:
+        from pytriton_llama_b200 import SamplingParams
+        llm = generator.llm
+        params = SamplingParams(temperature=args.temperature, top_p=args.top_p, max_gen_len=args.max_gen_len, n=args.n, logprobs=True,
+                                top_logprobs=args.top_logprobs)
+        req = llm.add_request(ids, params)
+        for _ in llm.run():
+            pass
+        engine.check_device_status()
+        for r in (req, *req.siblings):
+            mean = sum(r.logprobs) / max(1, len(r.logprobs))
+            print(f"{mean:.4f} " + " ".join(str(t) for t in r.output))
+            for t, lp, entropy, best in zip(r.output, r.logprobs, r.entropies, r.top_logprobs):
+                print(f"  {t} {lp:.4f} entropy {entropy:.4f}: " + " ".join(f"{a} {v:.4f}" for a, v in best))
         show_stats()
 
     from pytriton_llama_b200.utils import prompt_for_tokenizer
@@ -102,7 +122,7 @@ def main(argv: Optional[List[str]] = None) -> int:
         show_stats()
 
     if args.prompt_ids:
-        run_ids(args.prompt_ids)
+        (run_scored if args.n > 1 or args.top_logprobs else run_ids)(args.prompt_ids)
         return 0
     if args.prompt is not None:
         run_text(args.prompt)

@@ -8,11 +8,11 @@ from .config import EngineConfig, LlamaConfig, TibepelConfig  # noqa: F401
 from .sampling import SamplingParams  # noqa: F401
 
 __all__ = ["EngineConfig", "LlamaConfig", "TibepelConfig", "SamplingParams", "LLM", "Engine", "StepEntry",
-           "GenerateText", "GenerateStreamText"]
+           "GenerateText", "GenerateStreamText", "PromptScores"]
 
 
 def __getattr__(name):
-    if name in ("LLM", "GenerateText", "GenerateStreamText"):
+    if name in ("LLM", "GenerateText", "GenerateStreamText", "PromptScores"):
         from .engine import llm
         return getattr(llm, name)
     if name in ("Engine", "StepEntry"):

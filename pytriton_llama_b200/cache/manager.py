@@ -17,12 +17,17 @@ completes goes, -1 for a token that completes none.
 
 Cache entries (one per run of a layer that stores keys and values) with equal needs form a
 group.  A page id is valid in every entry of its group: entry e keeps its share of page p in
-``kv[e][p]`` of shape [2 (k, v), kv_heads, page_size, head_dim].
+``kv[e][p]`` of shape [2 (k, v), kv_heads, page_size, head_dim]; keys and values in 8 bits are uint8
+there, and ``words[e][p]`` holds their scales, int32 [kv_heads, page_size / 16, 2 (k, v)].
+
+A request can be forked: the new ones share its full pages, which nothing writes again, and get copies of the
+page it is in the middle of and of its states.  ``compact`` moves the pages in use to the front of their
+pools, and ``resize`` gives the pools another number of pages.
 """
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Dict, Hashable, List, Optional, Tuple
+from typing import Dict, Hashable, List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -56,6 +61,9 @@ class PagePool:
     def used_pages(self) -> int:
         return self.num_pages - len(self._free)
 
+    def holders(self, page: int) -> int:
+        return self._count[page]
+
     def take(self, n: int) -> List[int]:
         if n > len(self._free):
             raise OutOfPages(f"{n} pages wanted, {len(self._free)} free of {self.num_pages}")
@@ -77,6 +85,26 @@ class PagePool:
         if self._count[page] == 0:
             self._free.append(page)
 
+    def compact(self) -> Dict[int, int]:
+        """Renames the pages in use so that they come first; returns old -> new of those that move.  No
+        page is both."""
+        used = self.used_pages
+        holes = [p for p in range(used) if self._count[p] == 0]
+        moves = dict(zip((p for p in range(used, self.num_pages) if self._count[p] > 0), holes))
+        for old, new in moves.items():
+            self._count[new], self._count[old] = self._count[old], 0
+        self._free = list(range(self.num_pages - 1, used - 1, -1))
+        return moves
+
+    def resize(self, num_pages: int) -> None:
+        """The pool with another number of pages; those in use have to come first (``compact``)."""
+        used = self.used_pages
+        if num_pages <= 0 or num_pages < used or any(c for c in self._count[used:]):
+            raise OutOfPages(f"{used} pages are in use, {num_pages} are to stay")
+        self._count = (self._count + [0] * num_pages)[:num_pages]
+        self.num_pages = num_pages
+        self._free = list(range(num_pages - 1, used - 1, -1))
+
     def check(self) -> None:
         free = set(self._free)
         assert len(free) == len(self._free), "a page is in the free list twice"
@@ -93,14 +121,22 @@ class CacheGroup:
     kv: Dict[int, torch.Tensor] = field(default_factory=dict)
     state: Dict[int, torch.Tensor] = field(default_factory=dict)
     states: Dict[int, Dict[str, torch.Tensor]] = field(default_factory=dict)   # entry -> named states
+    words: Dict[int, torch.Tensor] = field(default_factory=dict)               # entry -> scales of keys and values in 8 bits
 
     @property
     def paged(self) -> bool:
         return self.pool is not None
 
     def page_bytes(self, element_size: int) -> int:
-        n = self.need
-        return n.kv_heads * (n.head_dim + n.stored_v_dim) * self.page_size * element_size * len(self.entries)
+        return self.need.page_bytes(self.page_size, element_size) * len(self.entries)
+
+    def page_tensors(self) -> List[torch.Tensor]:
+        """Everything that has a row per page."""
+        return list(self.kv.values()) + list(self.words.values())
+
+    def state_tensors(self) -> List[torch.Tensor]:
+        """Everything that has a row per request slot."""
+        return list(self.state.values()) + [t for by_name in self.states.values() for t in by_name.values()]
 
 
 class _Table:
@@ -133,9 +169,9 @@ class _Table:
     def array(self) -> np.ndarray:
         return self.pages[:self.n]
 
-    def held_below(self, block: int, first: int = 0) -> int:
-        """Pages held in blocks ``first`` .. ``block`` - 1."""
-        return int((self.pages[first:min(block, self.n)] >= 0).sum()) if block > first else 0
+    def held_below(self, block: int, first: int, pool: PagePool) -> int:
+        """Pages that blocks ``first`` .. ``block`` - 1 hold alone."""
+        return sum(p >= 0 and pool.holders(p) == 1 for p in self.pages[first:min(block, self.n)].tolist()) if block > first else 0
 
 
 @dataclass
@@ -185,7 +221,10 @@ class CacheManager:
                         grp.kv[e] = torch.zeros((grp.pool.num_pages, n.kv_heads * page_size * (n.head_dim + n.stored_v_dim)),
                                                 dtype=dtype, device=self.device)
                         continue
-                    if grp.paged and n.stored_v_dim == n.head_dim:
+                    if grp.paged and n.bits == 8:
+                        grp.kv[e] = torch.zeros((num_pages, 2, n.kv_heads, page_size, n.head_dim), dtype=torch.uint8, device=self.device)
+                        grp.words[e] = torch.zeros((num_pages, n.kv_heads, page_size // 16, 2), dtype=torch.int32, device=self.device)
+                    elif grp.paged and n.stored_v_dim == n.head_dim:
                         grp.kv[e] = torch.zeros((num_pages, 2, n.kv_heads, page_size, n.head_dim),
                                                 dtype=dtype, device=self.device)
                     elif grp.paged:     # a page holds its keys, then its values (none where the keys hold them)
@@ -273,7 +312,7 @@ class CacheManager:
             held = len(r.tables[gi]) if r else self._blocks_for(grp, have)
             need = total_blocks - held
             if r is not None and grp.need.kind in ("window", "chunk"):
-                need -= r.tables[gi].held_below(self._first_needed_block(grp, have), self._kept_blocks(grp))
+                need -= r.tables[gi].held_below(self._first_needed_block(grp, have), self._kept_blocks(grp), grp.pool)
             out[gi] = need
         return out
 
@@ -358,23 +397,115 @@ class CacheManager:
                     pool.give_back(p)
         self._free_slots.append(r.slot)
 
+    # ------------------------------------------------------------------ forks, and pages that move
+    def fork(self, req: Hashable, children: Sequence[Hashable], copy) -> None:
+        """Makes ``children`` requests that hold what ``req`` holds.  Full pages are shared; the page that ``req`` is in the
+        middle of, in every group, and its states are copied by ``copy(tensors, src rows, dst rows)`` (the operator
+        set's ``copy_pages``).  Changes nothing where slots or pages are short."""
+        r = self._requests[req]
+        children = list(children)
+        if len(set(children)) != len(children) or any(c in self._requests for c in children):
+            raise ValueError("a fork's new requests must be new, and each named once")
+        if len(children) > len(self._free_slots):
+            raise OutOfSlots(f"{len(children)} request slots wanted, {len(self._free_slots)} free")
+        open_block: Dict[int, int] = {}            # group -> the block that later tokens still write into
+        for gi, grp in enumerate(self.groups):
+            if not grp.paged:
+                continue
+            filled = r.tokens // grp.need.window if grp.need.kind == "summary" else r.tokens
+            b = filled // self.page_size
+            if filled % self.page_size and b < len(r.tables[gi]) and r.tables[gi][b] >= 0:
+                open_block[gi] = b
+                if len(children) > grp.pool.free_pages:
+                    raise OutOfPages(f"group {gi}: {len(children)} pages wanted, {grp.pool.free_pages} free")
+        if not children:
+            return
+        slots = [self._free_slots.pop() for _ in children]
+        for c, slot in zip(children, slots):
+            self._requests[c] = _Request(slot=slot, tokens=r.tokens, tables={g: _Table(self.max_blocks) for g in r.tables})
+        for gi, table in r.tables.items():
+            grp = self.groups[gi]
+            b = open_block.get(gi)
+            for i, p in enumerate(table):
+                if p >= 0 and i != b:
+                    for _ in children:
+                        grp.pool.share(p)
+            own = grp.pool.take(len(children)) if b is not None else None
+            for i, c in enumerate(children):
+                t = self._requests[c].tables[gi]
+                t.extend(list(table))
+                if own is not None:
+                    t[b] = own[i]
+            if own is not None and grp.kv:
+                copy(grp.page_tensors(), [table[b]] * len(children), own)
+        if not r.tokens:                           # (a request that has not begun has no states yet: as ``admit``)
+            for st in (st for grp in self.groups for st in grp.state.values()):
+                for slot in slots:
+                    st[slot].zero_()
+        else:
+            states = [t for grp in self.groups for t in grp.state_tensors()]
+            if states:
+                copy(states, [r.slot] * len(children), slots)
+
+    def compact(self, copy) -> Dict[int, int]:
+        """Moves the pages in use to the front of their pools; returns group -> pages moved.  What holds page numbers
+        on the device (a step's block tables) is out of date afterwards."""
+        out = {}
+        for gi, grp in enumerate(self.groups):
+            if not grp.paged:
+                continue
+            moves = grp.pool.compact()
+            out[gi] = len(moves)
+            if not moves:
+                continue
+            if grp.kv:
+                copy(grp.page_tensors(), list(moves), list(moves.values()))
+            rename = np.arange(grp.pool.num_pages, dtype=np.int32)
+            rename[list(moves)] = list(moves.values())
+            for r in self._requests.values():
+                pages = r.tables[gi].array()
+                held = pages >= 0
+                pages[held] = rename[pages[held]]
+        return out
+
+    def resize(self, num_pages: int, copy) -> None:
+        """Gives every pool ``num_pages`` pages (pools of block means what goes with them), entry by entry in new memory.  Raises
+        where more are in use."""
+        want = {gi: self.summary_pages(num_pages, grp.need.window) if grp.need.kind == "summary" else num_pages
+                for gi, grp in enumerate(self.groups) if grp.paged}
+        for gi, n in want.items():
+            if n <= 0 or n < self.groups[gi].pool.used_pages:
+                raise OutOfPages(f"group {gi}: {self.groups[gi].pool.used_pages} pages are in use, {n} are to stay")
+        self.compact(copy)
+        for gi, n in want.items():
+            grp = self.groups[gi]
+            used = grp.pool.used_pages
+            for held in (grp.kv, grp.words):
+                for e in list(held):
+                    old = held[e]
+                    held[e] = torch.zeros((n, *old.shape[1:]), dtype=old.dtype, device=old.device)
+                    held[e][:used].copy_(old[:used])
+            grp.pool.resize(n)
+
     def release_all(self) -> None:
         for req in list(self._requests):
             self.release(req)
 
     # ------------------------------------------------------------------ checks
     def check_invariants(self) -> None:
-        """No page lost, none held twice, none both free and held."""
+        """No page lost, none held by more or fewer requests than its count says, none both free and held."""
         for gi, grp in enumerate(self.groups):
             if not grp.paged:
                 continue
             grp.pool.check()
-            held: Dict[int, Hashable] = {}
+            held: Dict[int, List[Hashable]] = {}
             for req, r in self._requests.items():
                 for p in r.tables[gi]:
                     if p >= 0:
-                        assert p not in held, f"page {p} of group {gi} is held by {held[p]!r} and {req!r}"
-                        held[p] = req
+                        held.setdefault(p, []).append(req)
+                        assert len(held[p]) <= grp.pool.holders(p), f"page {p} of group {gi} is held by {held[p]}, counted {grp.pool.holders(p)} times"
+            for p, by in held.items():
+                assert len(by) == grp.pool.holders(p), f"page {p} of group {gi} is held by {by}, counted {grp.pool.holders(p)} times"
             assert len(held) == grp.pool.used_pages, (
                 f"group {gi}: {grp.pool.used_pages} pages in use but requests hold {len(held)}")
         slots = [r.slot for r in self._requests.values()]

@@ -29,6 +29,8 @@ def parse_dtype(name) -> torch.dtype:
 class EngineConfig:
     dtype: torch.dtype = torch.bfloat16
     page_size: int = 16
+    cache_bits: Optional[int] = None           # 8: keys and values are held in 8 bits with a scale per 16 positions and head (models
+                                               # whose attention reads such a cache; pages of whole sixteens); None: in ``dtype``
     max_gpu_num_blocks: Optional[int] = None   # pages per cache group; None: sized from free memory
     gpu_memory_fraction: float = 0.9           # lite_llama/executor/mem_manager.py:98-108 uses 0.9 too
     max_seq_len: int = 2048                    # longest request (prompt + generated)
@@ -48,6 +50,10 @@ class EngineConfig:
         for name in ("page_size", "max_seq_len", "max_num_seqs", "max_batched_tokens"):
             if getattr(self, name) <= 0:
                 raise ValueError(f"{name} must be positive")
+        if self.cache_bits not in (None, 8):
+            raise ValueError("cache_bits must be 8, or None for the compute type")
+        if self.cache_bits == 8 and self.page_size % 16:
+            raise ValueError(f"pages of {self.page_size} positions: an 8-bit cache has pages of whole sixteens")
         if self.max_gpu_num_blocks is not None and self.max_gpu_num_blocks <= 0:
             raise ValueError("max_gpu_num_blocks must be positive")
         self.graph_context_buckets = tuple(sorted(int(c) for c in self.graph_context_buckets))

@@ -35,6 +35,8 @@ class LayerCacheView:
     states: Dict[str, torch.Tensor] = field(default_factory=dict)   # named per-request states: [slots, *shape], float32 unless the need says otherwise
     summary_group: Optional[GroupStepView] = None   # paging data of the entry's block means (``CacheNeed.pool_block``): the slot
                                                     # of a token is where the mean of the block it completes goes (-1: it completes none)
+    words: Optional[torch.Tensor] = None            # with keys and values in 8 bits: the blocks' scales, int32 [pages, kv_heads, page_size / 16, 2];
+                                                    # ``kv`` is then uint8 [pages, 2, kv_heads, page_size, head_dim]
     summary: Optional[torch.Tensor] = None          # [pages, kv_heads * page_size * (head_dim + value_dim)], mean keys first
 
     def member(self, prefix: str) -> "LayerCacheView":
@@ -43,7 +45,7 @@ class LayerCacheView:
         cut = len(prefix) + 1
         return LayerCacheView(self.group, self.kv, self.state, self.write,
                               {k[cut:]: v for k, v in self.states.items() if k.startswith(prefix + ".")},
-                              self.summary_group, self.summary)
+                              self.summary_group, words=self.words, summary=self.summary)
 
 
 @dataclass

@@ -160,8 +160,13 @@ class Engine:
             from ..ops.cuda import CudaOps
             ops = CudaOps(self.device)
         self.ops = ops
-        self.runtime = Runtime(self.device, self.config.dtype, ops)
+        self.runtime = Runtime(self.device, self.config.dtype, ops, cache_bits=self.config.cache_bits)
         self.model = DecoderModel(spec, self.runtime)
+        if self.config.cache_bits:
+            left = [e for e, n in self.model.cache_entries().items() if n.kind != "none" and n.bits != self.config.cache_bits]
+            if left:
+                raise ValueError(f"cache_bits={self.config.cache_bits}: this model has attention that keeps its keys and values in the compute type "
+                                 f"only (cache entries {left})")
         if model_dir is not None:
             tensors = read_folder(model_dir)
             ignorable = ["lm_head.weight"] if spec.lm_head is None else []
@@ -205,7 +210,7 @@ class Engine:
         for need in entries.values():
             if need.kind in ("full", "window", "chunk"):
                 k = need.group_key()
-                per_page[k] = per_page.get(k, 0) + need.kv_heads * (need.head_dim + need.stored_v_dim) * self.config.page_size * esize
+                per_page[k] = per_page.get(k, 0) + need.page_bytes(self.config.page_size, esize)
                 if need.pool_block:      # its share of a page of block means
                     per_page[k] += -(-need.kv_heads * (need.head_dim + need.stored_v_dim) * self.config.page_size * esize // need.pool_block)
         if not per_page:
@@ -420,7 +425,7 @@ class Engine:
             grp = cache.groups[g]
             gs = cache.entry_summary_group.get(entry)
             return LayerCacheView(group=groups.get(g), kv=grp.kv.get(entry), state=grp.state.get(entry), write=write,
-                                  states=grp.states.get(entry, {}), summary_group=groups.get(gs) if gs is not None else None,
+                                  states=grp.states.get(entry, {}), words=grp.words.get(entry), summary_group=groups.get(gs) if gs is not None else None,
                                   summary=cache.groups[gs].kv.get(entry) if gs is not None else None)
         return ctx, cache_view
 
@@ -611,3 +616,43 @@ class Engine:
 
     def finish_all(self) -> None:
         self.cache.release_all()
+
+    def fork(self, request: Hashable, new_requests: Sequence[Hashable]) -> None:
+        """Makes ``new_requests`` that go on from where ``request`` is: they share its full pages and get copies of
+        the page it is in the middle of and of its states.  Raises ``OutOfSlots`` or ``OutOfPages`` and changes nothing where they
+        do not fit."""
+        self.cache.fork(request, new_requests, self.ops.copy_pages)
+
+    def compact_cache(self) -> int:
+        """Moves the pages in use to the front of their pools; returns how many moved."""
+        return sum(self.cache.compact(self.ops.copy_pages).values())
+
+    def resize_cache(self, num_pages: int) -> None:
+        """Gives the cache another number of pages per group while requests are live, so that memory can be given to something
+        else, or taken back.  Captured steps are captured again: they hold the old pages' addresses."""
+        if num_pages <= 0:
+            raise ValueError("num_pages must be positive")
+        self.cache.resize(int(num_pages), self.ops.copy_pages)
+        if self._graphs and self.device.type == "cuda":
+            torch.cuda.synchronize(self.device)
+        self._graphs.clear()
+        if self.device.type == "cuda":
+            torch.cuda.empty_cache()           # what the old pages took goes back to the device
+
+    def cached_kv(self, request: Hashable, entry: int = 0) -> torch.Tensor:
+        """The keys and values of ``request`` in a cache entry as attention reads them, [tokens, 2 (k, v), kv_heads, head_dim] in the compute
+        type; zeros where a page was given back."""
+        cache = self.cache
+        grp = cache.groups[cache.entry_group[entry]]
+        if not grp.paged or grp.need.v_dim != grp.need.head_dim or grp.need.shared_values:
+            raise ValueError(f"cache entry {entry} has no keys and values of one size")
+        n, ps = cache.tokens_of(request), cache.page_size
+        table = cache.block_table_array(request, cache.entry_group[entry])
+        if grp.need.bits == 8:
+            if n == 0:
+                return torch.empty((0, 2, grp.need.kv_heads, grp.need.head_dim), dtype=self.config.dtype, device=self.device)
+            return self.ops.read_kv8(grp.kv[entry], grp.words[entry], torch.from_numpy(table.copy())[None].to(self.device), [n], self.config.dtype)
+        pages = torch.from_numpy(table.astype(np.int64)).to(self.device)
+        kv = grp.kv[entry].view(grp.pool.num_pages, 2, grp.need.kv_heads, ps, grp.need.head_dim)[pages.clamp(min=0)]
+        kv = kv.masked_fill((pages < 0)[:, None, None, None, None], 0)
+        return kv.permute(0, 3, 1, 2, 4).flatten(0, 1)[:n]

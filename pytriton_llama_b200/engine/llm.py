@@ -10,7 +10,7 @@ safetensors files and there are no Triton kernels.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Dict, Generator, Hashable, Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -18,6 +18,7 @@ import torch
 from ..config.engine import EngineConfig
 from ..sampling.params import SamplingParams
 from ..sampling.sampler import Sampler
+from ..cache.manager import OutOfPages
 from .engine import Engine, StepEntry
 from .scheduler import PENDING, Request, Scheduler, StepPlan
 
@@ -30,6 +31,15 @@ class _Launched:
     host: Optional[torch.Tensor] = None  # int32 [2, rows]: tokens, bit patterns of the log-probabilities
     event: object = None
     logprobs: bool = False
+    scores: Optional[torch.Tensor] = None    # float32 [rows, 1 + 2 k]: ``Sampler.sample_device_scored``
+
+
+@dataclass
+class PromptScores:
+    """How a model rates a prompt: entry i is about token i + 1 after the tokens before it."""
+    logprobs: List[float] = field(default_factory=list)
+    entropies: List[float] = field(default_factory=list)              # of the distribution that the token comes from, in nats
+    top_logprobs: List[List[Tuple[int, float]]] = field(default_factory=list)   # [(token, log-probability)], best first, where asked for
 
 
 class LLM:
@@ -109,12 +119,18 @@ class LLM:
                 entries.append(StepEntry(req.id, req.tokens(p.start, p.length), [p.length - 1] if p.sample else []))
         # the plan was checked against the cache and the tokens at intake; the logits are sampled from at once
         out = self.engine.step(entries, validate=False, own_logits=False)
+        logits = out.logits
+        sampling = sum(p.sample for p in plan.portions)
+        forked = self.scheduler.fork(plan, self.engine.fork) if any(p.sample and p.request.to_fork for p in plan.portions) else []
         reqs = [p.request for p in plan.portions if p.sample]
+        if forked:        # further completions of a prompt draw their first token from its last logits
+            row = {r.id: i for i, r in enumerate(reqs[:sampling])}
+            logits = logits.index_select(0, torch.tensor([*range(sampling), *(row[parent.id] for _, parent in forked)], device=logits.device))
         launched = _Launched(plan, reqs)
         if reqs:
             n = len(reqs)
-            tokens, lp = self.sampler.sample_device(out.logits, [r.params for r in reqs], [r.number for r in reqs],
-                                                    [len(r.output) for r in reqs], out=self.engine.sampled[:n])
+            tokens, lp, scores = self.sampler.sample_device_scored(logits, [r.params for r in reqs], [r.number for r in reqs],
+                                                                   [len(r.output) for r in reqs], out=self.engine.sampled[:n])
             launched.logprobs = lp is not None
             if self.engine.device.type == "cuda":
                 launched.host, launched.event = self._staging[self._turn % len(self._staging)]
@@ -122,9 +138,13 @@ class LLM:
                 launched.host[0, :n].copy_(tokens, non_blocking=True)
                 if lp is not None:
                     launched.host[1, :n].view(torch.float32).copy_(lp, non_blocking=True)
+                if scores is not None:
+                    launched.scores = torch.empty(scores.shape, dtype=torch.float32, pin_memory=True)
+                    launched.scores.copy_(scores, non_blocking=True)
                 launched.event.record(torch.cuda.current_stream(self.engine.device))
             else:
                 launched.host = torch.stack([tokens.cpu(), (lp if lp is not None else torch.zeros(n)).cpu().view(torch.int32)])
+                launched.scores = scores
         self._rows = {r.id: i for i, r in enumerate(reqs)}
         self.scheduler.advance(plan)
         return launched
@@ -143,27 +163,91 @@ class LLM:
         if launched.logprobs:
             values = launched.host[1, :n].view(torch.float32).tolist()
             logprobs = {r.id: (v if r.params.logprobs else None) for r, v in zip(reqs, values)}
-        accepted, done = self.scheduler.resolve(launched.plan, sampled, logprobs)
+        scores = None
+        if launched.scores is not None:
+            rows = self.sampler.read_scores(launched.scores, [r.params for r in reqs])
+            scores = {r.id: s for r, s in zip(reqs, rows) if s is not None}
+        accepted, done = self.scheduler.resolve(launched.plan, sampled, logprobs, scores)
         return accepted, finished + done
 
     # ------------------------------------------------------------------ whole runs
     def generate(self, prompt_tokens: Sequence[Sequence[int]],
                  params: Union[None, SamplingParams, Sequence[SamplingParams]] = None) -> List[List[int]]:
-        """Generated token ids of every prompt (without the prompt), in the order given."""
+        """Generated token ids of every prompt (without the prompt), in the order given; with ``SamplingParams.n`` above 1 a
+        prompt's completions stand next to each other."""
         plist = self._params_list(params, len(prompt_tokens))
-        reqs = [self.add_request(p, sp) for p, sp in zip(prompt_tokens, plist)]
+        reqs = self._with_siblings([self.add_request(p, sp) for p, sp in zip(prompt_tokens, plist)])
         for _ in self.run():
             pass
         self.engine.check_device_status()
         return [list(r.output) for r in reqs]
 
+    @staticmethod
+    def _with_siblings(reqs: Sequence[Request]) -> List[Request]:
+        return [x for r in reqs for x in (r, *r.siblings)]
+
+    def score(self, prompt_tokens: Sequence[Sequence[int]], top: int = 0) -> List[PromptScores]:
+        """Rates prompts: the log-probability of every token but the first after those before it, the entropy of the
+        distribution it comes from, and with ``top`` (up to 32) that many of the most likely tokens in its place.  Prompts take
+        pages beside the requests that are live, and give them back."""
+        eng, cfg = self.engine, self.engine.config
+        if not 0 <= top <= 32:
+            raise ValueError("top must be in 0..32")
+        prompts = [[int(t) for t in p] for p in prompt_tokens]
+        for p in prompts:
+            if any(t < 0 or t >= eng.vocab_size for t in p):
+                raise ValueError(f"a prompt has a token outside the vocabulary of {eng.vocab_size}")
+            if len(p) > cfg.max_seq_len:
+                raise ValueError(f"a prompt of {len(p)} tokens; max_seq_len is {cfg.max_seq_len}")
+        out = [PromptScores() for _ in prompts]
+        room = max(1, min(cfg.max_batched_tokens, (1 << 28) // eng.vocab_size))       # rows of logits at once: up to 1 GiB of them
+        todo = [(i, 0) for i, p in enumerate(prompts) if len(p) > 1]                  # (prompt, tokens of it that have run)
+        live: List[Hashable] = []
+        try:
+            while todo:
+                entries, plan = [], []
+                left = room
+                for i, start in todo:
+                    n = min(left, len(prompts[i]) - 1 - start)
+                    key = ("score", id(out), i)
+                    asks = [(e.request, len(e.tokens)) for e in entries] + [(key, n)]
+                    if n <= 0 or not eng.cache.can_append(asks):
+                        break
+                    entries.append(StepEntry(key, prompts[i][start:start + n], list(range(n))))
+                    plan.append((i, start, n))
+                    left -= n
+                if not entries:
+                    raise OutOfPages("the cache has no room for a prompt's portion beside what is live")
+                live = list({*live, *(e.request for e in entries)})
+                logits = eng.step(entries, own_logits=False).logits
+                nxt = torch.tensor([t for i, s, n in plan for t in prompts[i][s + 1:s + n + 1]], dtype=torch.int32, device=logits.device)
+                lp, entropy, best, ids = (t.tolist() for t in eng.ops.token_scores(logits, nxt, top))
+                at = 0
+                for i, s, n in plan:
+                    out[i].logprobs += lp[at:at + n]
+                    out[i].entropies += entropy[at:at + n]
+                    if top:
+                        out[i].top_logprobs += [list(zip(a, b)) for a, b in zip(ids[at:at + n], best[at:at + n])]
+                    at += n
+                ran = {i: s + n for i, s, n in plan}
+                for i, s in list(ran.items()):
+                    if s == len(prompts[i]) - 1:
+                        eng.finish(("score", id(out), i))
+                        live.remove(("score", id(out), i))
+                todo = [(i, ran.get(i, s)) for i, s in todo if ran.get(i, s) < len(prompts[i]) - 1]
+        finally:
+            for key in live:
+                eng.finish(key)
+        eng.check_device_status()
+        return out
+
     def generate_stream(self, prompt_tokens: Sequence[Sequence[int]],
                         params: Union[None, SamplingParams, Sequence[SamplingParams]] = None
                         ) -> Generator[List[Tuple[int, List[int], bool]], None, None]:
         """Yields, after every step that produced tokens, a list of (prompt index, new token ids,
-        finished)."""
+        finished); with ``SamplingParams.n`` above 1 the index counts completions, in ``generate``'s order."""
         plist = self._params_list(params, len(prompt_tokens))
-        reqs = [self.add_request(p, sp) for p, sp in zip(prompt_tokens, plist)]
+        reqs = self._with_siblings([self.add_request(p, sp) for p, sp in zip(prompt_tokens, plist)])
         index = {r.id: i for i, r in enumerate(reqs)}
         early = [(index[r.id], [], True) for r in reqs if r.status == "finished"]
         if early:
@@ -222,13 +306,14 @@ class GenerateText(_TextMixin):
         self.device = dev
 
     def generate(self, prompt_tokens: List[List[int]], max_gen_len: Optional[int], temperature: float = 0.6,
-                 top_p: float = 0.9, echo: bool = False, logprobs: bool = False):
+                 top_p: float = 0.9, echo: bool = False, logprobs: bool = False, n: int = 1):
         """Token ids generated for each prompt, cut before the first end-of-sequence token
         (lite_llama/generate.py:192-204); with ``echo`` the prompt is put in front.  With ``logprobs``
         the result is (tokens, log-probabilities of the generated tokens), as in
-        lite_llama/generete_with_probs.py:87-96,154-165."""
-        params = SamplingParams(temperature=temperature, top_p=top_p, max_gen_len=max_gen_len, logprobs=logprobs)
-        reqs = [self.llm.add_request(p, params) for p in prompt_tokens]
+        lite_llama/generete_with_probs.py:87-96,154-165.  ``n`` completions of a prompt stand next to each other."""
+        params = SamplingParams(temperature=temperature, top_p=top_p, max_gen_len=max_gen_len, logprobs=logprobs, n=n)
+        reqs = self.llm._with_siblings([self.llm.add_request(p, params) for p in prompt_tokens])
+        prompt_tokens = [r.prompt for r in reqs]
         for _ in self.llm.run():
             pass
         self.llm.engine.check_device_status()

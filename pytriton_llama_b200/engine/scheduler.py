@@ -25,6 +25,7 @@ from collections import deque
 from dataclasses import dataclass, field
 from typing import Deque, Dict, Hashable, List, Optional
 
+from ..cache.manager import OutOfPages, OutOfSlots
 from ..sampling.params import SamplingParams
 
 WAITING, RUNNING, DRAINING, FINISHED = "waiting", "running", "draining", "finished"
@@ -39,6 +40,10 @@ class Request:
     number: int = 0                    # arrival number; also feeds the sampling counters
     output: List[int] = field(default_factory=list)
     logprobs: List[float] = field(default_factory=list)   # of the generated tokens, when asked for
+    top_logprobs: List[List[tuple]] = field(default_factory=list)   # per generated token [(token, log-probability)], best first, when asked for
+    entropies: List[float] = field(default_factory=list)  # of the distributions the tokens came from, with ``top_logprobs``
+    siblings: List["Request"] = field(default_factory=list)   # the further completions of the prompt (``SamplingParams.n``)
+    to_fork: List["Request"] = field(default_factory=list)    # those that wait for this request's prompt
     computed: int = 0                  # tokens of prompt + output that are in the cache
     status: str = WAITING
     finish_reason: Optional[str] = None
@@ -104,13 +109,50 @@ class Scheduler:
         params = params or SamplingParams()
         req = Request(request_id, list(prompt), params, number=self._counter)
         self._counter += 1
+        for i in range(1, params.n):
+            req.siblings.append(Request((request_id, i), req.prompt, params, number=self._counter))
+            self._counter += 1
+        req.to_fork = list(req.siblings)
         if not req.prompt:
             req.status, req.finish_reason = FINISHED, "empty_prompt"
         elif len(req.prompt) >= self.max_seq_len:
             req.status, req.finish_reason = FINISHED, "prompt_too_long"
         else:
             self.waiting.append(req)
+        for r in req.siblings if req.status == FINISHED else ():
+            r.status, r.finish_reason = FINISHED, req.finish_reason
         return req
+
+    def _too_small(self, req: Request, plan: "StepPlan") -> None:
+        """The cache can never hold the request, nor the completions that wait for its prompt."""
+        for r in (req, *req.to_fork):
+            r.status, r.finish_reason = FINISHED, "cache_too_small"
+            plan.finished.append(r)
+        req.to_fork = []
+
+    def fork(self, plan: "StepPlan", copies) -> List[tuple]:
+        """After the step of ``plan`` has been launched: the completions that wait for a prompt which is now in the cache go on
+        from it.  ``copies(request, new requests)`` forks the cache; where slots or pages are short the rest of them queue
+        and run the prompt themselves.  Returns (request, parent) of those that take part in the plan from here on: each
+        samples its first token from its parent's logits."""
+        out = []
+        for p in list(plan.portions):
+            if not p.sample or not p.request.to_fork:
+                continue
+            waiting, p.request.to_fork = p.request.to_fork, []
+            while waiting and len(self.running) < self.max_num_seqs and self.cache.free_slots() > 0:
+                child = waiting[0]
+                try:
+                    copies(p.request.id, [child.id])
+                except (OutOfPages, OutOfSlots):
+                    break
+                waiting.pop(0)
+                child.status, child.computed = RUNNING, p.start
+                self.running.append(child)
+                plan.portions.append(Portion(child, p.start, p.length, sample=True))
+                out.append((child, p.request))
+            self.waiting.extendleft(reversed(waiting))
+        return out
 
     def has_work(self) -> bool:
         return bool(self.waiting or self.running or self.draining)
@@ -180,8 +222,7 @@ class Scheduler:
                     elif len(self.running) == 1 and not accepted:
                         self.running.remove(req)
                         self.cache.release(req.id)
-                        req.status, req.finish_reason = FINISHED, "cache_too_small"
-                        plan.finished.append(req)
+                        self._too_small(req, plan)
                     else:
                         self._preempt(req, plan)
                     n = 0
@@ -197,8 +238,7 @@ class Scheduler:
             total = len(req.prompt) + len(req.output)
             if not self._fits_empty_cache(req, total + 1):
                 self.waiting.popleft()
-                req.status, req.finish_reason = FINISHED, "cache_too_small"
-                plan.finished.append(req)
+                self._too_small(req, plan)
                 continue
             n = min(req.pending, budget, self.max_portion)
             needs, slots = self._needs(req, n)
@@ -233,10 +273,10 @@ class Scheduler:
                 self.draining.append(req)
 
     def resolve(self, plan: StepPlan, sampled: Dict[Hashable, int],
-                logprobs: Optional[Dict[Hashable, Optional[float]]] = None):
+                logprobs: Optional[Dict[Hashable, Optional[float]]] = None, scores: Optional[Dict[Hashable, tuple]] = None):
         """The plan's tokens have been read: ``sampled`` has the new token of every portion with
-        ``sample`` set.  Returns (request id -> token for the tokens that count, requests that
-        finished); the pages of finished requests are given back here."""
+        ``sample`` set, ``scores`` (entropy, alternatives) of those that asked for them.  Returns (request id -> token for the tokens
+        that count, requests that finished); the pages of finished requests are given back here."""
         accepted: Dict[Hashable, int] = {}
         done: List[Request] = []
         for p in plan.portions:
@@ -248,6 +288,10 @@ class Scheduler:
             accepted[req.id] = tok
             if logprobs is not None and logprobs.get(req.id) is not None:
                 req.logprobs.append(float(logprobs[req.id]))
+            if scores is not None and req.id in scores:
+                entropy, best = scores[req.id]
+                req.entropies.append(entropy)
+                req.top_logprobs.append(best)
             if tok in self.eos_token_ids or tok in req.params.stop_token_ids:
                 req.finish_reason = "stop"
                 del req.output[p.out_index + 1:]

@@ -60,7 +60,7 @@ class GQAttention(Part):
 
     def cache_need(self) -> CacheNeed:
         return CacheNeed(kind="window" if self.window else "full", kv_heads=self.kv_heads,
-                         head_dim=self.head_dim, window=self.window)
+                         head_dim=self.head_dim, window=self.window, bits=self.rt.cache_bits or 0)
 
     fuses_residual = True   # forward() may add its output into the residual itself and return None
     accepts_normed = True   # x may be a norm's prepared input (the q|k|v product finishes the norm)
@@ -83,7 +83,9 @@ class GQAttention(Part):
             inv_freq, rot, whole = None, 0, None
         else:
             inv_freq, rot = table
-        if whole is not None:
+        if cache.words is not None:
+            o = self._attend_8_bits(x, qkv, ctx, cache, inv_freq, rot)
+        elif whole is not None:
             o = whole(x, self.w_qkv, ctx.positions, inv_freq, rot, g.slots, cache.kv, g.block_table, ctx.tok_req, self.heads,
                       self.kv_heads, self.head_dim, g.page_size, self.scale, window=self.window,
                       splits=ctx.attn_splits, hints=ctx, write=cache.write)
@@ -107,3 +109,16 @@ class GQAttention(Part):
                 return ops.linear_add(o, self.w_o, residual, next_norm=next_norm)
             return ops.linear_add(o, self.w_o, residual)      # None when the product's epilogue did the add
         return ops.linear(o, self.w_o)
+
+    def _attend_8_bits(self, x, qkv, ctx, cache, inv_freq, rot):
+        """The same over a cache that holds keys and values in 8 bits."""
+        ops, g = self.rt.ops, cache.group
+        if qkv is None:
+            qkv = ops.linear(x, self.w_qkv)
+        if cache.write:
+            ops.rope_kv8_write(qkv, ctx.positions, inv_freq, rot, g.slots, cache.kv, cache.words, self.heads, self.kv_heads, self.head_dim,
+                               g.page_size)
+        else:
+            ops.rope_kv_write(qkv, ctx.positions, inv_freq, rot, None, None, self.heads, self.kv_heads, self.head_dim, g.page_size)
+        return ops.paged_attention8(qkv, cache.kv, cache.words, g.block_table, ctx.tok_req, ctx.positions, self.heads, self.kv_heads, self.head_dim,
+                                    g.page_size, self.scale, window=self.window, hints=ctx)

@@ -80,7 +80,8 @@ class CacheNeed:
     the keys of positions below it stay visible, and held, whatever the window has passed.
     ``shared_values``: a key's first ``value_dim`` entries are its value; no values are stored.
     ``pool_block`` = P > 0: beside its pages of keys and values the entry keeps, in pages of their own, one mean key
-    and one mean value for every complete block of P positions of a request (never given back before the request ends)."""
+    and one mean value for every complete block of P positions of a request (never given back before the request ends).
+    ``bits`` = 8: keys and values are held in 8 bits with a scale per 16 positions and head; 0: in the compute type."""
     kind: str = "none"
     kv_heads: int = 0
     head_dim: int = 0
@@ -92,6 +93,7 @@ class CacheNeed:
     keep_first: int = 0
     shared_values: bool = False
     pool_block: int = 0
+    bits: int = 0
 
     @property
     def v_dim(self) -> int:
@@ -102,9 +104,14 @@ class CacheNeed:
         """Entries a page holds per value (0 where values are read out of the keys)."""
         return 0 if self.shared_values else self.v_dim
 
+    def page_bytes(self, page_size: int, element_size: int) -> int:
+        """Bytes of one page of one entry."""
+        values = self.kv_heads * (self.head_dim + self.stored_v_dim) * page_size
+        return values + self.kv_heads * (page_size // 16) * 8 if self.bits == 8 else values * element_size
+
     def group_key(self):
         return (self.kind, self.kv_heads, self.head_dim, self.window, self.state_shape, self.state_dtype,
-                self.value_dim, self.states, self.keep_first, self.shared_values, self.pool_block)
+                self.value_dim, self.states, self.keep_first, self.shared_values, self.pool_block, self.bits)
 
     def merged(self, other: "CacheNeed") -> "CacheNeed":
         """The need of a cache entry that ``self`` and ``other`` both read: everything either of them
@@ -127,6 +134,7 @@ class Runtime:
     device: torch.device
     dtype: torch.dtype
     ops: Any
+    cache_bits: Optional[int] = None            # 8: parts that can keep their keys and values in 8 bits do
     shared: Dict[str, torch.Tensor] = field(default_factory=dict)   # tensors of the model that parts of every layer read
 
 

@@ -14,6 +14,9 @@ class SamplingParams:
     stop_token_ids: List[int] = field(default_factory=list)
     seed: Optional[int] = None        # None: the engine's seed
     logprobs: bool = False            # also report log softmax(logits)[token] of every generated token
+    top_logprobs: int = 0             # also report that many of the most likely tokens at every step with their log-probabilities, and the
+                                      # entropy of the distribution (implies ``logprobs``; at most 32)
+    n: int = 1                        # completions of the prompt, which is run once (its pages are shared)
 
     def __post_init__(self):
         if self.temperature < 0:
@@ -22,3 +25,9 @@ class SamplingParams:
             raise ValueError("top_p must be in (0, 1]")
         if self.max_gen_len is not None and self.max_gen_len <= 0:
             raise ValueError("max_gen_len must be positive")
+        if not 0 <= self.top_logprobs <= 32:
+            raise ValueError("top_logprobs must be in 0..32")
+        if self.n < 1:
+            raise ValueError("n must be at least 1")
+        if self.top_logprobs:
+            self.logprobs = True

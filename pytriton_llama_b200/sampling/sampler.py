@@ -41,6 +41,28 @@ class Sampler:
     def sample_device(self, logits, params, request_numbers, token_indices, out=None):
         """The same without reading anything back: (int32 tokens on the device, written to ``out``
         if given; float32 log-probabilities on the device, or None if no row asks for them)."""
+        return self._draw(logits, params, request_numbers, token_indices, out, any(p.logprobs for p in params))
+
+    def sample_device_scored(self, logits, params, request_numbers, token_indices, out=None):
+        """(tokens, log-probabilities, scores): as ``sample_device``; scores, where a row asks for ``top_logprobs``, is float32
+        [rows, 1 + 2 k] on the device, k the most that a row asks for: the entropy, the k best log-probabilities, and the bits
+        of their int32 tokens."""
+        top = max((p.top_logprobs for p in params), default=0)
+        if not top:
+            return (*self.sample_device(logits, params, request_numbers, token_indices, out=out), None)
+        tokens, _ = self._draw(logits, params, request_numbers, token_indices, out, False)
+        lp, entropy, best, ids = self.ops.token_scores(logits, tokens, top)
+        return tokens, lp, torch.cat([entropy[:, None], best, ids.view(torch.float32)], 1)
+
+    @staticmethod
+    def read_scores(host: torch.Tensor, params) -> List:
+        """(entropy, [(token, log-probability), ...]) of every row of ``sample_device_scored``'s scores, once they are on the host; None
+        for rows that did not ask."""
+        k = host.shape[1] // 2
+        values, ids = host.tolist(), host[:, 1 + k:].contiguous().view(torch.int32).tolist()
+        return [(v[0], list(zip(i[:p.top_logprobs], v[1:1 + k]))) if p.top_logprobs else None for v, i, p in zip(values, ids, params)]
+
+    def _draw(self, logits, params, request_numbers, token_indices, out, logprobs: bool):
         rows = logits.shape[0]
         temperature = top_p = u = None
         if any(p.temperature > 0 for p in params):
@@ -51,7 +73,6 @@ class Sampler:
                 h[0, i], h[1, i], h[2, i] = p.temperature, p.top_p, uniform(seed, request_numbers[i], token_indices[i])
             dev = host.to(self.device, non_blocking=True)
             temperature, top_p, u = dev[0], dev[1], dev[2]
-        logprobs = any(p.logprobs for p in params)
         if hasattr(self.ops, "sample_tokens"):       # an operator set that does both at once
             return self.ops.sample_tokens(logits, temperature, top_p, u, out=out, logprobs=logprobs)
         tokens = self.ops.sample(logits, temperature, top_p, u, out=out)
