@@ -92,6 +92,10 @@ _SIGNATURES = {
     "ptl_moe_combine": [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _ptr],
     "ptl_rope_kv8_write": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ll, _ptr],
     "ptl_read_kv8": [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr],
+    "ptl_attention8_single": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                              _c_int, _c_f, _c_int, _c_int, _c_int, _ptr, _ptr, _c_int, _ptr],
+    "ptl_attention8_portion": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f, _c_int,
+                               _c_int, _ptr],
     "ptl_attention8_simt": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                             _c_int, _c_f, _c_int, _c_int, _c_int, _ptr],
     "ptl_paged_attention_simt": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int,
@@ -168,6 +172,8 @@ def load_library() -> ctypes.CDLL:
                                                     _c_int, _ptr, _ptr, _ptr, _ptr]
     lib.ptl_decode_units.argtypes = [_ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr]
     lib.ptl_decode_units.restype = _c_int
+    lib.ptl_decode_units_zeroed.argtypes = [_ptr, _ptr, _c_int, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr]
+    lib.ptl_decode_units_zeroed.restype = _c_int
     lib.ptl_decode_attention_pages_bf16.restype = _c_int
     lib.ptl_prefill_attention_bf16.argtypes = [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                                _c_int, _c_int, _c_f, _c_int, _c_int, _ptr]
@@ -977,6 +983,11 @@ class CudaOps:
         longest = getattr(hints, "max_ctx_len", 0) or block_table.shape[1] * page_size
         if window:
             longest = min(longest, window)
+        dec, tiles = self._work(hints, "decode_items"), self._work(hints, "prefill_tiles")
+        if d in (64, 128) and nq // nkv <= 16 and dec is not None and tiles is not None and q.shape[1] % 8 == 0:
+            if self._attention8_tensor_cores(out, q, codes, words, block_table, tok_req, positions, nq, nkv, d, page_size, float(scale),
+                                             int(window), longest, dec, tiles):
+                return out
         # blocks of 128 keys' turns: split until they fill the machine a few times
         splits = max(1, min(-(-longest // 256), 148 * 8 // max(1, tokens * nq), 64))
         part_acc = part_ml = None
@@ -988,6 +999,58 @@ class CudaOps:
                        q.shape[1], nq * d, block_table.shape[1], nq, nkv, d, page_size, float(scale), int(window), splits, codes.shape[0],
                        self._stream()), kernels=(2 if splits > 1 else 1) if tokens else 0)
         return out
+
+    def _attention8_tensor_cores(self, out, q, codes, words, block_table, tok_req, positions, nq, nkv, d, page_size, scale, window, longest,
+                                 dec, tiles) -> bool:
+        """Single tokens and portions by the tensor-core kernels; False where they do not take the sizes (nothing has run then)."""
+        stream, n, suffix = self._stream(), dec.items, _suffix(q.dtype)
+        if tiles.items > 65535:
+            return False
+        if n:
+            pairs = n * nkv
+            fit = self.DECODE_UNITS[d]               # blocks that fit at once
+            parts = max(1, min(8, 296 // pairs, -(-longest // 128)))
+            per_head, units, counters, part_acc, part_ml = 0, None, None, None, None
+            if (parts < 2 or longest > 1024 * parts) and pairs <= fit * 7 // 8 and longest > 64:
+                per_head = max(fit // nkv, n)
+                units, counters = self._decode8_unit_list(dec, tok_req, positions, q.shape[0], nq, nkv, d, window, per_head)
+                per_head = per_head if units is not None else 0
+                parts = 1
+            if per_head:
+                part_acc = self.empty((nkv * per_head, nq // nkv, d), torch.float32)
+                part_ml = self.empty((nkv * per_head, nq // nkv, 2), torch.float32)
+            rc = getattr(self.lib, "ptl_attention8_single" + suffix)(
+                _p(out), _p(part_acc), _p(part_ml), _p(q), _p(codes), _p(words), _p(block_table), None if dec.in_order else _p(dec.tensor),
+                _p(tok_req), _p(positions), n, q.shape[1], nq * d, block_table.shape[1], nq, nkv, d, page_size, scale, window, parts, per_head,
+                _p(units), _p(counters), codes.shape[0], stream)
+            if rc == -2:
+                return False
+            self._check(rc)
+        if tiles.items:
+            rc = getattr(self.lib, "ptl_attention8_portion" + suffix)(
+                _p(out), _p(q), _p(codes), _p(words), _p(block_table), _p(tiles.tensor), tiles.items, q.shape[1], nq * d, block_table.shape[1],
+                nq, nkv, d, page_size, scale, window, codes.shape[0], stream)
+            self._check(rc)
+        return True
+
+    def _decode8_unit_list(self, dec, tok_req, positions, rows: int, nq: int, nkv: int, d: int, window: int, per_head: int):
+        """(the units of the step's single tokens, their counters, zero): as ``_decode_unit_list``, with counters that belong to the list."""
+        memo = getattr(self, "_units8_memo", None)
+        stream = self._stream()
+        integers, key = (dec.tensor, tok_req, positions), None
+        if memo is not None and not any(t.is_inference() for t in integers):
+            key = (stream, dec.items, dec.in_order, *(x for t in integers for x in (t.data_ptr(), t._version)), rows, nq, nkv, d, int(window), per_head)
+            if key in memo:
+                return memo[key][:2]
+        units, counters = self.empty((nkv * per_head, 8), torch.int32), self.empty((rows * nkv,), torch.int32)
+        rc = self.lib.ptl_decode_units_zeroed(_p(units), _p(counters), counters.numel(), None if dec.in_order else _p(dec.tensor), _p(tok_req),
+                                              _p(positions), dec.items, nq, nkv, d, int(window), per_head, stream)
+        if rc == -2:
+            return None, None
+        self._check(rc)
+        if key is not None:
+            memo[key] = (units, counters, *integers)         # (held, so that their addresses are not given out again)
+        return units, counters
 
     # ------------------------------------------------------------------ pages
     def copy_pages(self, tensors, src, dst) -> None:
@@ -1027,12 +1090,12 @@ class CudaOps:
     def begin_forward(self) -> None:
         """Called by the model at the start of every forward pass: what was worked out for the last
         step's positions (the tables of rotary angles, the units of single tokens) is forgotten."""
-        self._rope_memo, self._pair_memo, self._units_memo = {}, {}, {}
+        self._rope_memo, self._pair_memo, self._units_memo, self._units8_memo = {}, {}, {}, {}
 
     def end_forward(self) -> None:
         """Called at the end of every forward pass: calls outside of one work their tables and units out themselves.  One kept from
         such a call to the next would be missing from a graph that captures the second of them."""
-        self._rope_memo = self._pair_memo = self._units_memo = None
+        self._rope_memo = self._pair_memo = self._units_memo = self._units8_memo = None
 
     def _pair_angles(self, positions: torch.Tensor, freq: torch.Tensor, dims: int, amplitude: float) -> torch.Tensor:
         """(cos, sin) [tokens, dims/2, 2] of position * freq, worked out once per forward pass and stream for every table of
