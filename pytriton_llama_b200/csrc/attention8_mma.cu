@@ -4,32 +4,34 @@
 //   q . k = s_k 2^e (x . c + sum(x) / 2),        sum_j p_j v_j = sum over blocks of s_v (sum p_j c_j + sum p_j / 2):
 // the two products run on half floats with float32 sums, a block's step is a float32 factor of its 16 keys' scores and of its 16
 // keys' part of the output, and the halves cost one float32 sum a row.  x is a half float exactly for bfloat16 q (but for entries
-// below 2^-14 of the row's largest, which lose bits below 2^-24 of it); weights p <= 1 are rounded to half floats, 2^-11 of each.
+// below 2^-14 of the row's largest, which lose bits below 2^-24 of it); weights are rounded to half floats, 2^-11 of each.
 // float32 rows take two half floats each, x = x1 + x2 and p = p1 + p2, and twice the products.
 //
-// No shared memory on the way in.  For m16n8k16 the 16 dimensions of a step and the 8 columns of a value product may be any, as long
-// as both operands agree, so they are chosen for the loads: lane (g, c) reads 16 bytes of key g's row at 16 c, which are its operand
-// of four steps, and D / 8 bytes of value rows 2c, 2c + 1, 2c + 8, 2c + 9 at g D / 8, which are its operand of D / 8 products.  A
-// byte becomes half float 1024 + u by one byte permutation, and 1024 + u - 1152 = c exactly.  A warp asks for the next keys as soon as
-// it has multiplied this turn's, and for the next values likewise, so loads run under the other half of the turn.
+// Keys and values are the rows of m16n8k16's first operand (S^T = C_k X^T, O^T = C_v^T P^T): 8 query rows fill the other side, where
+// they would leave half of the first one empty, and what is made of the codes serves as many tiles of 8 rows as a warp has.
+// The 16 dimensions of a step and the 16 rows of a value product may be any, as long as both sides agree, so they are chosen for the
+// loads: lane (g, c) reads 16 bytes of key rows g and g + 8 at 16 c, which are its operand of four steps, and D / 8 bytes of value
+// rows 2c, 2c + 1, 2c + 8, 2c + 9 at g D / 8, which are its operand of D / 16 products.  A pair of bytes becomes 1024 + u by one
+// byte permutation, and 1024 + u - 1152 = c exactly.  Weights come out of the scores' layout by an 8 x 8 transposition.
 //
-// Rows of a tile: the heads of the group for one token, or for as many tokens of a portion as fit 16 rows.  Two ways of sharing:
-// - single tokens (SINGLE): the four warps of a block take turns through the keys of one (token, kv head), or of a part of them, and
-//   join through shared memory.  Parts of one (token, kv head) join in a cluster, or, where the contexts are cut into parts of equal
-//   length (the list of decode_units_kernel), in the block that ends last.
-// - portions: a warp has a tile of its own; the block's warps have neighbouring ones, which read the same keys out of L1.
+// A row's reference maximum only moves when a score is above it by more than 2^8: the comparison is one vote a turn, and
+// the reduction over the keys' lanes and the rescaling of the output happen a few times a row.
+//
+// Keys and values of 16 positions and a head are 16 D bytes each in one piece, and come by bulk copies into rings of slots in shared memory.
+// Waits for them are bounded: one that gives up says so in *status, and the block ends once its copies have.
 #include "kv8.cuh"
-#include "mma_utils.cuh"
+#include "tcgen05_utils.cuh"
 
 namespace ptl {
 
 constexpr int kA8Warps = 4;
+constexpr int kA8Turn = 2;                                    // blocks of 16 keys a turn
 
 struct A8Params {
   void* out;
   float* part_acc;            // [blocks][G][D]
   float* part_ml;             // [blocks][G][2], in units of log2
-  int* counters;              // a zero per (item, kv head)
+  int* counters;              // a zero per (row, kv head)
   const void* q;
   const unsigned char* codes;
   const uint32_t* words;
@@ -38,8 +40,23 @@ struct A8Params {
   const int* tok_req;
   const int* positions;
   const int4* units;
+  int* status;
   int q_stride, out_stride, bt_stride, nq, nkv, blocks_per_page, page_shift, num_pages, window, splits, cluster;
   float scale_log2;
+
+  __device__ __forceinline__ int page_of(const int* table, int block) const {
+    const int pg = page_shift >= 0 ? block >> page_shift : block / blocks_per_page;
+    const int page = pg < bt_stride ? __ldg(table + pg) : -1;
+    return page < num_pages ? page : -1;
+  }
+  __device__ __forceinline__ int sub_of(int block) const { return page_shift >= 0 ? block & (blocks_per_page - 1) : block % blocks_per_page; }
+  template <int D> __device__ __forceinline__ const unsigned char* keys(int page, int kvh, int sub) const {
+    return codes + (((size_t)page * 2 * nkv + kvh) * blocks_per_page + sub) * (kKv8Block * D);
+  }
+  template <int D> __device__ __forceinline__ size_t plane() const { return (size_t)nkv * blocks_per_page * (kKv8Block * D); }
+  __device__ __forceinline__ uint2 word(int page, int kvh, int sub) const {
+    return __ldg(reinterpret_cast<const uint2*>(words) + ((size_t)page * nkv + kvh) * blocks_per_page + sub);
+  }
 };
 
 __device__ __forceinline__ float a8_exp2(float x) {
@@ -47,15 +64,19 @@ __device__ __forceinline__ float a8_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Bytes `sel` picks, two of them, as half floats u - 128.
-__device__ __forceinline__ uint32_t a8_pair(uint32_t bytes, uint32_t sel) {
-  uint32_t x, y;
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(x) : "r"(bytes), "r"(0x64646464u), "r"(sel));      // 1024 + u
-  asm("sub.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x64806480u));
+__device__ __forceinline__ uint32_t a8_prmt(uint32_t a, uint32_t b, uint32_t sel) {
+  uint32_t x;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(x) : "r"(a), "r"(b), "r"(sel));
+  return x;
+}
+// Bytes 0 and 1 (HIGH: 2 and 3), as half floats u - 128.
+template <bool HIGH> __device__ __forceinline__ uint32_t a8_pair(uint32_t bytes) {
+  uint32_t y;
+  asm("sub.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a8_prmt(bytes, 0x64646464u, HIGH ? 0x4342u : 0x4140u)), "r"(0x64806480u));
   return y;
 }
 __device__ __forceinline__ uint32_t a8_pack(float lo, float hi) {
@@ -66,46 +87,46 @@ __device__ __forceinline__ uint32_t a8_pack(float lo, float hi) {
 __device__ __forceinline__ void a8_unpack(uint32_t v, float& lo, float& hi) {
   asm("{\n.reg .f16 a, b;\nmov.b32 {a, b}, %2;\ncvt.f32.f16 %0, a;\ncvt.f32.f16 %1, b;\n}" : "=f"(lo), "=f"(hi) : "r"(v));
 }
-template <int BYTES> __device__ __forceinline__ void a8_load(uint32_t (&r)[BYTES / 4], const unsigned char* p) {
-  if constexpr (BYTES == 16) {
-    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "l"(p));
-  } else {
-    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
-  }
+// The transposed 8 x 8 matrix of 16-bit elements of a warp.
+__device__ __forceinline__ uint32_t a8_transpose(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 __device__ __forceinline__ float ld_peer_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
 
-// Rows per warp: 16 (WIDE) or 8, the upper half of the product's rows then being zeros.
-template <int D, typename T, bool WIDE> struct A8Warp {
+// NT tiles of 8 query rows in a warp.  Lane (g, c) holds, of the rows 8 n + 2c and 8 n + 2c + 1 (j = 0, 1), their statistics and the output's
+// dimensions g D / 8 .. (g + 1) D / 8 - 1.
+template <int D, typename T, int NT> struct A8Rows {
   static constexpr int kParts = sizeof(T) == 4 ? 2 : 1;
-  static constexpr int kHalves = WIDE ? 2 : 1;
-  static constexpr int kChunks = D / 64;                     // 16-byte pieces of a key row a lane takes
-  static constexpr int kTurn = D == 64 ? 2 : 1;              // blocks of 16 keys a turn
-  static constexpr int kTiles = D / 8;                       // value products
-  uint32_t qa[kParts][kChunks * 4][2 * kHalves];
-  float half_sum[kHalves];                                   // sum(x) / 2
-  float factor[kHalves];                                     // 2^e scale log2(e)
-  int first[kHalves], last[kHalves];                         // positions a row sees
-  float o[kTiles][2 * kHalves];
-  float m[kHalves], l[kHalves], w[kHalves];
+  static constexpr int kSteps = D / 16;
+  uint32_t qb[kParts][kSteps][NT][2];
+  float half_sum[NT][2];                                     // sum(x) / 2
+  float factor[NT][2];                                       // 2^e scale log2(e)
+  int first[NT][2], last[NT][2];                             // positions a row sees
+  float o[kSteps][NT][4];                                    // dimension 2 i + (e >> 1) of the lane's, row j = e & 1
+  float m[NT][2], l[NT][2], w[NT][2];                        // reference maximum (log2), and the lane's sums of p and of p s_v
 
-  // Row `row` of the tile is query head head0 + row % group of token t0 + row / group.
-  __device__ __forceinline__ void load_rows(const A8Params& p, int t0, int tokens, int pos0, int kvh, int group) {
+  // Row `row` of the warp's is query head kvh * group + row % group of token t0 + row / group.
+  __device__ __forceinline__ void load(const A8Params& p, int t0, int tokens, int pos0, int kvh, int group) {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-      const int row = g + 8 * h;
+    for (int n = 0; n < NT; ++n) {
+      const int row = 8 * n + g;
       const bool here = row < tokens * group;
-      const int token = here ? row / group : 0;
-      float x[kChunks][16];
-      const T* src = static_cast<const T*>(p.q) + (size_t)(t0 + token) * p.q_stride + (size_t)(kvh * group + (here ? row % group : 0)) * D + 16 * c;
+      float x[kSteps / 4][16];
+      const T* src = static_cast<const T*>(p.q) + (size_t)(t0 + (here ? row / group : 0)) * p.q_stride + (size_t)(kvh * group + (here ? row % group : 0)) * D + 16 * c;
       float big = 0.f;
 #pragma unroll
-      for (int k = 0; k < kChunks; ++k)
+      for (int k = 0; k < kSteps / 4; ++k)
 #pragma unroll
         for (int i = 0; i < 16; i += Vec16<T>::N) {
           Vec16<T> v;
@@ -118,13 +139,12 @@ template <int D, typename T, bool WIDE> struct A8Warp {
         }
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      // 2^e with |x| < 2; the powers of two that 1 / 2^e can be
+      // 2^e with |x| < 2, within the powers of two whose inverse is a normal number
       const uint32_t e = min(max(__float_as_uint(big) >> 23, 2u), 252u);
-      const float scale = __uint_as_float(e << 23), inverse = __uint_as_float((254u - e) << 23);
-      factor[h] = scale * p.scale_log2;
+      const float inverse = __uint_as_float((254u - e) << 23);
       float sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < kChunks; ++k)
+      for (int k = 0; k < kSteps / 4; ++k)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -136,226 +156,227 @@ template <int D, typename T, bool WIDE> struct A8Warp {
               float fa, fb;
               a8_unpack(half, fa, fb);
               sum += fa + fb;
-              qa[part][4 * k + i][j * kHalves + h] = half;
+              qb[part][4 * k + i][n][j] = half;
               a -= fa; b -= fb;
             }
           }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      half_sum[h] = 0.5f * sum;
-      last[h] = here ? pos0 + token : -1;
-      first[h] = p.window > 0 && last[h] + 1 > p.window ? last[h] + 1 - p.window : 0;
-      m[h] = -INFINITY; l[h] = 0.f; w[h] = 0.f;
+      const float f = __uint_as_float(e << 23) * p.scale_log2;
 #pragma unroll
-      for (int n = 0; n < kTiles; ++n) { o[n][2 * h] = 0.f; o[n][2 * h + 1] = 0.f; }
+      for (int j = 0; j < 2; ++j) {                          // row 8 n + 2c + j is held by the lanes of g = 2c + j here
+        half_sum[n][j] = 0.5f * __shfl_sync(0xffffffffu, sum, 4 * (2 * c + j));
+        factor[n][j] = __shfl_sync(0xffffffffu, f, 4 * (2 * c + j));
+        const int r = 8 * n + 2 * c + j;
+        last[n][j] = r < tokens * group ? pos0 + r / group : -1;
+        first[n][j] = p.window > 0 && last[n][j] + 1 > p.window ? last[n][j] + 1 - p.window : 0;
+        m[n][j] = -INFINITY; l[n][j] = 0.f; w[n][j] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+        for (int x2 = 0; x2 < 4; ++x2) o[i][n][x2] = 0.f;
     }
   }
 
-  // Blocks begin, begin + stride, ... of kTurn blocks of 16 positions each, below `end`, of request r.  Rows with every position of
-  // [all_first, all_last] in sight are not masked there.
-  __device__ __forceinline__ void walk(const A8Params& p, int r, int kvh, int begin, int stride, int end, int all_first, int all_last) {
+  // kA8Turn blocks of 16 keys: their keys at slot[b], their values 16 D bytes further, their words, and their first positions.  Positions
+  // of [all_first, all_last] are in every row's sight.
+  __device__ __forceinline__ void turn(const unsigned char* const (&slot)[kA8Turn], const bool (&have)[kA8Turn], const uint2 (&word)[kA8Turn],
+                                       const int (&key0)[kA8Turn], int all_first, int all_last) {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int page_size = p.blocks_per_page * kKv8Block;
-    const size_t plane = (size_t)p.nkv * page_size * D;
-    const int* table = p.block_table + (size_t)r * p.bt_stride;
-    const unsigned char* at[kTurn];
-    uint2 word[kTurn], word_next[kTurn];
-    bool have[kTurn], have_next[kTurn];
-    uint32_t k[kTurn][2][kChunks][4], v[kTurn][4][D / 32];
-    int page[kTurn];
-    auto look_up = [&](int i) {
+    float s[kA8Turn][NT][4];
+    float f[kA8Turn][NT][2];
 #pragma unroll
-      for (int b = 0; b < kTurn; ++b) {
-        const int blk = i + b, pg = p.page_shift >= 0 ? blk >> p.page_shift : blk / p.blocks_per_page;
-        page[b] = blk < end && pg < p.bt_stride ? __ldg(table + pg) : -1;
-      }
-    };
-    auto load_keys = [&](int i) {
+    for (int b = 0; b < kA8Turn; ++b) {
 #pragma unroll
-      for (int b = 0; b < kTurn; ++b) {
-        const int blk = i + b, sub = p.page_shift >= 0 ? blk & ((1 << p.page_shift) - 1) : blk % p.blocks_per_page;
-        have_next[b] = page[b] >= 0 && page[b] < p.num_pages;
-        if (!have_next[b]) { word_next[b] = make_uint2(0u, 0u); continue; }
-        at[b] = p.codes + (size_t)page[b] * 2 * plane + ((size_t)kvh * page_size + sub * kKv8Block) * D;
-        word_next[b] = __ldg(reinterpret_cast<const uint2*>(p.words + (((size_t)page[b] * p.nkv + kvh) * p.blocks_per_page + sub) * 2));
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int e = 0; e < 4; ++e) s[b][n][e] = half_sum[n][e & 1];
+      const float step = 2.0f * kv8_half_step(word[b].x & 255u);
 #pragma unroll
-          for (int h = 0; h < kChunks; ++h) a8_load<16>(k[b][n][h], at[b] + (n * 8 + g) * D + h * 64 + 16 * c);
-      }
-    };
-    auto load_values = [&]() {
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int b = 0; b < kTurn; ++b)
-        if (have[b]) {
+        for (int j = 0; j < 2; ++j) f[b][n][j] = fmaxf(factor[n][j] * step, 1e-37f);       // (0 times the -inf of a masked key is none)
+      if (have[b]) {
+        const uint4* k = reinterpret_cast<const uint4*>(slot[b]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) a8_load<D / 8>(v[b][j], at[b] + plane + ((j >> 1) * 8 + 2 * c + (j & 1)) * D + g * (D / 8));
-        }
-    };
-    look_up(begin);
-    load_keys(begin);
+        for (int h = 0; h < D / 64; ++h) {
+          const uint4 k0 = k[g * (D / 16) + 4 * h + c], k1 = k[(g + 8) * (D / 16) + 4 * h + c];
+          const uint32_t x0[4] = {k0.x, k0.y, k0.z, k0.w}, x1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
-    for (int b = 0; b < kTurn; ++b) { word[b] = word_next[b]; have[b] = have_next[b]; }
-    load_values();
-    look_up(begin + stride);
-    for (int i = begin; i < end; i += stride) {
-      float s[kTurn][2][2 * kHalves];
-#pragma unroll
-      for (int b = 0; b < kTurn; ++b) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          float acc[4] = {half_sum[0], half_sum[0], half_sum[kHalves - 1], half_sum[kHalves - 1]};
-          if (have[b]) {
-#pragma unroll
-            for (int h = 0; h < kChunks; ++h)
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                const uint32_t b0 = a8_pair(k[b][n][h][x], 0x4140u), b1 = a8_pair(k[b][n][h][x], 0x4342u);
-#pragma unroll
-                for (int part = 0; part < kParts; ++part) {
-                  const uint32_t(&a)[2 * kHalves] = qa[part][4 * h + x];
-                  mma_f16_16816(acc, a[0], WIDE ? a[kHalves - 1] : 0u, a[kHalves], WIDE ? a[2 * kHalves - 1] : 0u, b0, b1);
-                }
-              }
-          }
-          const float step = 2.0f * kv8_half_step(word[b].x & 255u);
-#pragma unroll
-          for (int h = 0; h < kHalves; ++h) {
-            s[b][n][2 * h] = acc[2 * h] * (factor[h] * step);
-            s[b][n][2 * h + 1] = acc[2 * h + 1] * (factor[h] * step);
-          }
-        }
-        const int key0 = (i + b) * kKv8Block;
-        if (key0 < all_first || key0 + kKv8Block - 1 > all_last || !have[b] || ((word[b].x | word[b].y) >> 16)) {
-          const uint32_t marks = (word[b].x | word[b].y) >> 16;
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 2 * kHalves; ++e) {
-              const int off = n * 8 + 2 * c + (e & 1), key = key0 + off;
-              if ((marks >> off) & 1u) s[b][n][e] = __uint_as_float(0x7fc00000u);
-              if (key < first[e >> 1] || key > last[e >> 1] || !have[b]) s[b][n][e] = -INFINITY;
-            }
-        }
-      }
-      // this turn's keys are used: the next ones
-      float vstep[kTurn];
-      bool held[kTurn];
-#pragma unroll
-      for (int b = 0; b < kTurn; ++b) { vstep[b] = 2.0f * kv8_half_step(word[b].y & 255u); held[b] = have[b]; }
-      if (i + stride < end) {
-        load_keys(i + stride);
-        look_up(i + 2 * stride);
-      }
-      uint32_t pa[kParts][kTurn][2][kHalves];
-      bool moved = false;
-      float alpha[kHalves];
-#pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        float mx = m[h];
-#pragma unroll
-        for (int b = 0; b < kTurn; ++b)
-          mx = fmaxf(mx, fmaxf(fmaxf(s[b][0][2 * h], s[b][0][2 * h + 1]), fmaxf(s[b][1][2 * h], s[b][1][2 * h + 1])));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float use = mx == -INFINITY ? 0.f : mx;
-        alpha[h] = a8_exp2(m[h] - use);
-        moved |= mx > m[h];
-        m[h] = mx;
-        float sum = 0.f, wsum = 0.f;
-#pragma unroll
-        for (int b = 0; b < kTurn; ++b) {
-          float pr[2][2], part_sum = 0.f;
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            pr[n][0] = a8_exp2(s[b][n][2 * h] - use);
-            pr[n][1] = a8_exp2(s[b][n][2 * h + 1] - use);
-            part_sum += pr[n][0] + pr[n][1];
-#pragma unroll
-            for (int part = 0; part < kParts; ++part) {
-              const uint32_t half = a8_pack(pr[n][0], pr[n][1]);
-              pa[part][b][n][h] = half;
-              if (part + 1 < kParts) {
-                float fa, fb;
-                a8_unpack(half, fa, fb);
-                pr[n][0] -= fa; pr[n][1] -= fb;
-              }
-            }
-          }
-          sum += part_sum;
-          wsum = fmaf(part_sum, vstep[b], wsum);
-        }
-        l[h] = fmaf(l[h], alpha[h], sum);
-        w[h] = fmaf(w[h], alpha[h], wsum);
-      }
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-          for (int e = 0; e < 2 * kHalves; ++e) o[n][e] *= alpha[e >> 1];
-      }
-#pragma unroll
-      for (int b = 0; b < kTurn; ++b) {
-        if (!held[b]) continue;
-#pragma unroll
-        for (int x = 0; x < D / 32; ++x) {
-          // four bytes of each of four value rows -> the operands of four products
-          uint32_t lo[2], hi[2];
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            asm("prmt.b32 %0, %1, %2, %3;" : "=r"(lo[n]) : "r"(v[b][2 * n][x]), "r"(v[b][2 * n + 1][x]), "r"(0x5140u));
-            asm("prmt.b32 %0, %1, %2, %3;" : "=r"(hi[n]) : "r"(v[b][2 * n][x]), "r"(v[b][2 * n + 1][x]), "r"(0x7362u));
-          }
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const uint32_t sel = y & 1 ? 0x4342u : 0x4140u;
-            const uint32_t b0 = a8_pair(y < 2 ? lo[0] : hi[0], sel), b1 = a8_pair(y < 2 ? lo[1] : hi[1], sel);
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t a[4] = {a8_pair<false>(x0[i]), a8_pair<false>(x1[i]), a8_pair<true>(x0[i]), a8_pair<true>(x1[i])};
 #pragma unroll
             for (int part = 0; part < kParts; ++part)
-              mma_f16_16816(acc, pa[part][b][0][0], WIDE ? pa[part][b][0][kHalves - 1] : 0u, pa[part][b][1][0],
-                            WIDE ? pa[part][b][1][kHalves - 1] : 0u, b0, b1);
 #pragma unroll
-            for (int e = 0; e < 2 * kHalves; ++e) o[4 * x + y][e] = fmaf(acc[e], vstep[b], o[4 * x + y][e]);
+              for (int n = 0; n < NT; ++n) mma_f16_16816(s[b][n], a, qb[part][4 * h + i][n][0], qb[part][4 * h + i][n][1]);
           }
         }
       }
-      if (i + stride < end) {
+      const uint32_t marks = (word[b].x | word[b].y) >> 16;
+      if (!have[b] || key0[b] < all_first || key0[b] + kKv8Block - 1 > all_last || marks) {
 #pragma unroll
-        for (int b = 0; b < kTurn; ++b) { word[b] = word_next[b]; have[b] = have_next[b]; }
-        load_values();
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int off = g + 8 * (e >> 1), key = key0[b] + off;
+            if ((marks >> off) & 1u) s[b][n][e] = __uint_as_float(0x7fc00000u);
+            if (!have[b] || key < first[n][e & 1] || key > last[n][e & 1]) s[b][n][e] = -INFINITY;
+          }
+      }
+    }
+    // the largest score of the lane's keys above a row's reference by more than 8 moves the reference
+    float top[NT][2];
+    bool above = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        top[n][j] = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < kA8Turn; ++b) top[n][j] = fmaxf(top[n][j], fmaxf(s[b][n][j], s[b][n][2 + j]) * f[b][n][j]);
+        above |= top[n][j] > m[n][j] + 8.0f;
+      }
+    if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float alpha[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float mx = fmaxf(top[n][j], m[n][j]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          alpha[j] = mx == -INFINITY ? 1.0f : a8_exp2(m[n][j] - mx);
+          m[n][j] = mx;
+          l[n][j] *= alpha[j];
+          w[n][j] *= alpha[j];
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][n][e] *= alpha[e & 1];
+      }
+    }
+    uint32_t pb[kParts][kA8Turn][NT][2];
+    float vstep[kA8Turn];
+#pragma unroll
+    for (int b = 0; b < kA8Turn; ++b) {
+      vstep[b] = 2.0f * kv8_half_step(word[b].y & 255u);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float pr[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float use = m[n][e & 1] == -INFINITY ? 0.f : m[n][e & 1];
+          pr[e] = a8_exp2(fmaf(s[b][n][e], f[b][n][e & 1], -use));
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float sum = pr[j] + pr[2 + j];
+          l[n][j] += sum;
+          w[n][j] = fmaf(sum, vstep[b], w[n][j]);
+        }
+#pragma unroll
+        for (int part = 0; part < kParts; ++part)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t half = a8_pack(pr[2 * x], pr[2 * x + 1]);
+            pb[part][b][n][x] = a8_transpose(half);
+            if (part + 1 < kParts) {
+              float fa, fb;
+              a8_unpack(half, fa, fb);
+              pr[2 * x] -= fa; pr[2 * x + 1] -= fb;
+            }
+          }
       }
     }
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
+    for (int b = 0; b < kA8Turn; ++b) {
+      if (!have[b]) continue;
+      uint32_t v[4][D / 32];
 #pragma unroll
-      for (int x = 1; x <= 2; x <<= 1) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], x);
-        w[h] += __shfl_xor_sync(0xffffffffu, w[h], x);
+      for (int r = 0; r < 4; ++r) {
+        const unsigned char* row = slot[b] + kKv8Block * D + ((r >> 1) * 8 + 2 * c + (r & 1)) * D + g * (D / 8);
+        if constexpr (D == 64) {
+          const uint2 x = *reinterpret_cast<const uint2*>(row);
+          v[r][0] = x.x; v[r][1] = x.y;
+        } else {
+          const uint4 x = *reinterpret_cast<const uint4*>(row);
+          v[r][0] = x.x; v[r][1] = x.y; v[r][2] = x.z; v[r][3] = x.w;
+        }
       }
 #pragma unroll
-      for (int n = 0; n < kTiles; ++n) { o[n][2 * h] += 0.5f * w[h]; o[n][2 * h + 1] += 0.5f * w[h]; }
+      for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          // two bytes of each of the four rows: rows 2c and 2c + 1 side by side, then the other two
+          const uint32_t lo = a8_prmt(v[0][x], v[1][x], y ? 0x7362u : 0x5140u), hi = a8_prmt(v[2][x], v[3][x], y ? 0x7362u : 0x5140u);
+          const uint32_t a[4] = {a8_pair<false>(lo), a8_pair<true>(lo), a8_pair<false>(hi), a8_pair<true>(hi)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) mma_f16_16816(acc, a, pb[part][b][n][0], pb[part][b][n][1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[2 * x + y][n][e] = fmaf(acc[e], vstep[b], o[2 * x + y][n][e]);
+          }
+        }
     }
   }
-  // Lane (g, c) holds, of row g + 8 h, the dimensions c D / 4 + (0 .. D / 4 - 1): this is entry `i` of them.
-  __device__ __forceinline__ float entry(int h, int i) const { return o[i % kTiles][2 * h + i / kTiles]; }
+
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int x = 4; x <= 16; x <<= 1) {
+          l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], x);
+          w[n][j] += __shfl_xor_sync(0xffffffffu, w[n][j], x);
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) { o[i][n][j] += 0.5f * w[n][j]; o[i][n][2 + j] += 0.5f * w[n][j]; }
+      }
+  }
+  // Entry `i` of the lane's D / 8 dimensions of row 8 n + 2c + j.
+  __device__ __forceinline__ float entry(int n, int j, int i) const { return o[i / 2][n][2 * (i % 2) + j]; }
 };
 
 // What a row's weight sum l and a part's (m, l) give: parts without keys count nothing, a sum that is no number stays one.
 __device__ __forceinline__ float a8_weight(float m, float l, float M) { return l == 0.f ? 0.f : a8_exp2(m - M); }
 __device__ __forceinline__ float a8_inverse(float l) { return l == 0.f ? 0.f : 1.0f / l; }
 
-template <int D, typename T, bool WIDE>
-__global__ void __launch_bounds__(kA8Warps * 32, D == 64 && !WIDE ? 4 : 1)
+template <int D, int NT> struct A8Single {
+  static constexpr int kRing = D == 64 ? 6 : 4;                            // slots a warp has
+  static constexpr int kSlot = 2 * kKv8Block * D;
+  static constexpr int kRingBytes = kA8Warps * kRing * kSlot;
+  static constexpr int kJoinBytes = kA8Warps * 8 * NT * (D + 2) * 4 + 8 * NT * (D + 2) * 4;      // the warps' rows, and the block's: where the rings were
+  static constexpr int kSmem = kRingBytes > kJoinBytes ? kRingBytes : kJoinBytes;
+};
+
+// Single tokens: the four warps of a block take turns through the keys of one (token, kv head), or of a part of them, and join
+// through shared memory.  The parts of a (token, kv head) join in a cluster, or, where the contexts are cut into parts of equal
+// length (the list of decode_units_kernel), in the block that ends last.  Every warp fetches its own keys, kRing blocks ahead.
+template <int D, typename T, int NT>
+__global__ void __launch_bounds__(kA8Warps * 32, NT == 1 && sizeof(T) == 2 ? (D == 64 ? 4 : 3) : 1)
 attention8_single_kernel(const A8Params p) {
-  using W = A8Warp<D, T, WIDE>;
-  constexpr int kRows = WIDE ? 16 : 8;
-  __shared__ float s_o[kA8Warps][kRows][D], s_m[kA8Warps][kRows], s_l[kA8Warps][kRows];
-  __shared__ float s_part[kRows * D], s_pm[kRows], s_pl[kRows];
+  using Cfg = A8Single<D, NT>;
+  constexpr int kRows = 8 * NT, kRing = Cfg::kRing;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ __align__(8) uint64_t s_full[kA8Warps][kRing];
   __shared__ int s_last;
+  __shared__ volatile int s_abort;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const uint32_t full0 = smem_addr(&s_full[warp][0]);
+  if (lane == 0) {
+    for (int i = 0; i < kRing; ++i) mbar_init(full0 + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (tid == 0) s_abort = 0;
+  __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int group = p.nq / p.nkv;
   T* out = static_cast<T*>(p.out);
   int t, r, pos, kvh, split, splits, pair;
@@ -382,19 +403,86 @@ attention8_single_kernel(const A8Params p) {
   }
   const int lo = p.window > 0 && pos + 1 > p.window ? pos + 1 - p.window : 0;
   const int b0 = lo / kKv8Block, blocks = pos < 0 ? 0 : pos / kKv8Block - b0 + 1;
-  const int per = ((blocks + splits - 1) / splits + W::kTurn - 1) / W::kTurn * W::kTurn;
+  const int per = (blocks + splits - 1) / splits;
   const int begin = b0 + min(blocks, split * per), end = b0 + min(blocks, (split + 1) * per);
-  W w;
-  w.load_rows(p, t, 1, pos, kvh, group);
-  w.walk(p, r, kvh, begin + warp * W::kTurn, kA8Warps * W::kTurn, end, lo, pos);
-#pragma unroll
-  for (int h = 0; h < W::kHalves; ++h) {
-    const int row = g + 8 * h;
-#pragma unroll
-    for (int i = 0; i < D / 4; i += 4)
-      *reinterpret_cast<float4*>(&s_o[warp][row][c * (D / 4) + i]) = make_float4(w.entry(h, i), w.entry(h, i + 1), w.entry(h, i + 2), w.entry(h, i + 3));
-    if (c == 0) { s_m[warp][row] = w.m[h]; s_l[warp][row] = w.l[h]; }
+  // ---- this warp's blocks: begin + warp + 4 i, i < count.  A lane looks up every 32nd of them: its page, and its words
+  const int count = max(0, (end - begin - warp + kA8Warps - 1) / kA8Warps);
+  const int* table = p.block_table + (size_t)r * p.bt_stride;
+  auto block_at = [&](int i) { return begin + warp + kA8Warps * i; };
+  auto page_at = [&](int i) { return i < count ? p.page_of(table, block_at(i)) : -1; };
+  auto word_at = [&](int i, int page) { return page >= 0 ? p.word(page, kvh, p.sub_of(block_at(i))) : make_uint2(0u, 0u); };
+  const uint32_t slot0 = smem_addr(smem) + warp * (kRing * Cfg::kSlot);
+  auto fetch = [&](int i, int page) {                         // (lane 0) block i into its slot
+    const uint32_t bar = full0 + 8 * (i % kRing), dst = slot0 + (i % kRing) * Cfg::kSlot;
+    if (page < 0) { mbar_arrive(bar); return; }
+    mbar_expect_tx(bar, Cfg::kSlot);
+    const unsigned char* src = p.keys<D>(page, kvh, p.sub_of(block_at(i)));
+    bulk_load(dst, src, Cfg::kSlot / 2, bar);
+    bulk_load(dst + Cfg::kSlot / 2, src + p.plane<D>(), Cfg::kSlot / 2, bar);
+  };
+  int page_cur = page_at(lane), page_nxt = page_at(32 + lane);
+  for (int i = 0; i < min(kRing, count); ++i) {
+    const int page = __shfl_sync(0xffffffffu, page_cur, i);
+    if (lane == 0) fetch(i, page);
   }
+  uint2 word_cur = word_at(lane, page_cur);
+  A8Rows<D, T, NT> rows;
+  rows.load(p, t, 1, pos, kvh, group);
+  int gave_up = -1;                                           // the block whose wait ran out
+  for (int base = 0; base < count; base += 32) {
+    const uint2 word_nxt = word_at(base + 32 + lane, page_nxt);
+    const int page_nn = page_at(base + 64 + lane);
+    const int stop = min(32, count - base);
+    for (int i = 0; i < stop; i += kA8Turn) {
+      const unsigned char* slot[kA8Turn];
+      bool have[kA8Turn];
+      uint2 word[kA8Turn];
+      int key0[kA8Turn];
+#pragma unroll
+      for (int b = 0; b < kA8Turn; ++b) {
+        const int at = base + i + b;
+        word[b].x = __shfl_sync(0xffffffffu, word_cur.x, i + b);
+        word[b].y = __shfl_sync(0xffffffffu, word_cur.y, i + b);
+        have[b] = __shfl_sync(0xffffffffu, page_cur, i + b) >= 0;        // (false behind the last block)
+        key0[b] = block_at(at) * kKv8Block;
+        slot[b] = smem + warp * (kRing * Cfg::kSlot) + (at % kRing) * Cfg::kSlot;
+        if (i + b < stop && gave_up < 0 &&
+            !__all_sync(0xffffffffu, mbar_wait(full0 + 8 * (at % kRing), (at / kRing) & 1, &s_abort, p.status, 9))) gave_up = at;
+      }
+      if (gave_up >= 0) break;
+      rows.turn(slot, have, word, key0, lo, pos);
+      __syncwarp();                                           // the slots are read: their next blocks
+#pragma unroll
+      for (int b = 0; b < kA8Turn; ++b) {
+        const int ahead = i + b + kRing;
+        const int page = __shfl_sync(0xffffffffu, ahead < 32 ? page_cur : page_nxt, ahead & 31);
+        if (lane == 0 && i + b < stop && base + ahead < count) fetch(base + ahead, page);
+      }
+    }
+    if (gave_up >= 0) break;
+    page_cur = page_nxt; page_nxt = page_nn; word_cur = word_nxt;
+  }
+  if (gave_up >= 0)                                           // this warp's copies still under way end before the memory is used for something else
+    for (int i = gave_up; i < min(gave_up + kRing, count); ++i) mbar_drain(full0 + 8 * (i % kRing), (i / kRing) & 1);
+  rows.finish();
+  __syncthreads();                                            // the rings are read
+  float(*s_o)[kRows][D] = reinterpret_cast<float(*)[kRows][D]>(smem);
+  float(*s_m)[kRows] = reinterpret_cast<float(*)[kRows]>(smem + kA8Warps * kRows * D * 4);
+  float(*s_l)[kRows] = s_m + kA8Warps;
+  float* s_part = reinterpret_cast<float*>(s_l + kA8Warps);
+  float* s_pm = s_part + kRows * D;
+  float* s_pl = s_pm + kRows;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int row = 8 * n + 2 * c + j;
+#pragma unroll
+      for (int i = 0; i < D / 8; i += 4)
+        *reinterpret_cast<float4*>(&s_o[warp][row][g * (D / 8) + i]) =
+            make_float4(rows.entry(n, j, i), rows.entry(n, j, i + 1), rows.entry(n, j, i + 2), rows.entry(n, j, i + 3));
+      if (g == 0) { s_m[warp][row] = rows.m[n][j]; s_l[warp][row] = rows.l[n][j]; }
+    }
   __syncthreads();
   const bool whole = splits == 1;
   for (int e = tid; e < group * D; e += kA8Warps * 32) {
@@ -426,7 +514,7 @@ attention8_single_kernel(const A8Params p) {
     __syncwarp();
     cluster_arrive();
     cluster_wait();
-    const uint32_t at_o = smem_u32(s_part), at_m = smem_u32(s_pm), at_l = smem_u32(s_pl);
+    const uint32_t at_o = smem_addr(s_part), at_m = smem_addr(s_pm), at_l = smem_addr(s_pl);
     const int share = (group * D + splits - 1) / splits;
     for (int e = split * share + tid; e < min(group * D, (split + 1) * share); e += kA8Warps * 32) {
       const int row = e / D;
@@ -484,40 +572,134 @@ attention8_single_kernel(const A8Params p) {
   }
 }
 
+// Portions: a warp has rows of its own, the heads of the group for as many neighbouring tokens as fit 8 NT rows; the block's warps have
+// neighbouring ones and read the same keys out of one ring of slots (a turn's kA8Turn blocks each) that a fifth warp keeps filled.
+template <int D, typename T> struct A8Portion {
+  static constexpr int kTiles = D == 64 ? (sizeof(T) == 2 ? 4 : 2) : 2;
+  static constexpr int kRing = 4;
+  static constexpr int kSlot = kA8Turn * 2 * kKv8Block * D;
+  static constexpr int kSmem = kRing * kSlot;
+};
+
 template <int D, typename T>
-__global__ void __launch_bounds__(kA8Warps * 32)
+__global__ void __launch_bounds__((kA8Warps + 1) * 32)
 attention8_portion_kernel(const A8Params p) {
-  using W = A8Warp<D, T, true>;
+  using Cfg = A8Portion<D, T>;
+  constexpr int NT = Cfg::kTiles, kRing = Cfg::kRing;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ __align__(8) uint64_t s_full[kRing], s_empty[kRing];
+  __shared__ uint2 s_word[kRing][kA8Turn];
+  __shared__ int s_have[kRing][kA8Turn];
+  __shared__ volatile int s_abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const uint32_t full0 = smem_addr(s_full), empty0 = smem_addr(s_empty);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kRing; ++i) { mbar_init(full0 + 8 * i, 1); mbar_init(empty0 + 8 * i, kA8Warps); }
+    s_abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
-  const int group = p.nq / p.nkv, per_tile = 16 / group;      // tokens of a warp
+  const int group = p.nq / p.nkv, per_warp = 8 * NT / group, per_block = per_warp * kA8Warps;      // tokens
   const int kvh = blockIdx.x % p.nkv;
-  const int tile = gridDim.y - 1 - blockIdx.y;                // the last rows of a portion see the most keys: first
-  const int* tl = p.items + 4 * tile;
-  const int sub = (blockIdx.x / p.nkv) * kA8Warps + (threadIdx.x >> 5);
-  const int begin = sub * per_tile, tokens = min(per_tile, tl[2] - begin);
+  const int* tl = p.items + 4 * (gridDim.y - 1 - blockIdx.y);   // the last rows of a portion see the most keys: first
+  const int sub = gridDim.x / p.nkv - 1 - blockIdx.x / p.nkv;
+  const int tokens = min(per_block, tl[2] - sub * per_block);
   if (tokens <= 0) return;
-  const int t0 = tl[1] + begin, pos0 = tl[3] + begin, last = pos0 + tokens - 1;
+  const int t0 = tl[1] + sub * per_block, pos0 = tl[3] + sub * per_block;
   const int lo = p.window > 0 && pos0 + 1 > p.window ? pos0 + 1 - p.window : 0;
-  const int lo_last = p.window > 0 && last + 1 > p.window ? last + 1 - p.window : 0;
-  W w;
-  w.load_rows(p, t0, tokens, pos0, kvh, group);
-  w.walk(p, tl[0], kvh, lo / kKv8Block, W::kTurn, last / kKv8Block + 1, lo_last, pos0);
-  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int row = g + 8 * h;
-    if (row >= tokens * group) continue;
-    const float inv = a8_inverse(w.l[h]);
-    T* dst = static_cast<T*>(p.out) + (size_t)(t0 + row / group) * p.out_stride + (size_t)(kvh * group + row % group) * D + c * (D / 4);
-#pragma unroll
-    for (int i = 0; i < D / 4; i += Vec16<T>::N) {
-      Vec16<T> v;
-#pragma unroll
-      for (int j = 0; j < Vec16<T>::N; ++j) v.set(j, w.entry(h, i + j) * inv);
-      store16(dst + i, v);
+  const int begin = lo / kKv8Block, end = (pos0 + tokens - 1) / kKv8Block + 1;
+  const int turns = (end - begin + kA8Turn - 1) / kA8Turn;
+  if (warp == kA8Warps) {
+    // ---- the slots: lane 0 fetches, the lanes look ahead for the pages of 32 blocks
+    const int* table = p.block_table + (size_t)tl[0] * p.bt_stride;
+    int page = -1;
+    uint2 word = make_uint2(0u, 0u);
+    for (int i = 0; i < turns; ++i) {
+      const int b32 = i * kA8Turn % 32;
+      if (b32 == 0) {
+        const int block = begin + i * kA8Turn + lane;
+        page = block < end ? p.page_of(table, block) : -1;
+        word = page >= 0 ? p.word(page, kvh, p.sub_of(block)) : make_uint2(0u, 0u);
+      }
+      const int s = i % kRing;
+      if (!__all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, ((i / kRing) & 1) ^ 1, &s_abort, p.status, 9))) {
+        for (int k = max(0, i - kRing); k < i; ++k) mbar_drain(full0 + 8 * (k % kRing), (k / kRing) & 1);
+        return;
+      }
+      const bool mine = lane >= b32 && lane < b32 + kA8Turn;
+      if (mine) { s_word[s][lane - b32] = word; s_have[s][lane - b32] = page >= 0; }
+      const unsigned got = __ballot_sync(0xffffffffu, mine && page >= 0);
+      __syncwarp();
+      const uint32_t bar = full0 + 8 * s;
+      if (lane == 0) mbar_expect_tx(bar, __popc(got) * 2 * kKv8Block * D);      // (its arrival publishes the words)
+      __syncwarp();
+      if (mine && page >= 0) {
+        const unsigned char* src = p.keys<D>(page, kvh, p.sub_of(begin + i * kA8Turn + lane - b32));
+        const uint32_t dst = smem_addr(smem) + s * Cfg::kSlot + (lane - b32) * 2 * kKv8Block * D;
+        bulk_load(dst, src, kKv8Block * D, bar);
+        bulk_load(dst + kKv8Block * D, src + p.plane<D>(), kKv8Block * D, bar);
+      }
+      __syncwarp();
     }
+    return;
   }
+  const int my_tokens = min(per_warp, tokens - warp * per_warp);
+  const int my_t0 = t0 + warp * per_warp, my_pos0 = pos0 + warp * per_warp, my_last = my_pos0 + my_tokens - 1;
+  const int my_lo = p.window > 0 && my_pos0 + 1 > p.window ? my_pos0 + 1 - p.window : 0;
+  const int all_first = p.window > 0 && my_last + 1 > p.window ? my_last + 1 - p.window : 0;
+  A8Rows<D, T, NT> rows;
+  rows.load(p, my_t0, max(0, my_tokens), my_pos0, kvh, group);
+  for (int i = 0; i < turns; ++i) {
+    const int s = i % kRing, first_key = (begin + i * kA8Turn) * kKv8Block;
+    if (!__all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, (i / kRing) & 1, &s_abort, p.status, 9))) {
+      for (int k = i; k < min(i + kRing, turns); ++k) mbar_drain(full0 + 8 * (k % kRing), (k / kRing) & 1);
+      return;
+    }
+    if (my_tokens > 0 && first_key <= my_last && first_key + kA8Turn * kKv8Block > my_lo) {
+      const unsigned char* slot[kA8Turn];
+      bool have[kA8Turn];
+      uint2 word[kA8Turn];
+      int key0[kA8Turn];
+#pragma unroll
+      for (int b = 0; b < kA8Turn; ++b) {
+        slot[b] = smem + s * Cfg::kSlot + b * 2 * kKv8Block * D;
+        have[b] = s_have[s][b];
+        word[b] = s_word[s][b];
+        key0[b] = first_key + b * kKv8Block;
+      }
+      rows.turn(slot, have, word, key0, all_first, my_pos0);
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty0 + 8 * s);
+  }
+  rows.finish();
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int row = 8 * n + 2 * c + j;
+      if (row >= my_tokens * group) continue;
+      const float inv = a8_inverse(rows.l[n][j]);
+      T* dst = static_cast<T*>(p.out) + (size_t)(my_t0 + row / group) * p.out_stride + (size_t)(kvh * group + row % group) * D + g * (D / 8);
+#pragma unroll
+      for (int i = 0; i < D / 8; i += Vec16<T>::N) {
+        Vec16<T> v;
+#pragma unroll
+        for (int x = 0; x < Vec16<T>::N; ++x) v.set(x, rows.entry(n, j, i + x) * inv);
+        store16(dst + i, v);
+      }
+    }
+}
+
+template <int D, typename T, int NT>
+static int launch_single(const A8Params& p, unsigned blocks, cudaStream_t stream) {
+  using Cfg = A8Single<D, NT>;
+  static SmemRaised raised = {};
+  if (int rc = raise_shared_memory("attention8_single", attention8_single_kernel<D, T, NT>, Cfg::kSmem, raised)) return rc;
+  return launch_kernel_cluster("attention8_single", attention8_single_kernel<D, T, NT>, dim3(blocks), dim3(kA8Warps * 32), Cfg::kSmem, stream,
+                               p.cluster ? p.splits : 1, p);
 }
 
 template <int D, typename T>
@@ -526,11 +708,14 @@ static int launch_attention8(const A8Params& p, int singles, int tiles, int per_
   if (singles) {
     const long long blocks = per_head ? (long long)p.nkv * per_head : (long long)singles * p.nkv * p.splits;
     PTL_REQUIRE(blocks <= 0x7fffffffLL, "attention8: too many blocks");
-    auto kernel = group <= 8 ? attention8_single_kernel<D, T, false> : attention8_single_kernel<D, T, true>;
-    return launch_kernel_cluster("attention8_single", kernel, dim3((unsigned)blocks), dim3(kA8Warps * 32), 0, stream, p.cluster ? p.splits : 1, p);
+    return group <= 8 ? launch_single<D, T, 1>(p, (unsigned)blocks, stream) : launch_single<D, T, 2>(p, (unsigned)blocks, stream);
   }
-  const int per_tile = 16 / group, blocks_of_tile = ((128 + per_tile - 1) / per_tile + kA8Warps - 1) / kA8Warps;
-  return launch_kernel("attention8_portion", attention8_portion_kernel<D, T>, dim3(p.nkv * blocks_of_tile, tiles), dim3(kA8Warps * 32), 0, stream, p);
+  using Cfg = A8Portion<D, T>;
+  static SmemRaised raised = {};
+  if (int rc = raise_shared_memory("attention8_portion", attention8_portion_kernel<D, T>, Cfg::kSmem, raised)) return rc;
+  const int per_block = 8 * Cfg::kTiles / group * kA8Warps;
+  return launch_kernel("attention8_portion", attention8_portion_kernel<D, T>, dim3(p.nkv * ((128 + per_block - 1) / per_block), tiles),
+                       dim3((kA8Warps + 1) * 32), Cfg::kSmem, stream, p);
 }
 
 template <typename T>
@@ -543,7 +728,7 @@ static int attention8_mma(A8Params p, int singles, int tiles, int d, int page_si
               "attention8: q, out and codes must be 16-byte and words 8-byte aligned");
   PTL_REQUIRE(p.splits >= 1 && (!p.cluster || p.splits <= 8), "attention8: a cluster has up to 8 parts");
   PTL_REQUIRE(per_head == 0 || (p.units && aligned16(p.units) && p.counters && p.part_acc && p.part_ml), "attention8: units need their list and scratch");
-  PTL_REQUIRE(per_head != 0 || p.splits == 1 || p.cluster, "attention8: parts of a token join in a cluster or are listed as units");
+  PTL_REQUIRE(p.status != nullptr, "attention8: needs a status word");
   p.blocks_per_page = page_size / kKv8Block;
   p.page_shift = -1;
   for (int b = 0; b < 20; ++b) if ((1 << b) == p.blocks_per_page) p.page_shift = b;
@@ -556,22 +741,23 @@ static int attention8_mma(A8Params p, int singles, int tiles, int d, int page_si
 // Single tokens: `items` their rows (null: 0..n_items-1).  With per_head > 0 the keys are dealt out in units (`units` from
 // ptl_decode_units_zeroed with the same sizes and with `counters`, one int per (row, kv head) of q), part_acc [nkv * per_head, nq / nkv, d] and part_ml
 // [..., 2]; else every (token, kv head) has `splits` parts, up to 8, which join in a cluster.  -2: sizes this kernel does not take.
+// *status: raised when a wait for a copy gave up.
 #define PTL_ATTENTION8_MMA(NAME, T)                                                                                                         \
   PTL_EXPORT int ptl_attention8_single_##NAME(void* out, float* part_acc, float* part_ml, const void* q, const void* codes,                 \
                                               const void* words, const int* block_table, const int* items, const int* tok_req,             \
                                               const int* positions, int n_items, int q_stride, int out_stride, int bt_stride, int nq,       \
                                               int nkv, int d, int page_size, float scale, int window, int splits, int per_head,             \
-                                              const int* units, int* counters, int num_pages, void* stream) {                               \
+                                              const int* units, int* counters, int num_pages, int* status, void* stream) {                  \
     ptl::A8Params p{out, part_acc, part_ml, counters, q, (const unsigned char*)codes, (const uint32_t*)words, block_table, items, tok_req,  \
-                    positions, (const int4*)units, q_stride, out_stride, bt_stride, nq, nkv, 0, 0, num_pages, window, splits,               \
+                    positions, (const int4*)units, status, q_stride, out_stride, bt_stride, nq, nkv, 0, 0, num_pages, window, splits,       \
                     per_head == 0 && splits > 1, scale * 1.4426950408889634f};                                                              \
     return ptl::attention8_mma<T>(p, n_items, 0, d, page_size, per_head, stream);                                                           \
   }                                                                                                                                         \
   PTL_EXPORT int ptl_attention8_portion_##NAME(void* out, const void* q, const void* codes, const void* words, const int* block_table,      \
                                                const int* tiles, int n_tiles, int q_stride, int out_stride, int bt_stride, int nq, int nkv, \
-                                               int d, int page_size, float scale, int window, int num_pages, void* stream) {                \
+                                               int d, int page_size, float scale, int window, int num_pages, int* status, void* stream) {   \
     ptl::A8Params p{out, nullptr, nullptr, nullptr, q, (const unsigned char*)codes, (const uint32_t*)words, block_table, tiles, nullptr,    \
-                    nullptr, nullptr, q_stride, out_stride, bt_stride, nq, nkv, 0, 0, num_pages, window, 1, 0,                              \
+                    nullptr, nullptr, status, q_stride, out_stride, bt_stride, nq, nkv, 0, 0, num_pages, window, 1, 0,                      \
                     scale * 1.4426950408889634f};                                                                                           \
     return ptl::attention8_mma<T>(p, 0, n_tiles, d, page_size, 0, stream);                                                                  \
   }

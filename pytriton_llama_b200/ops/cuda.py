@@ -93,9 +93,9 @@ _SIGNATURES = {
     "ptl_rope_kv8_write": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ll, _ptr],
     "ptl_read_kv8": [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr],
     "ptl_attention8_single": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
-                              _c_int, _c_f, _c_int, _c_int, _c_int, _ptr, _ptr, _c_int, _ptr],
+                              _c_int, _c_f, _c_int, _c_int, _c_int, _ptr, _ptr, _c_int, _ptr, _ptr],
     "ptl_attention8_portion": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f, _c_int,
-                               _c_int, _ptr],
+                               _c_int, _ptr, _ptr],
     "ptl_attention8_simt": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                             _c_int, _c_f, _c_int, _c_int, _c_int, _ptr],
     "ptl_paged_attention_simt": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int,
@@ -1022,14 +1022,14 @@ class CudaOps:
             rc = getattr(self.lib, "ptl_attention8_single" + suffix)(
                 _p(out), _p(part_acc), _p(part_ml), _p(q), _p(codes), _p(words), _p(block_table), None if dec.in_order else _p(dec.tensor),
                 _p(tok_req), _p(positions), n, q.shape[1], nq * d, block_table.shape[1], nq, nkv, d, page_size, scale, window, parts, per_head,
-                _p(units), _p(counters), codes.shape[0], stream)
+                _p(units), _p(counters), codes.shape[0], _p(self._tc_status_word()), stream)
             if rc == -2:
                 return False
             self._check(rc)
         if tiles.items:
             rc = getattr(self.lib, "ptl_attention8_portion" + suffix)(
                 _p(out), _p(q), _p(codes), _p(words), _p(block_table), _p(tiles.tensor), tiles.items, q.shape[1], nq * d, block_table.shape[1],
-                nq, nkv, d, page_size, scale, window, codes.shape[0], stream)
+                nq, nkv, d, page_size, scale, window, codes.shape[0], _p(self._tc_status_word()), stream)
             self._check(rc)
         return True
 
