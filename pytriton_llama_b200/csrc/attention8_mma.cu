@@ -14,6 +14,10 @@
 // rows 2c, 2c + 1, 2c + 8, 2c + 9 at g D / 8, which are its operand of D / 16 products.  A pair of bytes becomes 1024 + u by one
 // byte permutation, and 1024 + u - 1152 = c exactly.  Weights come out of the scores' layout by an 8 x 8 transposition.
 //
+// Warps of several tiles of rows sum the output in units of the largest value step so far, 2^(E - 133), by the products themselves: weights
+// carry 2^(E_b - E) of their block.  A block whose step is more than 2^8 smaller, where such a weight would leave the half floats'
+// normal numbers, is multiplied by itself and added with its step, as every block of a warp of one tile is.
+//
 // A row's reference maximum only moves when a score is above it by more than 2^8: the comparison is one vote a turn, and
 // the reduction over the keys' lanes and the rescaling of the output happen a few times a row.
 //
@@ -64,9 +68,16 @@ __device__ __forceinline__ float a8_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// 2^k, 0 below the normal numbers.
+__device__ __forceinline__ float a8_power(int k) { return k < -126 ? 0.f : __uint_as_float((uint32_t)(127 + k) << 23); }
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same, to `c` and not to what is in d.
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 __device__ __forceinline__ uint32_t a8_prmt(uint32_t a, uint32_t b, uint32_t sel) {
   uint32_t x;
@@ -114,29 +125,40 @@ template <int D, typename T, int NT> struct A8Rows {
   int first[NT][2], last[NT][2];                             // positions a row sees
   float o[kSteps][NT][4];                                    // dimension 2 i + (e >> 1) of the lane's, row j = e & 1
   float m[NT][2], l[NT][2], w[NT][2];                        // reference maximum (log2), and the lane's sums of p and of p s_v
+  static constexpr bool kUnits = NT > 1;
+  int unit;                                                  // kUnits: E of the step that o and w are counted in
 
-  // Row `row` of the warp's is query head kvh * group + row % group of token t0 + row / group.
-  __device__ __forceinline__ void load(const A8Params& p, int t0, int tokens, int pos0, int kvh, int group) {
+  // Row `row` of the warp's is query head kvh * group + row % group of token t0 + row / group.  `fetch` asks for what `load` works on.
+  static constexpr int kRaw = D / 4 / Vec16<T>::N;           // packets of a row a lane holds
+  struct Raw { Vec16<T> v[NT][kRaw]; };
+  __device__ __forceinline__ static void fetch(Raw& raw, const A8Params& p, int t0, int tokens, int kvh, int group) {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int row = 8 * n + g;
       const bool here = row < tokens * group;
-      float x[kSteps / 4][16];
       const T* src = static_cast<const T*>(p.q) + (size_t)(t0 + (here ? row / group : 0)) * p.q_stride + (size_t)(kvh * group + (here ? row % group : 0)) * D + 16 * c;
+#pragma unroll
+      for (int i = 0; i < kRaw; ++i) {
+        constexpr int kPer = 16 / Vec16<T>::N;
+        if (here) raw.v[n][i] = load16(src + 64 * (i / kPer) + i % kPer * Vec16<T>::N);
+        else
+#pragma unroll
+          for (int j = 0; j < Vec16<T>::N; ++j) raw.v[n][i].set(j, 0.f);
+      }
+    }
+  }
+  __device__ __forceinline__ void load(const Raw& raw, const A8Params& p, int tokens, int pos0, int group) {
+    const int lane = threadIdx.x & 31, c = lane & 3;
+    unit = 0;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      auto x = [&](int k, int i) { return raw.v[n][(16 * k + i) / Vec16<T>::N].get(i % Vec16<T>::N); };
       float big = 0.f;
 #pragma unroll
       for (int k = 0; k < kSteps / 4; ++k)
 #pragma unroll
-        for (int i = 0; i < 16; i += Vec16<T>::N) {
-          Vec16<T> v;
-          if (here) v = load16(src + 64 * k + i);
-#pragma unroll
-          for (int j = 0; j < Vec16<T>::N; ++j) {
-            x[k][i + j] = here ? v.get(j) : 0.f;
-            big = fmaxf(big, fabsf(x[k][i + j]));
-          }
-        }
+        for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(x(k, i)));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
       // 2^e with |x| < 2, within the powers of two whose inverse is a normal number
@@ -149,7 +171,7 @@ template <int D, typename T, int NT> struct A8Rows {
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float a = x[k][4 * i + 2 * j] * inverse, b = x[k][4 * i + 2 * j + 1] * inverse;
+            float a = x(k, 4 * i + 2 * j) * inverse, b = x(k, 4 * i + 2 * j + 1) * inverse;
 #pragma unroll
             for (int part = 0; part < kParts; ++part) {
               const uint32_t half = a8_pack(a, b);
@@ -188,10 +210,6 @@ template <int D, typename T, int NT> struct A8Rows {
     float f[kA8Turn][NT][2];
 #pragma unroll
     for (int b = 0; b < kA8Turn; ++b) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[b][n][e] = half_sum[n][e & 1];
       const float step = 2.0f * kv8_half_step(word[b].x & 255u);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -209,7 +227,12 @@ template <int D, typename T, int NT> struct A8Rows {
 #pragma unroll
             for (int part = 0; part < kParts; ++part)
 #pragma unroll
-              for (int n = 0; n < NT; ++n) mma_f16_16816(s[b][n], a, qb[part][4 * h + i][n][0], qb[part][4 * h + i][n][1]);
+              for (int n = 0; n < NT; ++n) {
+                if (h == 0 && i == 0 && part == 0)
+                  mma_f16_16816(s[b][n], a, qb[0][0][n][0], qb[0][0][n][1], half_sum[n][0], half_sum[n][1], half_sum[n][0], half_sum[n][1]);
+                else
+                  mma_f16_16816(s[b][n], a, qb[part][4 * h + i][n][0], qb[part][4 * h + i][n][1]);
+              }
           }
         }
       }
@@ -221,7 +244,7 @@ template <int D, typename T, int NT> struct A8Rows {
           for (int e = 0; e < 4; ++e) {
             const int off = g + 8 * (e >> 1), key = key0[b] + off;
             if ((marks >> off) & 1u) s[b][n][e] = __uint_as_float(0x7fc00000u);
-            if (!have[b] || key < first[n][e & 1] || key > last[n][e & 1]) s[b][n][e] = -INFINITY;
+            if (!have[b] || key < first[n][e & 1] || key > last[n][e & 1]) s[b][n][e] = -INFINITY;      // (without its keys a block has no scores yet)
           }
       }
     }
@@ -258,24 +281,46 @@ template <int D, typename T, int NT> struct A8Rows {
           for (int e = 0; e < 4; ++e) o[i][n][e] *= alpha[e & 1];
       }
     }
+    int ev[kA8Turn];
+#pragma unroll
+    for (int b = 0; b < kA8Turn; ++b) ev[b] = (int)(word[b].y & 255u);
+    if constexpr (kUnits) {
+      // the unit follows the largest value step; a block far below it keeps its own
+      int e_max = unit;
+#pragma unroll
+      for (int b = 0; b < kA8Turn; ++b) e_max = max(e_max, ev[b]);
+      if (e_max > unit) {
+        const float f2 = unit == 0 ? 0.f : a8_power(unit - e_max);      // (nothing but zeros so far: o and w are 0)
+        unit = e_max;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          w[n][0] *= f2; w[n][1] *= f2;
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][n][e] *= f2;
+        }
+      }
+    }
     uint32_t pb[kParts][kA8Turn][NT][2];
-    float vstep[kA8Turn];
+    float apart[kA8Turn];                                    // the factor of a block that is multiplied by itself
+    bool own[kA8Turn];
 #pragma unroll
     for (int b = 0; b < kA8Turn; ++b) {
-      vstep[b] = 2.0f * kv8_half_step(word[b].y & 255u);
+      own[b] = !kUnits || ev[b] + 8 < unit;
+      apart[b] = !kUnits ? 2.0f * kv8_half_step(ev[b]) : ev[b] == 0 ? 0.f : a8_power(ev[b] - unit);
+      const float up = own[b] ? 1.0f : a8_power(unit - ev[b]), down = own[b] ? apart[b] : 1.0f, shift = own[b] ? 0.f : (float)(ev[b] - unit);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float pr[4];
+        const float use[2] = {(m[n][0] == -INFINITY ? 0.f : m[n][0]) - shift, (m[n][1] == -INFINITY ? 0.f : m[n][1]) - shift};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float use = m[n][e & 1] == -INFINITY ? 0.f : m[n][e & 1];
-          pr[e] = a8_exp2(fmaf(s[b][n][e], f[b][n][e & 1], -use));
-        }
+        for (int e = 0; e < 4; ++e) pr[e] = a8_exp2(fmaf(s[b][n][e], f[b][n][e & 1], -use[e & 1]));
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const float sum = pr[j] + pr[2 + j];
-          l[n][j] += sum;
-          w[n][j] = fmaf(sum, vstep[b], w[n][j]);
+          l[n][j] = kUnits ? fmaf(sum, up, l[n][j]) : l[n][j] + sum;
+          w[n][j] = fmaf(sum, down, w[n][j]);
         }
 #pragma unroll
         for (int part = 0; part < kParts; ++part)
@@ -306,26 +351,41 @@ template <int D, typename T, int NT> struct A8Rows {
           v[r][0] = x.x; v[r][1] = x.y; v[r][2] = x.z; v[r][3] = x.w;
         }
       }
+      // two bytes of each of the four rows: rows 2c and 2c + 1 side by side, then the other two
+      auto operand = [&](int x, int y, uint32_t (&a)[4]) {
+        const uint32_t lo = a8_prmt(v[0][x], v[1][x], y ? 0x7362u : 0x5140u), hi = a8_prmt(v[2][x], v[3][x], y ? 0x7362u : 0x5140u);
+        a[0] = a8_pair<false>(lo); a[1] = a8_pair<true>(lo); a[2] = a8_pair<false>(hi); a[3] = a8_pair<true>(hi);
+      };
+      if (kUnits && !own[b]) {
 #pragma unroll
-      for (int x = 0; x < D / 32; ++x)
+        for (int i = 0; i < kSteps; ++i) {
+          uint32_t a[4];
+          operand(i / 2, i % 2, a);
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          // two bytes of each of the four rows: rows 2c and 2c + 1 side by side, then the other two
-          const uint32_t lo = a8_prmt(v[0][x], v[1][x], y ? 0x7362u : 0x5140u), hi = a8_prmt(v[2][x], v[3][x], y ? 0x7362u : 0x5140u);
-          const uint32_t a[4] = {a8_pair<false>(lo), a8_pair<true>(lo), a8_pair<false>(hi), a8_pair<true>(hi)};
+          for (int part = 0; part < kParts; ++part)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16_16816(o[i][n], a, pb[part][b][n][0], pb[part][b][n][1]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          uint32_t a[4];
+          operand(i / 2, i % 2, a);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            float acc[4];
+            mma_f16_16816(acc, a, pb[0][b][n][0], pb[0][b][n][1], 0.f, 0.f, 0.f, 0.f);
+            if (kParts == 2) mma_f16_16816(acc, a, pb[kParts - 1][b][n][0], pb[kParts - 1][b][n][1]);
 #pragma unroll
-            for (int part = 0; part < kParts; ++part) mma_f16_16816(acc, a, pb[part][b][n][0], pb[part][b][n][1]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[2 * x + y][n][e] = fmaf(acc[e], vstep[b], o[2 * x + y][n][e]);
+            for (int e = 0; e < 4; ++e) o[i][n][e] = fmaf(acc[e], apart[b], o[i][n][e]);
           }
         }
+      }
     }
   }
 
   __device__ __forceinline__ void finish() {
+    const float step = kUnits ? 2.0f * kv8_half_step(unit) : 1.0f;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -336,7 +396,10 @@ template <int D, typename T, int NT> struct A8Rows {
           w[n][j] += __shfl_xor_sync(0xffffffffu, w[n][j], x);
         }
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) { o[i][n][j] += 0.5f * w[n][j]; o[i][n][2 + j] += 0.5f * w[n][j]; }
+        for (int i = 0; i < kSteps; ++i) {
+          o[i][n][j] = (o[i][n][j] + 0.5f * w[n][j]) * step;
+          o[i][n][2 + j] = (o[i][n][2 + j] + 0.5f * w[n][j]) * step;
+        }
       }
   }
   // Entry `i` of the lane's D / 8 dimensions of row 8 n + 2c + j.
@@ -421,13 +484,15 @@ attention8_single_kernel(const A8Params p) {
     bulk_load(dst + Cfg::kSlot / 2, src + p.plane<D>(), Cfg::kSlot / 2, bar);
   };
   int page_cur = page_at(lane), page_nxt = page_at(32 + lane);
+  A8Rows<D, T, NT> rows;
+  typename A8Rows<D, T, NT>::Raw raw;
+  rows.fetch(raw, p, t, 1, kvh, group);                       // (asked for beside the pages)
   for (int i = 0; i < min(kRing, count); ++i) {
     const int page = __shfl_sync(0xffffffffu, page_cur, i);
     if (lane == 0) fetch(i, page);
   }
   uint2 word_cur = word_at(lane, page_cur);
-  A8Rows<D, T, NT> rows;
-  rows.load(p, t, 1, pos, kvh, group);
+  rows.load(raw, p, 1, pos, group);
   int gave_up = -1;                                           // the block whose wait ran out
   for (int base = 0; base < count; base += 32) {
     const uint2 word_nxt = word_at(base + 32 + lane, page_nxt);
@@ -573,23 +638,23 @@ attention8_single_kernel(const A8Params p) {
 }
 
 // Portions: a warp has rows of its own, the heads of the group for as many neighbouring tokens as fit 8 NT rows; the block's warps have
-// neighbouring ones and read the same keys out of one ring of slots (a turn's kA8Turn blocks each) that a fifth warp keeps filled.
+// neighbouring ones and read the same keys out of one ring of slots, a turn's kA8Turn blocks each.  The warps take turns at fetching: turn i's
+// one refills the slot that turn i - kLag left, which the others are through with by then (but for the slowest, which it waits for).
 template <int D, typename T> struct A8Portion {
   static constexpr int kTiles = D == 64 ? (sizeof(T) == 2 ? 4 : 2) : 2;
-  static constexpr int kRing = 4;
+  static constexpr int kRing = 6, kLag = 2;
   static constexpr int kSlot = kA8Turn * 2 * kKv8Block * D;
   static constexpr int kSmem = kRing * kSlot;
 };
 
 template <int D, typename T>
-__global__ void __launch_bounds__((kA8Warps + 1) * 32)
+__global__ void __launch_bounds__(kA8Warps * 32)
 attention8_portion_kernel(const A8Params p) {
   using Cfg = A8Portion<D, T>;
-  constexpr int NT = Cfg::kTiles, kRing = Cfg::kRing;
+  constexpr int NT = Cfg::kTiles, kRing = Cfg::kRing, kLag = Cfg::kLag;
+  static_assert(32 % kA8Turn == 0 && kRing * kA8Turn <= 32, "pages are looked up for 32 blocks at a time, and the 32 after them");
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ __align__(8) uint64_t s_full[kRing], s_empty[kRing];
-  __shared__ uint2 s_word[kRing][kA8Turn];
-  __shared__ int s_have[kRing][kA8Turn];
   __shared__ volatile int s_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const uint32_t full0 = smem_addr(s_full), empty0 = smem_addr(s_empty);
@@ -611,50 +676,61 @@ attention8_portion_kernel(const A8Params p) {
   const int lo = p.window > 0 && pos0 + 1 > p.window ? pos0 + 1 - p.window : 0;
   const int begin = lo / kKv8Block, end = (pos0 + tokens - 1) / kKv8Block + 1;
   const int turns = (end - begin + kA8Turn - 1) / kA8Turn;
-  if (warp == kA8Warps) {
-    // ---- the slots: lane 0 fetches, the lanes look ahead for the pages of 32 blocks
-    const int* table = p.block_table + (size_t)tl[0] * p.bt_stride;
-    int page = -1;
-    uint2 word = make_uint2(0u, 0u);
-    for (int i = 0; i < turns; ++i) {
-      const int b32 = i * kA8Turn % 32;
-      if (b32 == 0) {
-        const int block = begin + i * kA8Turn + lane;
-        page = block < end ? p.page_of(table, block) : -1;
-        word = page >= 0 ? p.word(page, kvh, p.sub_of(block)) : make_uint2(0u, 0u);
-      }
-      const int s = i % kRing;
-      if (!__all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, ((i / kRing) & 1) ^ 1, &s_abort, p.status, 9))) {
-        for (int k = max(0, i - kRing); k < i; ++k) mbar_drain(full0 + 8 * (k % kRing), (k / kRing) & 1);
-        return;
-      }
-      const bool mine = lane >= b32 && lane < b32 + kA8Turn;
-      if (mine) { s_word[s][lane - b32] = word; s_have[s][lane - b32] = page >= 0; }
-      const unsigned got = __ballot_sync(0xffffffffu, mine && page >= 0);
-      __syncwarp();
-      const uint32_t bar = full0 + 8 * s;
-      if (lane == 0) mbar_expect_tx(bar, __popc(got) * 2 * kKv8Block * D);      // (its arrival publishes the words)
-      __syncwarp();
-      if (mine && page >= 0) {
-        const unsigned char* src = p.keys<D>(page, kvh, p.sub_of(begin + i * kA8Turn + lane - b32));
-        const uint32_t dst = smem_addr(smem) + s * Cfg::kSlot + (lane - b32) * 2 * kKv8Block * D;
-        bulk_load(dst, src, kKv8Block * D, bar);
-        bulk_load(dst + kKv8Block * D, src + p.plane<D>(), kKv8Block * D, bar);
-      }
-      __syncwarp();
+  const int* table = p.block_table + (size_t)tl[0] * p.bt_stride;
+  auto page_at = [&](int i) { return begin + i < end ? p.page_of(table, begin + i) : -1; };      // of the block's i-th block of keys
+  auto word_at = [&](int i, int page) { return page >= 0 ? p.word(page, kvh, p.sub_of(begin + i)) : make_uint2(0u, 0u); };
+  // lanes 0 .. kA8Turn - 1 fetch the turn's blocks, whose pages they are given
+  auto fetch = [&](int turn, int page) {
+    const int s = turn % kRing;
+    const uint32_t bar = full0 + 8 * s;
+    const unsigned got = __ballot_sync(0xffffffffu, lane < kA8Turn && page >= 0);
+    if (lane == 0) mbar_expect_tx(bar, __popc(got) * 2 * kKv8Block * D);
+    __syncwarp();
+    if (lane < kA8Turn && page >= 0) {
+      const unsigned char* src = p.keys<D>(page, kvh, p.sub_of(begin + turn * kA8Turn + lane));
+      const uint32_t dst = smem_addr(smem) + s * Cfg::kSlot + lane * 2 * kKv8Block * D;
+      bulk_load(dst, src, kKv8Block * D, bar);
+      bulk_load(dst + kKv8Block * D, src + p.plane<D>(), kKv8Block * D, bar);
     }
-    return;
-  }
-  const int my_tokens = min(per_warp, tokens - warp * per_warp);
+    __syncwarp();
+  };
+  const int my_tokens = max(0, min(per_warp, tokens - warp * per_warp));
   const int my_t0 = t0 + warp * per_warp, my_pos0 = pos0 + warp * per_warp, my_last = my_pos0 + my_tokens - 1;
   const int my_lo = p.window > 0 && my_pos0 + 1 > p.window ? my_pos0 + 1 - p.window : 0;
   const int all_first = p.window > 0 && my_last + 1 > p.window ? my_last + 1 - p.window : 0;
+  int page_cur = page_at(lane), page_nxt = page_at(32 + lane);
   A8Rows<D, T, NT> rows;
-  rows.load(p, my_t0, max(0, my_tokens), my_pos0, kvh, group);
+  {
+    typename A8Rows<D, T, NT>::Raw raw;
+    rows.fetch(raw, p, my_t0, my_tokens, kvh, group);
+    for (int i = 0; i < min(kRing - kLag, turns); ++i) {
+      const int page = __shfl_sync(0xffffffffu, page_cur, (i * kA8Turn + lane) & 31);
+      if (i % kA8Warps == warp) fetch(i, page);
+    }
+    rows.load(raw, p, my_tokens, my_pos0, group);
+  }
+  uint2 word_cur = word_at(lane, page_cur), word_nxt = word_at(32 + lane, page_nxt);
+  int page_nn = page_at(64 + lane);
   for (int i = 0; i < turns; ++i) {
+    const int at = i * kA8Turn % 32;
+    if (at == 0 && i > 0) {
+      page_cur = page_nxt; word_cur = word_nxt; page_nxt = page_nn;
+      word_nxt = word_at(i * kA8Turn + 32 + lane, page_nxt);
+      page_nn = page_at(i * kA8Turn + 64 + lane);
+    }
+    bool ok = true;
+    const int next = i + kRing - kLag;                        // the turn that takes the slot of turn i - kLag
+    if (next < turns) {
+      const int ahead = at + (kRing - kLag) * kA8Turn + lane;
+      const int near = __shfl_sync(0xffffffffu, page_cur, ahead & 31), far = __shfl_sync(0xffffffffu, page_nxt, ahead & 31);
+      if (next % kA8Warps == warp) {
+        ok = i < kLag || __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * (next % kRing), ((next / kRing) & 1) ^ 1, &s_abort, p.status, 9));
+        if (ok) fetch(next, ahead < 32 ? near : far);
+      }
+    }
     const int s = i % kRing, first_key = (begin + i * kA8Turn) * kKv8Block;
-    if (!__all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, (i / kRing) & 1, &s_abort, p.status, 9))) {
-      for (int k = i; k < min(i + kRing, turns); ++k) mbar_drain(full0 + 8 * (k % kRing), (k / kRing) & 1);
+    if (!ok || !__all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, (i / kRing) & 1, &s_abort, p.status, 9))) {
+      for (int k = i; k < min(i + kRing, turns); ++k) mbar_drain(full0 + 8 * (k % kRing), (k / kRing) & 1);      // (copies that are under way)
       return;
     }
     if (my_tokens > 0 && first_key <= my_last && first_key + kA8Turn * kKv8Block > my_lo) {
@@ -665,8 +741,9 @@ attention8_portion_kernel(const A8Params p) {
 #pragma unroll
       for (int b = 0; b < kA8Turn; ++b) {
         slot[b] = smem + s * Cfg::kSlot + b * 2 * kKv8Block * D;
-        have[b] = s_have[s][b];
-        word[b] = s_word[s][b];
+        have[b] = __shfl_sync(0xffffffffu, page_cur, at + b) >= 0;
+        word[b].x = __shfl_sync(0xffffffffu, word_cur.x, at + b);
+        word[b].y = __shfl_sync(0xffffffffu, word_cur.y, at + b);
         key0[b] = first_key + b * kKv8Block;
       }
       rows.turn(slot, have, word, key0, all_first, my_pos0);
@@ -715,7 +792,7 @@ static int launch_attention8(const A8Params& p, int singles, int tiles, int per_
   if (int rc = raise_shared_memory("attention8_portion", attention8_portion_kernel<D, T>, Cfg::kSmem, raised)) return rc;
   const int per_block = 8 * Cfg::kTiles / group * kA8Warps;
   return launch_kernel("attention8_portion", attention8_portion_kernel<D, T>, dim3(p.nkv * ((128 + per_block - 1) / per_block), tiles),
-                       dim3((kA8Warps + 1) * 32), Cfg::kSmem, stream, p);
+                       dim3(kA8Warps * 32), Cfg::kSmem, stream, p);
 }
 
 template <typename T>

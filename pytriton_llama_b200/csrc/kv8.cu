@@ -2,132 +2,165 @@
 //
 // Write.  qkv is a step's projection [tokens, (nq + 2 nkv) d] as in rope_kv.cu: q is turned by position * inv_freq
 // in place; k, turned likewise and rounded to the step's type, and v go into the blocks that `slots` name.  The k and v columns of
-// qkv stay as they are.  The rows of one block of 16 positions stand next to each other in the step (a request's tokens do);
-// the first row of such a run does the work for all of it, one warp per (head, k or v): the largest magnitude and the marks of the
-// new values, then, where the block's exponent grows, the codes that are there made coarser, then the new codes.  A run
-// that holds the block's first position starts the block anew.
+// qkv stay as they are.  The rows of one block of 16 positions stand next to each other in the step (a request's tokens do): a
+// run.  One warp does a run's work for one head's k or v: it reads the values once, into registers, for the largest magnitude
+// and the marks; then, where the block's exponent grows, the codes that are there are made coarser; then come the new codes.  A run
+// that holds the block's first position starts the block anew.  A block of threads looks at one row of the step, or, in steps
+// of more rows than fill the machine, at 16, and takes the runs that begin there.
 #include "kv8.cuh"
 
 namespace ptl {
 
 constexpr int kKv8Threads = 256;
 
-// Packet `i` (of Vec16<T>::N values) of k (part 0, turned) or v (part 1) of one head in one row.
-template <typename T>
-__device__ __forceinline__ void kv8_values_of(float (&x)[Vec16<T>::N], const T* head, int i, int half, int rot, bool turned,
-                                              const float* cs /* cos[half], sin[half] of the row */) {
-  constexpr int N = Vec16<T>::N;
-  const Vec16<T> a = load16(head + i * N);
-#pragma unroll
-  for (int j = 0; j < N; ++j) x[j] = a.get(j);
-  if (!turned || i * N >= rot) return;
-  if (half % N == 0) {
-    const bool first = i * N < half;
-    const Vec16<T> b = load16(head + i * N + (first ? half : -half));
-    const int c0 = i * N - (first ? 0 : half);
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      float o1, o2;
-      rope_rotate(first ? x[j] : b.get(j), first ? b.get(j) : x[j], cs[c0 + j], cs[half + c0 + j], o1, o2);
-      x[j] = to_f32(from_f32<T>(first ? o1 : o2));
-    }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const int e = i * N + j;
-    if (e >= rot) break;
-    const bool first = e < half;
-    const int c = first ? e : e - half;
-    float o1, o2;
-    rope_rotate(to_f32(head[c]), to_f32(head[c + half]), cs[c], cs[half + c], o1, o2);
-    x[j] = to_f32(from_f32<T>(first ? o1 : o2));
-  }
-}
-
 template <int N> struct Kv8Packet;
 template <> struct Kv8Packet<8> { using type = uint2; };
 template <> struct Kv8Packet<4> { using type = uint32_t; };
 
-template <typename T>
-__global__ void __launch_bounds__(kKv8Threads)
-rope_kv8_write_kernel(T* __restrict__ qkv, const int* __restrict__ positions, const float* __restrict__ inv_freq,
-                      const int* __restrict__ slots, unsigned char* __restrict__ codes, uint32_t* __restrict__ words, int tokens,
-                      int nq, int nkv, int d, int rot, int page_size, long long num_slots) {
-  extern __shared__ float cs[];                  // [up to 16 rows][cos[half], sin[half]]
-  constexpr int N = Vec16<T>::N;
-  const int t = blockIdx.x;
-  const int row_len = (nq + 2 * nkv) * d, half = rot / 2;
-  // positions, slots and frequencies are inputs of the step, not results of the kernel before this one
-  auto block_of = [&](int row) -> long long {
+// (cos, sin) of an angle: a call, so that the kernel holds it once.
+__device__ __noinline__ float2 kv8_angle(float a) {
+  float2 r;
+  sincosf(a, &r.y, &r.x);
+  return r;
+}
+
+struct Kv8WriteParams {
+  void* qkv;
+  const int* positions;
+  const float* inv_freq;
+  const int* slots;
+  unsigned char* codes;
+  uint32_t* words;
+  int tokens, nq, nkv, d, rot, page_size, rows_per_block;
+  long long num_slots;
+
+  // The block of 16 positions that a row goes to, -1: none.
+  __device__ __forceinline__ int block_of(int row) const {
     const int s = row >= 0 && row < tokens ? __ldg(slots + row) : -1;
     return s >= 0 && s < num_slots ? s / kKv8Block : -1;
-  };
-  const long long block = block_of(t);
-  const bool leads = block >= 0 && block_of(t - 1) != block;
-  int rows = 0;                                  // of the run (counted up to 16 at a time)
-  auto count_rows = [&](int first) {
-    int n = 0;
-    while (n < kKv8Block && block_of(first + n) == block) ++n;
-    return n;
-  };
-  if (leads) rows = count_rows(t);
-  if (!leads && (nq == 0 || !inv_freq)) return;
-  auto angles = [&](int first, int n) {
-    for (int e = threadIdx.x; e < n * half; e += kKv8Threads) {
-      const int r = e / half, j = e % half;
-      float s, c;
-      sincosf((float)__ldg(positions + first + r) * inv_freq[j], &s, &c);
-      cs[r * rot + j] = c;
-      cs[r * rot + half + j] = s;
+  }
+  __device__ __forceinline__ float2 angle(int row, int j) const { return kv8_angle((float)__ldg(positions + row) * inv_freq[j]); }
+};
+
+// The turned values of packet `i` of a k head in `row`; cs: cos[half], sin[half] of the row, or null.
+template <typename T>
+__device__ __forceinline__ void kv8_turn(const Kv8WriteParams& p, float (&x)[Vec16<T>::N], const T* head, int i, int row, const float* cs) {
+  constexpr int N = Vec16<T>::N;
+  const int half = p.rot / 2;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int e = i * N + j;
+    if (e >= p.rot) break;
+    const bool low = e < half;
+    const int a = low ? e : e - half;
+    float o1, o2;
+    const float2 cos_sin = cs ? make_float2(cs[a], cs[half + a]) : p.angle(row, a);
+    const float other = to_f32(head[low ? e + half : a]);
+    rope_rotate(low ? x[j] : other, low ? other : x[j], cos_sin.x, cos_sin.y, o1, o2);
+    x[j] = to_f32(from_f32<T>(low ? o1 : o2));
+  }
+}
+
+// D: the head size, or 0 for any (then the values are read twice).  TURN: there are frequencies.
+template <typename T, int D, bool TURN>
+__global__ void __launch_bounds__(kKv8Threads)
+rope_kv8_write_kernel(const Kv8WriteParams p) {
+  extern __shared__ float cs[];                  // [rows staged][cos[half], sin[half]]
+  constexpr int N = Vec16<T>::N;
+  constexpr int kPackets = D ? kKv8Block * D / N / 32 : 1;     // a lane has of a run's 16 rows
+  const int d = D ? D : p.d;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row_len = (p.nq + 2 * p.nkv) * d, half = p.rot / 2;
+  const int t0 = blockIdx.x * p.rows_per_block, t1 = min(p.tokens, t0 + p.rows_per_block);
+  T* qkv = static_cast<T*>(p.qkv);
+  // positions, slots and frequencies are inputs of the step, not results of the kernel before this one
+  const int mine = p.block_of(t0 - 1 + lane);                  // (rows t0 - 1 .. t0 + 30)
+  const int before = __shfl_up_sync(0xffffffffu, mine, 1);
+  const unsigned leads = __ballot_sync(0xffffffffu, lane >= 1 && t0 - 1 + lane < t1 && mine >= 0 && mine != before) >> 1;      // bit i: row t0 + i begins a run
+  if (!leads && (p.nq == 0 || !TURN)) return;
+  int staged = 0;                                              // rows from t0 on whose angles are in shared memory
+  if constexpr (TURN) {
+    const int last = 31 - __clz(leads | 1u);                   // the last run's first row, and up to 16 of its rows
+    const int of_last = __shfl_sync(0xffffffffu, mine, last + 1);
+    const unsigned same = __ballot_sync(0xffffffffu, lane > last && mine == of_last) >> (last + 1);
+    staged = max(t1 - t0, leads ? last + min(kKv8Block, __ffs(~same) - 1) : 0);
+    for (int e = threadIdx.x; e < staged * half; e += kKv8Threads) {
+      if (t0 + e / half >= p.tokens) break;
+      const float2 cos_sin = p.angle(t0 + e / half, e % half);
+      cs[e / half * p.rot + e % half] = cos_sin.x;
+      cs[e / half * p.rot + half + e % half] = cos_sin.y;
     }
-  };
-  if (inv_freq) angles(t, max(rows, 1));
+  }
   pdl_wait();
   pdl_launch_dependents();
   __syncthreads();
-  if (inv_freq) {                                // q of this row, in place
-    T* row = qkv + (size_t)t * row_len;
-    for (int e = threadIdx.x; e < nq * half; e += kKv8Threads) {
-      T* head = row + (size_t)(e / half) * d;
-      const int j = e % half;
+  if constexpr (TURN) {                          // q of these rows, in place
+    for (int e = blockIdx.y * kKv8Threads + threadIdx.x; e < (t1 - t0) * p.nq * half; e += gridDim.y * kKv8Threads) {
+      const int r = e / (p.nq * half), j = e % half;
+      T* head = qkv + (size_t)(t0 + r) * row_len + (size_t)(e / half % p.nq) * d;
       float o1, o2;
-      rope_rotate(to_f32(head[j]), to_f32(head[j + half]), cs[j], cs[half + j], o1, o2);
+      rope_rotate(to_f32(head[j]), to_f32(head[j + half]), cs[r * p.rot + j], cs[r * p.rot + half + j], o1, o2);
       head[j] = from_f32<T>(o1);
       head[j + half] = from_f32<T>(o2);
     }
   }
-  if (!leads) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int blocks_per_page = page_size / kKv8Block;
-  const long long page = block / blocks_per_page;
-  const int sub = (int)(block % blocks_per_page);
-  const int packets = d / N;
-  int first = t;
-  while (true) {
-    for (int unit = warp; unit < 2 * nkv; unit += kKv8Threads / 32) {
-      const int g = unit >> 1, part = unit & 1;
-      const T* src = qkv + (size_t)first * row_len + (size_t)(nq + part * nkv + g) * d;
-      const bool turned = part == 0 && inv_freq != nullptr;
-      unsigned char* dst = codes + (((size_t)page * 2 + part) * nkv + g) * page_size * d + (size_t)sub * kKv8Block * d;
-      uint32_t* word = words + ((size_t)page * nkv + g) * blocks_per_page * 2 + sub * 2 + part;
+  const int blocks_per_page = p.page_size / kKv8Block, units = 2 * p.nkv, packets = d / N;
+  for (int task = blockIdx.y * (kKv8Threads / 32) + warp; task < __popc(leads) * units; task += gridDim.y * (kKv8Threads / 32)) {
+    const int unit = task % units, g = unit >> 1, part = unit & 1;
+    int first = t0 + __fns(leads, 0, task / units + 1);
+    const int block = p.block_of(first);
+    const int page = block / blocks_per_page, sub = block % blocks_per_page;
+    unsigned char* dst = p.codes + (((size_t)page * 2 + part) * p.nkv + g) * p.page_size * d + (size_t)sub * kKv8Block * d;
+    uint32_t* word = p.words + ((size_t)page * p.nkv + g) * blocks_per_page * 2 + sub * 2 + part;
+    const bool turned = TURN && part == 0;
+    while (true) {                               // up to 16 rows at a time (more: the same positions again)
+      const int slot = lane < kKv8Block && first + lane < p.tokens ? __ldg(p.slots + first + lane) : -1;
+      const unsigned others = __ballot_sync(0xffffffffu, slot < 0 || slot >= p.num_slots || slot / kKv8Block != block);
+      const int rows = __ffs(others) - 1;        // (lanes 16 to 31 are others)
+      if (rows == 0) break;
+      const int off = slot % kKv8Block;
+      const uint32_t here = __reduce_or_sync(0xffffffffu, lane < rows ? 1u << off : 0u);
+      const T* src = qkv + (size_t)first * row_len + (size_t)(p.nq + part * p.nkv + g) * d;
       const uint32_t had = *word;
-      uint32_t amax = 0u, here = 0u, bad = 0u;    // bits of the largest magnitude; tokens of the run, and the marked ones among them
-      float x[N];
-      for (int e = lane; e < rows * packets; e += 32) {
-        const int r = e / packets;
-        const uint32_t bit = 1u << (__ldg(slots + first + r) % kKv8Block);
-        kv8_values_of<T>(x, src + (size_t)r * row_len, e % packets, half, rot, turned, cs + r * rot);
-        here |= bit;
+      Vec16<T> raw[kPackets];                    // (turned, once they have been looked at)
+      auto fetch = [&](int e) { return load16(src + (size_t)(e / packets) * row_len + e % packets * N); };
+      auto turn = [&](int e, Vec16<T>& v) {
+        if (!TURN || !turned) return;
+        float x[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = v.get(j);
+        const int row = first + e / packets;
+        kv8_turn<T>(p, x, src + (size_t)(e / packets) * row_len, e % packets, row, row - t0 < staged ? cs + (row - t0) * p.rot : nullptr);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v.set(j, x[j]);
+      };
+      uint32_t amax = 0u, bad = 0u;              // bits of the largest magnitude; the marked tokens
+      auto look = [&](int e, const Vec16<T>& v) {
+        bool odd = false;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          const uint32_t mag = __float_as_uint(x[j]) & 0x7fffffffu;
-          if (mag >= 0x7f800000u) bad |= bit;
-          else amax = max(amax, mag);
+          const uint32_t mag = __float_as_uint(v.get(j)) & 0x7fffffffu;
+          odd |= mag >= 0x7f800000u;
+          amax = max(amax, mag >= 0x7f800000u ? 0u : mag);
+        }
+        const int row_off = __ldg(p.slots + first + e / packets) % kKv8Block;
+        if (odd) bad |= 1u << row_off;
+      };
+      if constexpr (D != 0) {
+#pragma unroll
+        for (int i = 0; i < kPackets; ++i)
+          if (lane + 32 * i < rows * packets) raw[i] = fetch(lane + 32 * i);
+#pragma unroll
+        for (int i = 0; i < kPackets; ++i)
+          if (lane + 32 * i < rows * packets) { turn(lane + 32 * i, raw[i]); look(lane + 32 * i, raw[i]); }
+      } else {
+        for (int e = lane; e < rows * packets; e += 32) {
+          Vec16<T> v = fetch(e);
+          turn(e, v);
+          look(e, v);
         }
       }
       amax = __reduce_max_sync(0xffffffffu, amax);
-      here = __reduce_or_sync(0xffffffffu, here);
       bad = __reduce_or_sync(0xffffffffu, bad);
       const bool anew = here & 1u;
       const int e_old = anew ? 0 : (int)(had & 255u);
@@ -139,36 +172,44 @@ rope_kv8_write_kernel(T* __restrict__ qkv, const int* __restrict__ positions, co
           v.x = kv8_coarser(v.x, n); v.y = kv8_coarser(v.y, n); v.z = kv8_coarser(v.z, n); v.w = kv8_coarser(v.w, n);
           reinterpret_cast<uint4*>(dst)[i] = v;
         }
-        __syncwarp();
       }
+      __syncwarp();
       const float inverse = e_new ? kv8_inverse_step(e_new) : 0.f;
-      for (int e = lane; e < rows * packets; e += 32) {
-        const int r = e / packets, i = e % packets;
-        kv8_values_of<T>(x, src + (size_t)r * row_len, i, half, rot, turned, cs + r * rot);
+      auto store = [&](int e, const Vec16<T>& v) {
         uint32_t out[N / 4];
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          const bool finite = (__float_as_uint(x[j]) & 0x7fffffffu) < 0x7f800000u;
-          const uint32_t u = finite && e_new ? kv8_code(x[j], inverse) : 128u;
+          const float x = v.get(j);
+          const bool finite = (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u;
+          const uint32_t u = finite && e_new ? kv8_code(x, inverse) : 128u;
           out[j / 4] = j % 4 ? out[j / 4] | u << (8 * (j % 4)) : u;
         }
-        *reinterpret_cast<typename Kv8Packet<N>::type*>(dst + (size_t)(__ldg(slots + first + r) % kKv8Block) * d + i * N) =
-            *reinterpret_cast<typename Kv8Packet<N>::type*>(out);
+        const int row_off = __ldg(p.slots + first + e / packets) % kKv8Block;
+        *reinterpret_cast<typename Kv8Packet<N>::type*>(dst + (size_t)row_off * d + e % packets * N) = *reinterpret_cast<typename Kv8Packet<N>::type*>(out);
+      };
+      if constexpr (D != 0) {
+#pragma unroll
+        for (int i = 0; i < kPackets; ++i)
+          if (lane + 32 * i < rows * packets) store(lane + 32 * i, raw[i]);
+      } else {
+        for (int e = lane; e < rows * packets; e += 32) {
+          Vec16<T> v = fetch(e);
+          turn(e, v);
+          store(e, v);
+        }
       }
       if (lane == 0) *word = (uint32_t)e_new | ((((anew ? 0u : had >> 16) & ~here) | bad) << 16);
       __syncwarp();
+      first += rows;
+      if (rows < kKv8Block) break;
     }
-    first += rows;
-    rows = count_rows(first);                    // more rows than positions: the same ones again
-    if (rows == 0) break;
-    __syncthreads();
-    if (inv_freq) angles(first, rows);
-    __syncthreads();
   }
 }
 
-// Keys and values of the first length[r] tokens of the requests as numbers, request after request: out [tokens][2][heads][d].
+// Keys and values of the first length[r] tokens of the requests as numbers, request after request: out [tokens][2][heads][d].  A block
+// takes 1,024 pieces of 8 codes of one request, four a thread.
 constexpr int kKv8ReadRequests = 960;
+constexpr int kKv8ReadAhead = 4;
 struct Kv8ReadArgs {
   long long first_row;                     // of the output
   int requests, first_request;
@@ -180,39 +221,44 @@ __global__ void __launch_bounds__(kKv8Threads)
 read_kv8_kernel(T* __restrict__ out, const unsigned char* __restrict__ codes, const uint32_t* __restrict__ words,
                 const int* __restrict__ block_table, const __grid_constant__ Kv8ReadArgs args, int bt_stride, int nkv, int d, int page_size,
                 int num_pages) {
+  constexpr int N = 8;                     // codes of a piece
+  const int r = blockIdx.y;
+  const int t0 = r ? args.end[r - 1] : 0, tokens = args.end[r] - t0;
+  const int per_token = 2 * nkv * d / N;
+  const long long total = (long long)tokens * per_token;
+  const long long at = (long long)blockIdx.x * (kKv8Threads * kKv8ReadAhead) + threadIdx.x;
+  if (at - threadIdx.x >= total) return;
   pdl_wait();
   pdl_launch_dependents();
-  constexpr int N = 8;                     // codes a thread takes
-  const int per_token = 2 * nkv * d / N;
-  const long long total = (long long)args.end[args.requests - 1] * per_token;
-  for (long long i = (long long)blockIdx.x * kKv8Threads + threadIdx.x; i < total; i += (long long)gridDim.x * kKv8Threads) {
-    const int t = (int)(i / per_token), e = (int)(i % per_token) * N;
-    int lo = 0, hi = args.requests - 1;    // the first request that ends behind t
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (args.end[mid] > t) hi = mid; else lo = mid + 1;
-    }
-    const int pos = t - (lo ? args.end[lo - 1] : 0);
-    const int page = block_table[(size_t)(args.first_request + lo) * bt_stride + pos / page_size];
-    const int part = e / (nkv * d), g = e / d % nkv, off = pos % page_size;
-    float v[N];
-    if (page >= 0 && page < num_pages) {
-      const uint2 c = *reinterpret_cast<const uint2*>(codes + ((((size_t)page * 2 + part) * nkv + g) * page_size + off) * d + e % d);
-      const uint32_t w = words[(((size_t)page * nkv + g) * (page_size / kKv8Block) + off / kKv8Block) * 2 + part];
-      const float half_step = kv8_half_step(w & 255u);
-      const bool bad = w >> (16 + off % kKv8Block) & 1u;
+  const int* table = block_table + (size_t)(args.first_request + r) * bt_stride;
+  uint2 c[kKv8ReadAhead];
+  uint32_t w[kKv8ReadAhead];
+  bool have[kKv8ReadAhead];
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        v[j] = bad ? __uint_as_float(0x7fc00000u) : (float)(2 * (int)(((j < 4 ? c.x : c.y) >> (8 * (j & 3))) & 255u) - 255) * half_step;
-    } else {
+  for (int i = 0; i < kKv8ReadAhead; ++i) {
+    const long long x = at + i * kKv8Threads;
+    have[i] = false;
+    if (x >= total) continue;
+    const int pos = (int)(x / per_token), e = (int)(x % per_token) * N;
+    const int page = __ldg(table + pos / page_size), part = e / (nkv * d), g = e / d % nkv, off = pos % page_size;
+    if (page < 0 || page >= num_pages) continue;             // a position that has no page
+    have[i] = true;
+    c[i] = __ldg(reinterpret_cast<const uint2*>(codes + ((((size_t)page * 2 + part) * nkv + g) * page_size + off) * d + e % d));
+    w[i] = __ldg(words + (((size_t)page * nkv + g) * (page_size / kKv8Block) + off / kKv8Block) * 2 + part);
+  }
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = 0.f;          // a position that has no page
-    }
-    T* dst = out + (args.first_row + t) * 2 * nkv * d + e;
+  for (int i = 0; i < kKv8ReadAhead; ++i) {
+    const long long x = at + i * kKv8Threads;
+    if (x >= total) continue;
+    const int pos = (int)(x / per_token);
+    const float half_step = have[i] ? kv8_half_step(w[i] & 255u) : 0.f;
+    const bool bad = have[i] && (w[i] >> (16 + pos % kKv8Block) & 1u);
+    T* dst = out + (args.first_row + t0) * 2 * nkv * d + x * N;
     Vec16<T> p;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      p.set(j % Vec16<T>::N, v[j]);
+      const float v = have[i] ? (float)(2 * (int)(((j < 4 ? c[i].x : c[i].y) >> (8 * (j & 3))) & 255u) - 255) * half_step : 0.f;
+      p.set(j % Vec16<T>::N, bad ? __uint_as_float(0x7fc00000u) : v);
       if (j % Vec16<T>::N == Vec16<T>::N - 1) store16(dst + j + 1 - Vec16<T>::N, p);
     }
   }
@@ -222,18 +268,21 @@ template <typename T>
 static int rope_kv8_write(T* qkv, const int* positions, const float* inv_freq, const int* slots, void* codes, void* words, int tokens, int nq,
                           int nkv, int d, int rot, int page_size, long long num_slots, void* stream) {
   PTL_REQUIRE(tokens >= 0 && nq >= 0 && nkv > 0 && d > 0 && page_size > 0 && num_slots >= 0, "rope_kv8_write: bad sizes");
-  PTL_REQUIRE(d % 16 == 0 && d <= 1024, "rope_kv8_write: head size %d is no multiple of 16 up to 1,024", d);
+  PTL_REQUIRE(d % 16 == 0 && d <= 256, "rope_kv8_write: head size %d is no multiple of 16 up to 256", d);
+  PTL_REQUIRE(nkv <= 65535 * 4, "rope_kv8_write: too many heads");
   PTL_REQUIRE(page_size % kKv8Block == 0, "rope_kv8_write: pages of %d positions are not whole blocks of %d", page_size, kKv8Block);
   PTL_REQUIRE(rot % 2 == 0 && rot >= 0 && rot <= d, "rope_kv8_write: rotary width %d of head size %d", rot, d);
   PTL_REQUIRE(aligned16(qkv) && aligned16(codes), "rope_kv8_write: qkv and codes must be 16-byte aligned");
   if (tokens == 0) return 0;
   if (rot == 0) inv_freq = nullptr;
-  const size_t smem = inv_freq ? (size_t)kKv8Block * rot * sizeof(float) : 0;
-  static SmemRaised raised = {};
-  if (smem > 48 * 1024)
-    if (int rc = raise_shared_memory("rope_kv8_write", rope_kv8_write_kernel<T>, kKv8Block * 1024 * 4, raised)) return rc;
-  return launch_kernel("rope_kv8_write", rope_kv8_write_kernel<T>, dim3(tokens), dim3(kKv8Threads), smem, as_stream(stream), qkv, positions,
-                       inv_freq, slots, (unsigned char*)codes, (uint32_t*)words, tokens, nq, nkv, d, rot, page_size, num_slots);
+  Kv8WriteParams p{qkv, positions, inv_freq, slots, (unsigned char*)codes, (uint32_t*)words, tokens, nq, nkv, d, rot, page_size, 1, num_slots};
+  // a block a row while that does not fill the machine many times over; 64 tokens of 8 heads of 64: 6.5 us by one row, 16 rows of one block 20
+  p.rows_per_block = tokens > 1024 ? kKv8Block : 1;
+  const size_t smem = inv_freq ? (size_t)(p.rows_per_block + kKv8Block - 1) * rot * sizeof(float) : 0;
+  auto kernel = inv_freq ? (d == 64 ? rope_kv8_write_kernel<T, 64, true> : d == 128 ? rope_kv8_write_kernel<T, 128, true> : rope_kv8_write_kernel<T, 0, true>)
+                         : (d == 64 ? rope_kv8_write_kernel<T, 64, false> : d == 128 ? rope_kv8_write_kernel<T, 128, false> : rope_kv8_write_kernel<T, 0, false>);
+  return launch_kernel("rope_kv8_write", kernel, dim3((tokens + p.rows_per_block - 1) / p.rows_per_block, (2 * nkv + 7) / 8), dim3(kKv8Threads), smem,
+                       as_stream(stream), p);
 }
 
 template <typename T>
@@ -248,17 +297,19 @@ static int read_kv8(T* out, const void* codes, const void* words, const int* blo
     args.first_request = r0;
     args.requests = requests - r0 < kKv8ReadRequests ? requests - r0 : kKv8ReadRequests;
     long long sum = 0;
+    int longest = 0;
     for (int i = 0; i < args.requests; ++i) {
       const int n = lengths[r0 + i];
+      longest = n > longest ? n : longest;
       PTL_REQUIRE(n >= 0 && n <= (long long)bt_stride * page_size, "read_kv8: request %d of %d tokens does not fit its row of the table", r0 + i, n);
       sum += n;
       PTL_REQUIRE(sum <= 0x7fffffffLL, "read_kv8: too many tokens");
       args.end[i] = (int)sum;
     }
     if (sum > 0) {
-      const long long blocks = (sum * (2 * nkv * d / 8) + kKv8Threads - 1) / kKv8Threads;
-      const int grid = (int)(blocks < 148 * 16 ? blocks : 148 * 16);
-      if (int rc = launch_kernel("read_kv8", read_kv8_kernel<T>, dim3(grid), dim3(kKv8Threads), 0, as_stream(stream), out,
+      const long long blocks = ((long long)longest * (2 * nkv * d / 8) + kKv8Threads * kKv8ReadAhead - 1) / (kKv8Threads * kKv8ReadAhead);
+      PTL_REQUIRE(blocks <= 0x7fffffffLL, "read_kv8: a request is too long");
+      if (int rc = launch_kernel("read_kv8", read_kv8_kernel<T>, dim3((unsigned)blocks, args.requests), dim3(kKv8Threads), 0, as_stream(stream), out,
                                  (const unsigned char*)codes, (const uint32_t*)words, block_table, args, bt_stride, nkv, d, page_size, num_pages))
         return rc;
     }

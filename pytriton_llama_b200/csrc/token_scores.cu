@@ -7,9 +7,9 @@
 // A row is cut into slices, one block of a cluster each.  A thread keeps (m, S, U) of what it has read; threads, then blocks are
 // brought to one maximum.  The largest logits are found on the way: a 64-bit key holds the logit in an order of
 // whole numbers and, below it, the index the other way round, so keys are unique and of equal logits the lowest index is
-// the largest.  Every 8,192 logits, those above the threshold (the smallest of the `top` best so far) go to a list in shared
+// the largest.  Every 4,096 logits, those above the threshold (the smallest of the `top` best so far) go to a list in shared
 // memory.  Where more come than it has room for, the threshold is first raised to the `top`-th largest of the maxima of 64
-// groups of 128 logits: at most `top` * 128 logits can lie above that, and the list holds as many.
+// groups of 64 logits: at most `top` * 64 logits can lie above that, and the list holds as many.
 //
 // Logits of -inf have no probability.  A row with a NaN, with +inf, or with -inf only has no distribution: its
 // log-probabilities and its entropy are NaN.  Its alternatives are the largest logits all the same, NaN behind all others.
@@ -17,14 +17,13 @@
 
 namespace ptl {
 
-constexpr int kTsThreads = 512;
+constexpr int kTsThreads = 256;
 constexpr int kTsPerThread = 16;                       // logits of a turn
 constexpr int kTsTurn = kTsThreads * kTsPerThread;
 constexpr int kTsMaxTop = 32;
-constexpr int kTsGroups = 64;                          // of a turn, 8 threads each
-constexpr int kTsRoom = 4096 + kTsMaxTop;              // of the list: kTsMaxTop groups of 128 beside what is there
+constexpr int kTsGroups = 64;                          // of a turn, 4 threads each
+constexpr int kTsRoom = kTsMaxTop * (kTsTurn / kTsGroups) + kTsMaxTop;      // of the list: the groups that may lie above a raised threshold, and what is there
 constexpr int kTsMaxCluster = 8;
-static_assert(kTsMaxTop * (kTsTurn / kTsGroups) <= 4096, "what may lie above a raised threshold fits the list");
 
 typedef unsigned long long TsKey;
 // Larger logits have larger keys, equal ones larger keys at lower indices; NaN comes behind -inf.  No key is 0.
@@ -35,11 +34,22 @@ __device__ __forceinline__ TsKey ts_key(float x, int index) {
   return ((TsKey)order << 32) | (uint32_t)~index;
 }
 
+__device__ __forceinline__ float ts_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The logit of a key (0 and NaN keys: NaN).
+__device__ __forceinline__ float ts_logit(TsKey k) {
+  const uint32_t order = (uint32_t)(k >> 32);
+  return order == 0u ? __uint_as_float(0x7fc00000u) : __uint_as_float(order & 0x80000000u ? order ^ 0x80000000u : ~order);
+}
+
 // A sum S of e^(x - m), and U of e^(x - m) (x - m), taken to the maximum `to` >= m.  Further apart than 200 nothing is left; logits
 // of the type's lowest value are apart by what S times would not be a number.
 __device__ __forceinline__ void ts_move(float m, float to, float& S, float& U) {
-  if (m == -INFINITY) { S = U = 0.f; return; }
-  const float z = fmaxf(m - to, -200.f), f = exp2f(z * 1.4426950408889634f);
+  if (m == -INFINITY) { S = S != S ? S : 0.f; U = 0.f; return; }      // (NaN in S: a logit was none)
+  const float z = fmaxf(m - to, -200.f), f = ts_exp2(z * 1.4426950408889634f);
   U = f * (U + z * S);
   S *= f;
 }
@@ -50,7 +60,7 @@ struct TsShared {
   TsKey group[kTsGroups];
   TsKey threshold;
   TsKey merged[kTsMaxCluster * kTsMaxTop];             // in the first block of a cluster: every block's best
-  float sums[kTsMaxCluster][4];                        // ... and its m, S, U, and whether it has a logit with no place in a distribution
+  float sums[kTsMaxCluster][3];                        // ... and its m, S, U
   float red[33];
   int count;
 };
@@ -66,7 +76,7 @@ __device__ __forceinline__ void ts_select(const TsKey* keys, int n, int top, TsK
 }
 
 template <bool TOP>
-__global__ void __launch_bounds__(kTsThreads)
+__global__ void __launch_bounds__(kTsThreads, 3)
 token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, float* __restrict__ top_logprob, int* __restrict__ top_id,
                     const float* __restrict__ logits, const int* __restrict__ tokens, int vocab, int top, int slices) {
   extern __shared__ __align__(16) unsigned char smem[];
@@ -84,23 +94,30 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
   const int p0 = slice * per, p1 = min(packets, p0 + per);
   if (TOP && tid == 0) { sh.count = 0; sh.threshold = 0; }
   float m = -INFINITY, S = 0.f, U = 0.f;
-  bool fine = true;
   const int want = TOP ? min(top, max(0, min(vocab, p1 * 4 - skew) - max(0, p0 * 4 - skew))) : 0;      // this block's share of the best
   if (TOP) __syncthreads();
-  for (int base = p0; base < p1; base += kTsTurn / 4) {
-    float v[kTsPerThread];
+  // a turn's logits are asked for while the turn before is worked on
+  float ahead[kTsPerThread];
+  auto ask = [&](int base) {
 #pragma unroll
     for (int i = 0; i < kTsPerThread / 4; ++i) {
       const int p = base + i * kTsThreads + tid;
       const int e = p * 4 - skew;
       if (p < p1 && e >= 0 && e + 3 < vocab) {
         const float4 f = __ldcs(reinterpret_cast<const float4*>(x + e));
-        v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+        ahead[4 * i] = f.x; ahead[4 * i + 1] = f.y; ahead[4 * i + 2] = f.z; ahead[4 * i + 3] = f.w;
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[4 * i + j] = p < p1 && e + j >= 0 && e + j < vocab ? x[e + j] : -INFINITY;
+        for (int j = 0; j < 4; ++j) ahead[4 * i + j] = p < p1 && e + j >= 0 && e + j < vocab ? x[e + j] : -INFINITY;
       }
     }
+  };
+  ask(p0);
+  for (int base = p0; base < p1; base += kTsTurn / 4) {
+    float v[kTsPerThread];
+#pragma unroll
+    for (int i = 0; i < kTsPerThread; ++i) v[i] = ahead[i];
+    if (base + kTsTurn / 4 < p1) ask(base + kTsTurn / 4);
     float mx = v[0];
 #pragma unroll
     for (int i = 1; i < kTsPerThread; ++i) mx = fmaxf(mx, v[i]);
@@ -111,11 +128,9 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
     const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int i = 0; i < kTsPerThread; ++i) {
-      fine = fine && v[i] < INFINITY;                  // neither NaN nor +inf
-      const float z = fmaxf(v[i] - ref, -200.f);       // e^-200 is 0, and 0 * -200 is no NaN
-      const float e = exp2f(z * 1.4426950408889634f);
-      S += e;
-      U = fmaf(e, z, U);
+      const float z = v[i] - ref, e = ts_exp2(z * 1.4426950408889634f);
+      S += e;                                          // (a NaN stays in it; +inf shows in the maximum)
+      U = fmaf(e, fmaxf(z, -200.f), U);                // e^-200 is 0, and 0 * -200 is no NaN
     }
     if (TOP && want > 0) {
       // indices of this thread's logits: 4 * (base + i * kTsThreads + tid) - skew + j
@@ -125,13 +140,8 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
         return here ? ts_key(v[i], e) : (TsKey)0;
       };
       TsKey threshold = sh.threshold;
-      bool any = threshold == 0;
-      if (!any) {
-        const uint32_t least = (uint32_t)(threshold >> 32);
-#pragma unroll
-        for (int i = 0; i < kTsPerThread; ++i) any |= (uint32_t)(ts_key(v[i], 0) >> 32) >= least;
-      }
-      const int threads_with = __syncthreads_count(any);
+      float least = ts_logit(threshold);               // (NaN, a threshold that is no number or none: everything comes in)
+      const int threads_with = __syncthreads_count(!(mx < least));
       if (threads_with == 0) continue;                 // (the same in every thread)
       if (threads_with * kTsPerThread + sh.count > kTsRoom) {
         // raise the threshold: what the list holds down to the best, then the turn's group maxima
@@ -143,8 +153,14 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
           if (tid == 0) { sh.count = want; sh.threshold = max(sh.threshold, sh.best[want - 1]); }
         }
         TsKey mine = 0;
+        if (mx > -INFINITY) {                          // the first of the thread's largest (what is behind the row is -inf)
 #pragma unroll
-        for (int i = 0; i < kTsPerThread; ++i) mine = max(mine, key_at(i));
+          for (int i = kTsPerThread - 1; i >= 0; --i)
+            if (v[i] == mx) mine = key_at(i);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kTsPerThread; ++i) mine = max(mine, key_at(i));
+        }
 #pragma unroll
         for (int o = 1; o < kTsThreads / kTsGroups; o <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
         if (tid % (kTsThreads / kTsGroups) == 0) sh.group[tid / (kTsThreads / kTsGroups)] = mine;
@@ -159,13 +175,17 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
         }
         __syncthreads();
         threshold = sh.threshold;
+        least = ts_logit(threshold);
       }
+      if (!(mx < least)) {
 #pragma unroll
-      for (int i = 0; i < kTsPerThread; ++i) {
-        const TsKey k = key_at(i);
-        if (k > threshold) {
-          const int at = atomicAdd(&sh.count, 1);
-          if (at < kTsRoom) sh.list[at] = k;
+        for (int i = 0; i < kTsPerThread; ++i) {
+          if (v[i] < least) continue;
+          const TsKey k = key_at(i);
+          if (k > threshold) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kTsRoom) sh.list[at] = k;
+          }
         }
       }
       __syncthreads();
@@ -184,7 +204,6 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
   ts_move(m, bm, S, U);
   const float bU = block_sum(U, sh.red);
   const float bS = block_sum(S, sh.red);
-  const bool odd = __syncthreads_or(!fine);
   if (TOP && want > 0) {
     ts_select(sh.list, sh.count, want, sh.best);
     __syncthreads();
@@ -193,7 +212,7 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
   if (slices > 1) {
     cluster_arrive();                                  // every block of the cluster runs before a peer writes into it
     cluster_wait();
-    if (tid < 4) st_peer_f32(map_to_peer((uint32_t)__cvta_generic_to_shared(&sh.sums[slice][tid]), 0), tid == 0 ? bm : tid == 1 ? bS : tid == 2 ? bU : odd ? 1.f : 0.f);
+    if (tid < 3) st_peer_f32(map_to_peer((uint32_t)__cvta_generic_to_shared(&sh.sums[slice][tid]), 0), tid == 0 ? bm : tid == 1 ? bS : bU);
     if (TOP && tid < top) {
       const TsKey k = tid < want ? sh.best[tid] : 0;
       const uint32_t to = map_to_peer((uint32_t)__cvta_generic_to_shared(&sh.merged[slice * top + tid]), 0);
@@ -205,10 +224,9 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
     if (slice != 0) return;
   }
   float M = bm, St = bS, Ut = bU;
-  bool bad = odd;
   if (slices > 1) {
-    M = -INFINITY; bad = false;
-    for (int s = 0; s < slices; ++s) { M = fmaxf(M, sh.sums[s][0]); bad |= sh.sums[s][3] != 0.f; }
+    M = -INFINITY;
+    for (int s = 0; s < slices; ++s) M = fmaxf(M, sh.sums[s][0]);
     St = Ut = 0.f;
     for (int s = 0; s < slices; ++s) {
       float Ss = sh.sums[s][1], Us = sh.sums[s][2];
@@ -218,7 +236,7 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
     }
   }
   const float nan = __uint_as_float(0x7fc00000u);
-  bad |= M == -INFINITY;
+  const bool bad = M == -INFINITY || M == INFINITY || St != St;
   const float log_sum = logf(St);
   if (tid == 0) {
     const int t = tokens[row];
@@ -261,7 +279,7 @@ PTL_EXPORT int ptl_token_scores(float* logprob, float* entropy, float* top_logpr
   PTL_REQUIRE((reinterpret_cast<uintptr_t>(logits) & 3u) == 0, "token_scores: logits must be 4-byte aligned");
   if (rows == 0) return 0;
   int slices = 1;
-  while (slices < kTsMaxCluster && (long long)rows * slices * 2 <= 2368 && vocab / (slices * 2) >= 4096) slices *= 2;
+  while (slices < kTsMaxCluster && (long long)rows * slices * 2 <= 1184 && vocab / (slices * 2) >= 4096) slices *= 2;
   PTL_REQUIRE((long long)rows * slices <= 0x7fffffffLL, "token_scores: too many rows");
   static SmemRaised raised[2] = {};
   constexpr int kSmem = (int)sizeof(TsShared);

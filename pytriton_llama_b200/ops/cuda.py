@@ -441,6 +441,13 @@ class CudaOps:
         if dtype is not None and t.dtype != dtype:
             raise KernelError(f"{name} has element type {t.dtype}, expected {dtype}")
 
+    def _want_all(self, dtype, **tensors) -> None:
+        """``_want`` of several tensors of one type: a look at each, the message only where one does not fit."""
+        device = self.device
+        for name, t in tensors.items():
+            if t.dtype is not dtype or not t.is_contiguous() or t.device != device:
+                self._want(t, name, dtype)
+
     def empty(self, shape, dtype) -> torch.Tensor:
         return torch.empty(shape, dtype=dtype, device=self.device)
 
@@ -898,15 +905,17 @@ class CudaOps:
     KV8_BLOCK = 16         # positions that share a scale
 
     def _want_kv8(self, codes: torch.Tensor, words: torch.Tensor, nkv: int, d: int, page_size: int) -> None:
-        self._want(codes, "codes", torch.uint8)
-        self._want(words, "words", torch.int32)
+        self._want_all(torch.uint8, codes=codes)
+        self._want_all(torch.int32, words=words)
         if page_size % self.KV8_BLOCK:
             raise KernelError(f"8-bit cache: pages of {page_size} positions are no whole blocks of {self.KV8_BLOCK}")
         if d % 16 or d <= 0 or d > 256:
             raise KernelError(f"8-bit cache: head size {d} is no multiple of 16 up to 256")
-        if codes.dim() < 1 or codes[0].numel() != 2 * nkv * page_size * d or codes.shape[0] == 0:
-            raise KernelError(f"8-bit cache: pages of {tuple(codes.shape)} do not fit {nkv} heads of {d} and {page_size} positions")
-        if tuple(words.shape) != (codes.shape[0], nkv, page_size // self.KV8_BLOCK, 2):
+        shape = codes.shape
+        pages = shape[0] if shape else 0
+        if not pages or codes.numel() != pages * 2 * nkv * page_size * d:
+            raise KernelError(f"8-bit cache: pages of {tuple(shape)} do not fit {nkv} heads of {d} and {page_size} positions")
+        if words.shape != (pages, nkv, page_size // self.KV8_BLOCK, 2):
             raise KernelError(f"8-bit cache: words {tuple(words.shape)}, expected {(codes.shape[0], nkv, page_size // self.KV8_BLOCK, 2)}")
 
     def rope_kv8_write(self, qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optional[torch.Tensor], rot: int,
@@ -922,8 +931,7 @@ class CudaOps:
         Rows of the same 16 positions stand next to each other, no slot twice (a request's tokens do); rows with a slot that is
         negative or behind the pool write nothing."""
         self._want(qkv, "qkv")
-        self._want(positions, "positions", torch.int32)
-        self._want(slots, "slots", torch.int32)
+        self._want_all(torch.int32, positions=positions, slots=slots)
         self._want_kv8(codes, words, nkv, d, page_size)
         if qkv.dim() != 2 or qkv.shape[1] != (nq + 2 * nkv) * d:
             raise KernelError(f"qkv is {tuple(qkv.shape)}, expected rows of {(nq + 2 * nkv) * d} elements")
@@ -949,11 +957,12 @@ class CudaOps:
         contexts = np.ascontiguousarray(np.asarray(contexts, dtype=np.int64).reshape(-1))
         if block_table.dim() != 2 or contexts.size > block_table.shape[0]:
             raise KernelError(f"read_kv8: {contexts.size} requests, the table has {tuple(block_table.shape)} entries")
-        for r, n in enumerate(contexts):
-            if not 0 <= n <= block_table.shape[1] * page_size:
-                raise KernelError(f"read_kv8: a request of {n} tokens does not fit its row of the table")
+        total = 0
+        if contexts.size:
+            low, high, total = int(contexts.min()), int(contexts.max()), int(contexts.sum())
+            if low < 0 or high > block_table.shape[1] * page_size:
+                raise KernelError(f"read_kv8: a request of {low if low < 0 else high} tokens does not fit its row of the table")
         contexts = contexts.astype(np.int32)
-        total = int(contexts.sum(dtype=np.int64))
         out = self.empty((total, 2, nkv, d), dtype)
         fn = getattr(self.lib, "ptl_read_kv8" + _suffix(dtype))
         self._check(fn(_p(out), _p(codes), _p(words), _p(block_table), contexts.ctypes.data, contexts.size, block_table.shape[1], nkv, d,
@@ -968,11 +977,10 @@ class CudaOps:
         to no other; a position without a page is not seen; a row without a request or without keys is zeros."""
         self._want(q, "q")
         self._want_kv8(codes, words, nkv, d, page_size)
-        for name, t in (("block_table", block_table), ("tok_req", tok_req), ("positions", positions)):
-            self._want(t, name, torch.int32)
-        tokens = q.shape[0]
+        self._want_all(torch.int32, block_table=block_table, tok_req=tok_req, positions=positions)
         if q.dim() != 2 or q.shape[1] < nq * d or nq <= 0 or nq % nkv:
             raise KernelError(f"paged_attention8: q {tuple(q.shape)} for {nq} heads of {d} over {nkv} kv heads")
+        tokens = q.shape[0]
         if block_table.dim() != 2:
             raise KernelError(f"paged_attention8: the block table is {tuple(block_table.shape)}, expected a row per request")
         if tok_req.numel() < tokens or positions.numel() < tokens:
@@ -1010,19 +1018,21 @@ class CudaOps:
             pairs = n * nkv
             fit = self.DECODE_UNITS[d]               # blocks that fit at once
             parts = max(1, min(8, 296 // pairs, -(-longest // 128)))
-            per_head, units, counters, part_acc, part_ml = 0, None, None, None, None
+            per_head, units, counters, part_acc, part_ml, group = 0, None, None, None, None, nq // nkv
             if (parts < 2 or longest > 1024 * parts) and pairs <= fit * 7 // 8 and longest > 64:
                 per_head = max(fit // nkv, n)
-                units, counters = self._decode8_unit_list(dec, tok_req, positions, q.shape[0], nq, nkv, d, window, per_head)
+                units = self._decode8_unit_list(dec, tok_req, positions, q.shape[0], nq, nkv, d, window, per_head)
                 per_head = per_head if units is not None else 0
                 parts = 1
             if per_head:
-                part_acc = self.empty((nkv * per_head, nq // nkv, d), torch.float32)
-                part_ml = self.empty((nkv * per_head, nq // nkv, 2), torch.float32)
+                scratch = self.empty((nkv * per_head * group * (d + 2),), torch.float32)      # partial outputs, then their maxima and sums
+                part_acc = scratch.data_ptr()
+                part_ml = part_acc + nkv * per_head * group * d * 4
+                counters = units.data_ptr() + nkv * per_head * 32
             rc = getattr(self.lib, "ptl_attention8_single" + suffix)(
-                _p(out), _p(part_acc), _p(part_ml), _p(q), _p(codes), _p(words), _p(block_table), None if dec.in_order else _p(dec.tensor),
-                _p(tok_req), _p(positions), n, q.shape[1], nq * d, block_table.shape[1], nq, nkv, d, page_size, scale, window, parts, per_head,
-                _p(units), _p(counters), codes.shape[0], _p(self._tc_status_word()), stream)
+                out.data_ptr(), part_acc, part_ml, q.data_ptr(), codes.data_ptr(), words.data_ptr(), block_table.data_ptr(),
+                None if dec.in_order else dec.tensor.data_ptr(), tok_req.data_ptr(), positions.data_ptr(), n, q.shape[1], nq * d,
+                block_table.shape[1], nq, nkv, d, page_size, scale, window, parts, per_head, _p(units), counters, codes.shape[0], _p(self._tc_status_word()), stream)
             if rc == -2:
                 return False
             self._check(rc)
@@ -1034,58 +1044,62 @@ class CudaOps:
         return True
 
     def _decode8_unit_list(self, dec, tok_req, positions, rows: int, nq: int, nkv: int, d: int, window: int, per_head: int):
-        """(the units of the step's single tokens, their counters, zero): as ``_decode_unit_list``, with counters that belong to the list."""
+        """The units of the step's single tokens, 8 integers each, and behind them a counter per (row, kv head), zero: as ``_decode_unit_list``, but
+        the counters belong to the list, so that calls on several streams and several captured graphs have their own."""
         memo = getattr(self, "_units8_memo", None)
         stream = self._stream()
         integers, key = (dec.tensor, tok_req, positions), None
         if memo is not None and not any(t.is_inference() for t in integers):
             key = (stream, dec.items, dec.in_order, *(x for t in integers for x in (t.data_ptr(), t._version)), rows, nq, nkv, d, int(window), per_head)
             if key in memo:
-                return memo[key][:2]
-        units, counters = self.empty((nkv * per_head, 8), torch.int32), self.empty((rows * nkv,), torch.int32)
-        rc = self.lib.ptl_decode_units_zeroed(_p(units), _p(counters), counters.numel(), None if dec.in_order else _p(dec.tensor), _p(tok_req),
-                                              _p(positions), dec.items, nq, nkv, d, int(window), per_head, stream)
+                return memo[key][0]
+        units = self.empty((nkv * per_head * 8 + rows * nkv,), torch.int32)
+        rc = self.lib.ptl_decode_units_zeroed(units.data_ptr(), units.data_ptr() + nkv * per_head * 32, rows * nkv,
+                                              None if dec.in_order else _p(dec.tensor), _p(tok_req), _p(positions), dec.items, nq, nkv, d,
+                                              int(window), per_head, stream)
         if rc == -2:
-            return None, None
+            return None
         self._check(rc)
         if key is not None:
-            memo[key] = (units, counters, *integers)         # (held, so that their addresses are not given out again)
-        return units, counters
+            memo[key] = (units, *integers)                   # (held, so that their addresses are not given out again)
+        return units
 
     # ------------------------------------------------------------------ pages
     def copy_pages(self, tensors, src, dst) -> None:
         """tensor[dst[i]] = tensor[src[i]] for every i and every one of ``tensors`` (any types, rows of any size, at least as many
         rows as the largest index says), in one launch.  ``src`` and ``dst`` are host integers; no row is written twice, and none that is
         read is written."""
-        src = np.ascontiguousarray(np.asarray(src, dtype=np.int64).reshape(-1))
-        dst = np.ascontiguousarray(np.asarray(dst, dtype=np.int64).reshape(-1))
-        if src.size != dst.size:
-            raise KernelError(f"copy_pages: {src.size} rows to read, {dst.size} to write")
-        tensors = list(tensors)
-        if not src.size or not tensors:
+        if not isinstance(src, list) or not isinstance(dst, list):
+            src, dst = (np.asarray(x, dtype=np.int64).reshape(-1).tolist() for x in (src, dst))
+        n = len(src)
+        if n != len(dst):
+            raise KernelError(f"copy_pages: {n} rows to read, {len(dst)} to write")
+        if not n or not tensors:
             return
-        seen = np.unique(dst)
-        if seen.size != dst.size:
+        written = set(dst)
+        if len(written) != n:
             raise KernelError("copy_pages: a row is written twice")
-        if np.isin(src, seen, assume_unique=False).any():
+        if not written.isdisjoint(src):
             raise KernelError("copy_pages: a row that is read is written too")
-        low, high = int(min(src.min(), dst.min())), int(max(src.max(), dst.max()))
+        low, high = min(min(src), min(dst)), max(max(src), max(dst))
+        held, device = [], self.device
         for t in tensors:
-            self._want(t, "a tensor of pages")
-            if t.dim() < 1 or low < 0 or high >= t.shape[0] or high > 0x7fffffff:
+            if not t.is_contiguous() or t.device != device:
+                self._want(t, "a tensor of pages")
+            rows = t.shape[0] if t.dim() else 0
+            if low < 0 or high >= rows or high > 0x7fffffff:
                 raise KernelError(f"copy_pages: rows {low}..{high} of a tensor {tuple(t.shape)}")
-        starts = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel()]
-        starts.sort()
-        if any(a[1] > b[0] for a, b in zip(starts, starts[1:])):
+            size = t.nbytes
+            if size:
+                held.append((t.data_ptr(), size, size // rows))
+        in_order = sorted(held)
+        if any(a[0] + a[1] > b[0] for a, b in zip(in_order, in_order[1:])):
             raise KernelError("copy_pages: two tensors share memory")
-        held = [t for t in tensors if t.numel()]
-        n = len(held)
-        base = (_ptr * n)(*(t.data_ptr() for t in held))
-        row = (_c_ll * n)(*(t.numel() // t.shape[0] * t.element_size() for t in held))
-        src32, dst32 = src.astype(np.int32), dst.astype(np.int32)
+        k = len(held)
         launches = _c_int(0)
-        rc = self.lib.ptl_copy_pages(base, row, n, src32.ctypes.data, dst32.ctypes.data, src32.size, ctypes.byref(launches), self._stream())
-        self._check(rc, kernels=launches.value)
+        self._check(self.lib.ptl_copy_pages((_ptr * k)(*[x[0] for x in held]), (_c_ll * k)(*[x[2] for x in held]), k, (_c_int * n)(*src), (_c_int * n)(*dst),
+                                            n, ctypes.byref(launches), self._stream()), kernels=0)
+        self.launches += launches.value
 
     def begin_forward(self) -> None:
         """Called by the model at the start of every forward pass: what was worked out for the last
@@ -2568,8 +2582,8 @@ class CudaOps:
         ``top`` most likely tokens [rows, k] and the tokens, int32 [rows, k]), k = min(top, vocabulary), best first, of
         equal logits the lowest index first; ``top`` up to 32.  A token outside the vocabulary has -inf.  A row without a
         distribution (a NaN, +inf, or -inf only) has NaN log-probabilities and entropy; its alternatives are the largest logits, NaN last."""
-        self._want(logits, "logits", torch.float32)
-        self._want(tokens, "tokens", torch.int32)
+        self._want_all(torch.float32, logits=logits)
+        self._want_all(torch.int32, tokens=tokens)
         if logits.dim() != 2 or logits.shape[1] == 0:
             raise KernelError(f"token_scores: logits are {tuple(logits.shape)}, expected [rows, vocabulary]")
         rows, vocab = logits.shape
@@ -2577,12 +2591,12 @@ class CudaOps:
             raise KernelError(f"token_scores: {tokens.numel()} tokens for {rows} rows")
         if not 0 <= top <= self.SCORES_MAX_TOP:
             raise KernelError(f"token_scores: {top} alternatives, at most {self.SCORES_MAX_TOP}")
-        k = min(int(top), vocab)
-        scores = self.empty((2, rows), torch.float32)
-        best, ids = self.empty((rows, k), torch.float32), self.empty((rows, k), torch.int32)
-        self._check(self.lib.ptl_token_scores(_p(scores[0]), _p(scores[1]), _p(best), _p(ids), _p(logits), _p(tokens), rows, vocab, k,
-                                              self._stream()), kernels=1 if rows else 0)
-        return scores[0], scores[1], best, ids
+        k, device = min(int(top), vocab), self.device
+        logprob, entropy = torch.empty((rows,), dtype=torch.float32, device=device), torch.empty((rows,), dtype=torch.float32, device=device)
+        best, ids = torch.empty((rows, k), dtype=torch.float32, device=device), torch.empty((rows, k), dtype=torch.int32, device=device)
+        self._check(self.lib.ptl_token_scores(logprob.data_ptr(), entropy.data_ptr(), best.data_ptr(), ids.data_ptr(), logits.data_ptr(),
+                                              tokens.data_ptr(), rows, vocab, k, self._stream()), kernels=1 if rows else 0)
+        return logprob, entropy, best, ids
 
     def sample_tokens(self, logits: torch.Tensor, temperature: Optional[torch.Tensor], top_p: Optional[torch.Tensor],
                       u: Optional[torch.Tensor], out: Optional[torch.Tensor] = None, logprobs: bool = False):
