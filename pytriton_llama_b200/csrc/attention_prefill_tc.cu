@@ -35,6 +35,9 @@
 // Waits are bounded as in the matrix product: a wait that gives up records a code in *status and
 // the block drains.
 //
+// HOLES: pages may be missing in the middle of a request (an 8-bit cache's portions, kv8.cu, come here with their pages made bfloat16
+// in a place of their own).  A missing page's keys are masked, and the last page of the cache, zeros, is fetched in its place.
+//
 // tiles[2j], tiles[2j+1] = {request row, first token index, rows, position of the first token};
 // the second entry either continues the first (same request, first token and position + 128) or
 // has rows == 0.
@@ -103,7 +106,7 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 
-template <int D>
+template <int D, bool HOLES>
 __global__ void __launch_bounds__(PfCfg<D>::kThreads)
 prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv,
                             const PrefillTcParams p) {
@@ -189,9 +192,13 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
   const bool staged = n_blocks <= kTcStagedPages;
   if (staged)
     for (int i = threadIdx.x; i < n_blocks; i += Cfg::kThreads) s_pages[i] = i < have_blocks ? bt_global[first_block + i] : -1;
+  int holes = 0;
+  if (HOLES)
+    for (int i = threadIdx.x; i < have_blocks; i += Cfg::kThreads) holes |= bt_global[first_block + i] < 0;
   for (int i = threadIdx.x; i < Cfg::kExchangeBytes / 8; i += Cfg::kThreads) s_xchg[i] = 0ull;      // sequence numbers start at 0
   tcgen05_fence_before();
-  __syncthreads();
+  if (HOLES) holes = __syncthreads_or(holes);
+  else __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
@@ -259,7 +266,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       for (int i = 0; i < pages_per_tile; ++i) {
         const int bi = t * pages_per_tile + i;
         int page = staged ? s_pages[bi] : (bi < have_blocks ? bt_global[first_block + bi] : -1);
-        if (page < 0 || page >= p.num_pages) page = 0;             // beyond the request: any page, its keys get masked
+        if (page < 0 || page >= p.num_pages) page = HOLES ? p.num_pages - 1 : 0;      // beyond the request: any page, its keys get masked
         const int krow = (page * 2 * p.nkv + kvh) * p.page_size;
         const uint32_t off = (uint32_t)i * p.page_size * 128u;
 #pragma unroll
@@ -402,7 +409,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       tcgen05_fence_after();
       const int key0 = k_base + t * kTcKeys;
       const bool need_mask = key0 + kTcKeys - 1 > tile_pos0 || key0 < lo_raw[g] ||
-                             (p.window > 0 && key0 < tile_pos0 + kTcRows - 1 - p.window + 1);
+                             (p.window > 0 && key0 < tile_pos0 + kTcRows - 1 - p.window + 1) || (HOLES && holes);
       // the row's scores come out of TMEM once and stay in registers
       uint32_t v[kMyKeys];
 #pragma unroll
@@ -423,6 +430,10 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
           const int key = key0 + col0 + j;
           float x = __uint_as_float(v[j]);
           if (key > qpos || (p.window > 0 && key < qpos - p.window + 1)) x = -INFINITY;
+          if (HOLES && holes) {
+            const int bi = t * pages_per_tile + (col0 + j) / p.page_size;
+            if (bi < have_blocks && bt_global[first_block + bi] < 0) x = -INFINITY;
+          }
           v[j] = __float_as_uint(x);
           mx8[j & 7] = fmaxf(mx8[j & 7], x);
         }
@@ -566,18 +577,18 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
 
 namespace ptl {
 
-template <int D>
+template <int D, bool HOLES = false>
 static int launch_prefill_tc(const void* q, const void* cache, int n_tiles, int n_tokens, int q_stride, int nq, int nkv,
                              int page_size, int num_pages, const PrefillTcParams& p, cudaStream_t stream) {
   using Cfg = PfCfg<D>;
   static SmemRaised raised = {};
-  if (int rc = raise_shared_memory("prefill_attention_tc", prefill_attention_tc_kernel<D>, Cfg::kSmem, raised)) return rc;
+  if (int rc = raise_shared_memory("prefill_attention_tc", prefill_attention_tc_kernel<D, HOLES>, Cfg::kSmem, raised)) return rc;
   CUtensorMap mq, mkv;
   int rc = make_map(&mq, q, n_tokens, q_stride, kTcRows);                 // whole step: [tokens, q_stride], boxes of 64 x 128
   if (rc) return rc;
   rc = make_map(&mkv, cache, num_pages * 2 * nkv * page_size, D, page_size);     // cache as rows of one head's D values, boxes of 64 x page
   if (rc) return rc;
-  return launch_kernel("prefill_attention_tc", prefill_attention_tc_kernel<D>, dim3(nq, n_tiles / 2), dim3(Cfg::kThreads), Cfg::kSmem,
+  return launch_kernel("prefill_attention_tc", prefill_attention_tc_kernel<D, HOLES>, dim3(nq, n_tiles / 2), dim3(Cfg::kThreads), Cfg::kSmem,
                        stream, mq, mkv, p);
 }
 
@@ -587,10 +598,10 @@ static int launch_prefill_tc(const void* q, const void* cache, int n_tiles, int 
 // warp-level kernel): head size 64 or 128 only, pages of 8 keys or more that divide the key tile
 // (128 keys with head size 64, 64 with 128), 16-byte aligned rows; -1 on an error.  `tiles` holds
 // n_tiles entries in pairs (n_tiles is even): see the top of the file.
-PTL_EXPORT int ptl_prefill_attention_tc_bf16(void* out, const void* q, const void* cache, const int* block_table,
-                                             const int* tiles, int n_tiles, int n_tokens, int q_stride, int out_stride,
-                                             int bt_stride, int nq, int nkv, int d, int page_size, float scale,
-                                             int window, int num_pages, int* status, void* stream) {
+static int prefill_attention_tc_entry(void* out, const void* q, const void* cache, const int* block_table,
+                                      const int* tiles, int n_tiles, int n_tokens, int q_stride, int out_stride,
+                                      int bt_stride, int nq, int nkv, int d, int page_size, float scale,
+                                      int window, int num_pages, bool holes, int* status, void* stream) {
   using namespace ptl;
   PTL_REQUIRE(n_tiles >= 0 && nq > 0 && nkv > 0 && page_size > 0 && num_pages > 0, "prefill_attention_tc: bad sizes");
   PTL_REQUIRE(n_tiles % 2 == 0, "prefill_attention_tc: tiles come in pairs, %d is odd", n_tiles);
@@ -605,6 +616,26 @@ PTL_EXPORT int ptl_prefill_attention_tc_bf16(void* out, const void* q, const voi
   p.out = (__nv_bfloat16*)out; p.block_table = block_table; p.tiles = tiles; p.status = status;
   p.out_stride = out_stride; p.bt_stride = bt_stride; p.nq = nq; p.nkv = nkv; p.page_size = page_size;
   p.window = window; p.num_pages = num_pages; p.scale_log2 = scale * 1.4426950408889634f;
+  if (holes)
+    return d == 64 ? launch_prefill_tc<64, true>(q, cache, n_tiles, n_tokens, q_stride, nq, nkv, page_size, num_pages, p, as_stream(stream))
+                   : launch_prefill_tc<128, true>(q, cache, n_tiles, n_tokens, q_stride, nq, nkv, page_size, num_pages, p, as_stream(stream));
   if (d == 64) return launch_prefill_tc<64>(q, cache, n_tiles, n_tokens, q_stride, nq, nkv, page_size, num_pages, p, as_stream(stream));
   return launch_prefill_tc<128>(q, cache, n_tiles, n_tokens, q_stride, nq, nkv, page_size, num_pages, p, as_stream(stream));
+}
+
+PTL_EXPORT int ptl_prefill_attention_tc_bf16(void* out, const void* q, const void* cache, const int* block_table,
+                                             const int* tiles, int n_tiles, int n_tokens, int q_stride, int out_stride,
+                                             int bt_stride, int nq, int nkv, int d, int page_size, float scale,
+                                             int window, int num_pages, int* status, void* stream) {
+  return prefill_attention_tc_entry(out, q, cache, block_table, tiles, n_tiles, n_tokens, q_stride, out_stride, bt_stride, nq, nkv, d, page_size,
+                                    scale, window, num_pages, false, status, stream);
+}
+
+// The same where pages may be missing (-1) in the middle of a request; the cache's last page is zeros.
+PTL_EXPORT int ptl_prefill_attention_tc_holes_bf16(void* out, const void* q, const void* cache, const int* block_table,
+                                                   const int* tiles, int n_tiles, int n_tokens, int q_stride, int out_stride,
+                                                   int bt_stride, int nq, int nkv, int d, int page_size, float scale,
+                                                   int window, int num_pages, int* status, void* stream) {
+  return prefill_attention_tc_entry(out, q, cache, block_table, tiles, n_tiles, n_tokens, q_stride, out_stride, bt_stride, nq, nkv, d, page_size,
+                                    scale, window, num_pages, true, status, stream);
 }

@@ -200,6 +200,10 @@ def load_library() -> ctypes.CDLL:
     lib.ptl_prefill_attention_tc_bf16.argtypes = [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                                   _c_int, _c_int, _c_int, _c_f, _c_int, _c_int, _ptr, _ptr]
     lib.ptl_prefill_attention_tc_bf16.restype = _c_int
+    lib.ptl_prefill_attention_tc_holes_bf16.argtypes = lib.ptl_prefill_attention_tc_bf16.argtypes
+    lib.ptl_prefill_attention_tc_holes_bf16.restype = _c_int
+    lib.ptl_kv8_expand_bf16.argtypes = [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr]
+    lib.ptl_kv8_expand_bf16.restype = _c_int
     lib.ptl_argmax.argtypes = [_ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_ll, _ptr]
     lib.ptl_argmax.restype = _c_int
     lib.ptl_take_tokens.argtypes = [_ptr, _ptr, _ptr, _c_int, _c_int, _ptr]
@@ -1037,10 +1041,36 @@ class CudaOps:
                 return False
             self._check(rc)
         if tiles.items:
+            if q.dtype == torch.bfloat16 and self._attention8_portions(out, q, codes, words, block_table, nq, nkv, d, page_size, scale, window,
+                                                                       tiles, stream):
+                return True
             rc = getattr(self.lib, "ptl_attention8_portion" + suffix)(
                 _p(out), _p(q), _p(codes), _p(words), _p(block_table), _p(tiles.tensor), tiles.items, q.shape[1], nq * d, block_table.shape[1],
                 nq, nkv, d, page_size, scale, window, codes.shape[0], _p(self._tc_status_word()), stream)
             self._check(rc)
+        return True
+
+    KV8_EXPAND_BYTES = 1 << 30       # of pages made bfloat16 for one call, at most
+
+    def _attention8_portions(self, out, q, codes, words, block_table, nq, nkv, d, page_size, scale, window, tiles, stream) -> bool:
+        """bfloat16 portions on the fifth-generation tensor cores, over the pages they see made bfloat16 first; False where they are too many
+        (a captured step counts its longest contexts) or of a size that those tiles do not take."""
+        keys = 128 if d == 64 else 64
+        if page_size > keys or keys % page_size or tiles.items // 2 > 65535:
+            return False
+        requests, width = block_table.shape
+        slots = min(requests, tiles.items // 2)
+        pages = slots * width + 1
+        if pages * 4 * nkv * page_size * d > self.KV8_EXPAND_BYTES:
+            return False
+        place = self.empty((pages * 2 * nkv * page_size * d,), torch.bfloat16)
+        table = self.empty((requests, width), torch.int32)
+        self._check(self.lib.ptl_kv8_expand_bf16(place.data_ptr(), table.data_ptr(), codes.data_ptr(), words.data_ptr(), block_table.data_ptr(),
+                                                 tiles.tensor.data_ptr(), tiles.items, slots, width, width, nkv, d, page_size, codes.shape[0],
+                                                 window, stream))
+        self._check(self.lib.ptl_prefill_attention_tc_holes_bf16(out.data_ptr(), q.data_ptr(), place.data_ptr(), table.data_ptr(), tiles.tensor.data_ptr(),
+                                                                 tiles.items, q.shape[0], q.shape[1], nq * d, width, nq, nkv, d, page_size, scale,
+                                                                 window, pages, self._tc_status_word().data_ptr(), stream))
         return True
 
     def _decode8_unit_list(self, dec, tok_req, positions, rows: int, nq: int, nkv: int, d: int, window: int, per_head: int):

@@ -72,12 +72,13 @@ def attend(q, values, bad, positions, scale, window=0):
     return out, size, score
 
 
-def tolerance(dtype, out, size, score, d, keys):
-    """How far a kernel may be off: the output's rounding, half a step of the type; weights rounded to half floats, 2^-11 of each
-    (and 2^-25 of the largest where they leave the normal numbers, keys of them at most); 2 eps for a relative error eps of
+def tolerance(dtype, out, size, score, d, keys, weights=torch.float16):
+    """How far a kernel may be off: the output's rounding, half a step of the type; weights rounded to ``weights`` (bfloat16 rows: half floats for
+    single tokens, bfloat16 for portions on the fifth-generation tensor cores), half a step of each, 2^-11 or 2^-8
+    (and 2^-25 of the largest where half floats leave the normal numbers, keys of them at most); 2 eps for a relative error eps of
     e^s, where a score's d products and sums in float32, two more for its scale and the exponential's few ulps, err by
     (d + 8) 2^-24 of |q| |k| scale; and the float32 sums over the keys."""
     half = torch.finfo(dtype).eps / 2
     eps = (d + 8) * 2.0 ** -24 * (1 + score[..., None])
-    rounding = 2.0 ** -11 + keys * 2.0 ** -25 if dtype == torch.bfloat16 else 2.0 ** -22
+    rounding = torch.finfo(weights).eps / 2 + keys * 2.0 ** -25 if dtype == torch.bfloat16 else 2.0 ** -22
     return half * out.abs() + size * (2 * eps + 2 * rounding + (keys + 64) * 2.0 ** -24) + 1e-30
