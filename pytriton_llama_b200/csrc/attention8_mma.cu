@@ -45,7 +45,7 @@ struct A8Params {
   const int* positions;
   const int4* units;
   int* status;
-  int q_stride, out_stride, bt_stride, nq, nkv, blocks_per_page, page_shift, num_pages, window, splits, cluster;
+  int q_stride, out_stride, bt_stride, nq, nkv, blocks_per_page, page_shift, num_pages, window, splits, cluster;      // (portions: splits of their keys)
   float scale_log2;
 
   __device__ __forceinline__ int page_of(const int* table, int block) const {
@@ -674,7 +674,9 @@ attention8_portion_kernel(const A8Params p) {
   if (tokens <= 0) return;
   const int t0 = tl[1] + sub * per_block, pos0 = tl[3] + sub * per_block;
   const int lo = p.window > 0 && pos0 + 1 > p.window ? pos0 + 1 - p.window : 0;
-  const int begin = lo / kKv8Block, end = (pos0 + tokens - 1) / kKv8Block + 1;
+  const int begin0 = lo / kKv8Block, all = (pos0 + tokens - 1) / kKv8Block + 1 - begin0;
+  const int per_split = ((all + p.splits - 1) / p.splits + kA8Turn - 1) / kA8Turn * kA8Turn;
+  const int begin = begin0 + min(all, (int)blockIdx.z * per_split), end = begin0 + min(all, ((int)blockIdx.z + 1) * per_split);
   const int turns = (end - begin + kA8Turn - 1) / kA8Turn;
   const int* table = p.block_table + (size_t)tl[0] * p.bt_stride;
   auto page_at = [&](int i) { return begin + i < end ? p.page_of(table, begin + i) : -1; };      // of the block's i-th block of keys
@@ -758,6 +760,15 @@ attention8_portion_kernel(const A8Params p) {
     for (int j = 0; j < 2; ++j) {
       const int row = 8 * n + 2 * c + j;
       if (row >= my_tokens * group) continue;
+      if (p.splits > 1) {
+        const size_t at = ((size_t)(my_t0 + row / group) * p.nq + kvh * group + row % group) * p.splits + blockIdx.z;
+#pragma unroll
+        for (int i = 0; i < D / 8; i += 4)
+          *reinterpret_cast<float4*>(p.part_acc + at * D + g * (D / 8) + i) =
+              make_float4(rows.entry(n, j, i), rows.entry(n, j, i + 1), rows.entry(n, j, i + 2), rows.entry(n, j, i + 3));
+        if (g == 0) { p.part_ml[2 * at] = rows.m[n][j]; p.part_ml[2 * at + 1] = rows.l[n][j]; }
+        continue;
+      }
       const float inv = a8_inverse(rows.l[n][j]);
       T* dst = static_cast<T*>(p.out) + (size_t)(my_t0 + row / group) * p.out_stride + (size_t)(kvh * group + row % group) * D + g * (D / 8);
 #pragma unroll
@@ -768,6 +779,43 @@ attention8_portion_kernel(const A8Params p) {
         store16(dst + i, v);
       }
     }
+}
+
+// The splits of portions joined: a warp a row of the tiles and query head.
+template <int D, typename T>
+__global__ void __launch_bounds__(kA8Warps * 32)
+attention8_join_kernel(const A8Params p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int* tl = p.items + 4 * blockIdx.y;
+  const int i = blockIdx.x * kA8Warps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (i / p.nq >= tl[2]) return;
+  const size_t row = (size_t)(tl[1] + i / p.nq), at = (row * p.nq + i % p.nq) * p.splits;
+  float M = -INFINITY, L = 0.f, acc[D / 32];
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) acc[k] = 0.f;
+  for (int z = 0; z < p.splits; ++z) M = fmaxf(M, __ldg(p.part_ml + 2 * (at + z)));
+#pragma unroll 4
+  for (int z = 0; z < p.splits; ++z) {
+    const float m = __ldg(p.part_ml + 2 * (at + z)), l = __ldg(p.part_ml + 2 * (at + z) + 1), f = a8_weight(m, l, M);
+    if (l == 0.f) continue;
+    L = fmaf(f, l, L);
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) acc[k] = fmaf(f, __ldg(p.part_acc + (at + z) * D + k * 32 + lane), acc[k]);
+  }
+  const float inv = a8_inverse(L);
+  T* dst = static_cast<T*>(p.out) + row * p.out_stride + (size_t)(i % p.nq) * D + lane;
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) dst[k * 32] = from_f32<T>(acc[k] * inv);
+}
+
+int attention8_join_bf16(void* out, const float* part_acc, const float* part_ml, const int* tiles, int n_tiles, int out_stride, int nq, int d, int splits,
+                         void* stream) {
+  A8Params p{};
+  p.out = out; p.part_acc = const_cast<float*>(part_acc); p.part_ml = const_cast<float*>(part_ml); p.items = tiles;
+  p.out_stride = out_stride; p.nq = nq; p.splits = splits;
+  return launch_kernel("attention8_join", d == 64 ? attention8_join_kernel<64, __nv_bfloat16> : attention8_join_kernel<128, __nv_bfloat16>,
+                       dim3((128 * nq + kA8Warps - 1) / kA8Warps, n_tiles), dim3(kA8Warps * 32), 0, as_stream(stream), p);
 }
 
 template <int D, typename T, int NT>
@@ -791,8 +839,10 @@ static int launch_attention8(const A8Params& p, int singles, int tiles, int per_
   static SmemRaised raised = {};
   if (int rc = raise_shared_memory("attention8_portion", attention8_portion_kernel<D, T>, Cfg::kSmem, raised)) return rc;
   const int per_block = 8 * Cfg::kTiles / group * kA8Warps;
-  return launch_kernel("attention8_portion", attention8_portion_kernel<D, T>, dim3(p.nkv * ((128 + per_block - 1) / per_block), tiles),
-                       dim3(kA8Warps * 32), Cfg::kSmem, stream, p);
+  if (int rc = launch_kernel("attention8_portion", attention8_portion_kernel<D, T>, dim3(p.nkv * ((128 + per_block - 1) / per_block), tiles, p.splits),
+                             dim3(kA8Warps * 32), Cfg::kSmem, stream, p)) return rc;
+  if (p.splits == 1) return 0;
+  return launch_kernel("attention8_join", attention8_join_kernel<D, T>, dim3((128 * p.nq + kA8Warps - 1) / kA8Warps, tiles), dim3(kA8Warps * 32), 0, stream, p);
 }
 
 template <typename T>
@@ -803,7 +853,8 @@ static int attention8_mma(A8Params p, int singles, int tiles, int d, int page_si
   if ((d != 64 && d != 128) || p.nq / p.nkv > 16 || tiles > 65535 || p.q_stride % 8 || p.out_stride % 8) return -2;
   PTL_REQUIRE(aligned16(p.q) && aligned16(p.out) && aligned16(p.codes) && (reinterpret_cast<uintptr_t>(p.words) & 7u) == 0,
               "attention8: q, out and codes must be 16-byte and words 8-byte aligned");
-  PTL_REQUIRE(p.splits >= 1 && (!p.cluster || p.splits <= 8), "attention8: a cluster has up to 8 parts");
+  PTL_REQUIRE(p.splits >= 1 && (!p.cluster || p.splits <= 8) && p.splits <= 65535, "attention8: a cluster has up to 8 parts");
+  PTL_REQUIRE(tiles == 0 || p.splits == 1 || (p.part_acc && p.part_ml), "attention8: splits > 1 need scratch buffers");
   PTL_REQUIRE(per_head == 0 || (p.units && aligned16(p.units) && p.counters && p.part_acc && p.part_ml), "attention8: units need their list and scratch");
   PTL_REQUIRE(p.status != nullptr, "attention8: needs a status word");
   p.blocks_per_page = page_size / kKv8Block;
@@ -819,6 +870,7 @@ static int attention8_mma(A8Params p, int singles, int tiles, int d, int page_si
 // ptl_decode_units_zeroed with the same sizes and with `counters`, one int per (row, kv head) of q), part_acc [nkv * per_head, nq / nkv, d] and part_ml
 // [..., 2]; else every (token, kv head) has `splits` parts, up to 8, which join in a cluster.  -2: sizes this kernel does not take.
 // *status: raised when a wait for a copy gave up.
+// Portions: with splits > 1 part_acc [rows of q, nq, splits, d] and part_ml [rows of q, nq, splits, 2], float32.
 #define PTL_ATTENTION8_MMA(NAME, T)                                                                                                         \
   PTL_EXPORT int ptl_attention8_single_##NAME(void* out, float* part_acc, float* part_ml, const void* q, const void* codes,                 \
                                               const void* words, const int* block_table, const int* items, const int* tok_req,             \
@@ -830,11 +882,12 @@ static int attention8_mma(A8Params p, int singles, int tiles, int d, int page_si
                     per_head == 0 && splits > 1, scale * 1.4426950408889634f};                                                              \
     return ptl::attention8_mma<T>(p, n_items, 0, d, page_size, per_head, stream);                                                           \
   }                                                                                                                                         \
-  PTL_EXPORT int ptl_attention8_portion_##NAME(void* out, const void* q, const void* codes, const void* words, const int* block_table,      \
-                                               const int* tiles, int n_tiles, int q_stride, int out_stride, int bt_stride, int nq, int nkv, \
-                                               int d, int page_size, float scale, int window, int num_pages, int* status, void* stream) {   \
-    ptl::A8Params p{out, nullptr, nullptr, nullptr, q, (const unsigned char*)codes, (const uint32_t*)words, block_table, tiles, nullptr,    \
-                    nullptr, nullptr, status, q_stride, out_stride, bt_stride, nq, nkv, 0, 0, num_pages, window, 1, 0,                      \
+  PTL_EXPORT int ptl_attention8_portion_##NAME(void* out, float* part_acc, float* part_ml, const void* q, const void* codes,                \
+                                               const void* words, const int* block_table, const int* tiles, int n_tiles, int q_stride,      \
+                                               int out_stride, int bt_stride, int nq, int nkv, int d, int page_size, float scale,           \
+                                               int window, int splits, int num_pages, int* status, void* stream) {                          \
+    ptl::A8Params p{out, part_acc, part_ml, nullptr, q, (const unsigned char*)codes, (const uint32_t*)words, block_table, tiles, nullptr,    \
+                    nullptr, nullptr, status, q_stride, out_stride, bt_stride, nq, nkv, 0, 0, num_pages, window, splits, 0,                 \
                     scale * 1.4426950408889634f};                                                                                           \
     return ptl::attention8_mma<T>(p, 0, n_tiles, d, page_size, 0, stream);                                                                  \
   }

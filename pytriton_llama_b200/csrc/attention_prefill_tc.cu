@@ -36,7 +36,9 @@
 // the block drains.
 //
 // HOLES: pages may be missing in the middle of a request (an 8-bit cache's portions, kv8.cu, come here with their pages made bfloat16
-// in a place of their own).  A missing page's keys are masked, and the last page of the cache, zeros, is fetched in its place.
+// in a place of their own).  A missing page's keys are masked, and the last page of the cache, zeros, is fetched in its place.  There too the
+// keys may be split over blockIdx.z where pairs and heads are fewer than SMs (a key tile takes a block 1.3 to 2 us, however few
+// blocks there are): a block leaves its accumulator, maximum and sum, and a kernel of its own joins them.
 //
 // tiles[2j], tiles[2j+1] = {request row, first token index, rows, position of the first token};
 // the second entry either continues the first (same request, first token and position + 128) or
@@ -84,6 +86,9 @@ struct PrefillTcParams {
   int* status;
   int out_stride, bt_stride, nq, nkv, page_size, window, num_pages;
   float scale_log2;
+  int splits;                      // HOLES: of the keys; with more than one
+  float* part_acc;                 // [rows of q][nq][splits][D]
+  float* part_ml;                  // [rows of q][nq][splits][2], the maximum in units of log2
 };
 
 // Barriers (8 bytes each): q_full, per tile of the pair s_full, s_free, p_full and o_done (one of each per P
@@ -151,13 +156,32 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     lo_raw[g] = (p.window > 0 && pos_g[g] - p.window + 1 > 0) ? pos_g[g] - p.window + 1 : 0;
     k_end[g] = pos_g[g] + rows_g[g];
   }
-  const int k_base = lo_raw[0] / p.page_size * p.page_size;    // tiles start on a page boundary
+  int k_base = lo_raw[0] / p.page_size * p.page_size;    // tiles start on a page boundary
+  int tiles_of_split = 0x7fffffff;
+  if (HOLES && p.splits > 1) {
+    const int all = (max(k_end[0], rows_g[1] > 0 ? k_end[1] : 0) - k_base + kTcKeys - 1) / kTcKeys;
+    tiles_of_split = (all + p.splits - 1) / p.splits;
+    k_base += blockIdx.z * tiles_of_split * kTcKeys;
+  }
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
-    t_first[g] = (lo_raw[g] - k_base) / kTcKeys;
-    t_last[g] = rows_g[g] > 0 ? (k_end[g] - k_base + kTcKeys - 1) / kTcKeys : 0;     // one past the last
+    t_first[g] = max(0, lo_raw[g] - k_base) / kTcKeys;
+    t_last[g] = rows_g[g] > 0 ? min(tiles_of_split, max(0, k_end[g] - k_base + kTcKeys - 1) / kTcKeys) : 0;     // one past the last
   }
   const int ntiles = max(t_last[0], t_last[1]);
+  // HOLES: a row of the pair without keys in this split
+  auto no_part = [&](int row) {
+    if (row < 0) return;
+    const size_t at = ((size_t)(tok0 + row) * p.nq + h) * p.splits + blockIdx.z;
+    p.part_ml[2 * at] = -INFINITY;
+    p.part_ml[2 * at + 1] = 0.f;
+  };
+  if (HOLES && p.splits > 1 && ntiles == 0) {
+    pdl_wait();
+    pdl_launch_dependents();
+    for (int i = threadIdx.x; i < 2 * kTcRows; i += Cfg::kThreads) no_part(i % kTcRows < rows_g[i / kTcRows] ? i : -1);
+    return;
+  }
   const int pages_per_tile = kTcKeys / p.page_size;
   const int* bt_global = p.block_table + (size_t)req * p.bt_stride;
   auto takes_part = [&](int g, int t) { return rows_g[g] > 0 && t >= t_first[g] && t < t_last[g]; };
@@ -408,8 +432,16 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       if (!ok) break;
       tcgen05_fence_after();
       const int key0 = k_base + t * kTcKeys;
+      int missing = 0;                                          // a bit for each 16 keys of the tile whose page is
+      if (HOLES && holes) {
+#pragma unroll 1
+        for (int b = 0; b < kTcKeys / 16; ++b) {
+          const int bi = (t * kTcKeys + b * 16) / p.page_size;
+          if (bi < have_blocks && bt_global[first_block + bi] < 0) missing |= 1 << b;
+        }
+      }
       const bool need_mask = key0 + kTcKeys - 1 > tile_pos0 || key0 < lo_raw[g] ||
-                             (p.window > 0 && key0 < tile_pos0 + kTcRows - 1 - p.window + 1) || (HOLES && holes);
+                             (p.window > 0 && key0 < tile_pos0 + kTcRows - 1 - p.window + 1) || (HOLES && missing);
       // the row's scores come out of TMEM once and stay in registers
       uint32_t v[kMyKeys];
 #pragma unroll
@@ -430,10 +462,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
           const int key = key0 + col0 + j;
           float x = __uint_as_float(v[j]);
           if (key > qpos || (p.window > 0 && key < qpos - p.window + 1)) x = -INFINITY;
-          if (HOLES && holes) {
-            const int bi = t * pages_per_tile + (col0 + j) / p.page_size;
-            if (bi < have_blocks && bt_global[first_block + bi] < 0) x = -INFINITY;
-          }
+          if (HOLES && (missing >> ((col0 + j) / 16)) & 1) x = -INFINITY;
           v[j] = __float_as_uint(x);
           mx8[j & 7] = fmaxf(mx8[j & 7], x);
         }
@@ -510,6 +539,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       if (ok) ok = exchange(0, m_run, 0x80000001u, m_other);
       if (ok) ok = exchange(1, l_run, 0x80000002u, l_other);
       if (ok && n > 0) ok = mbar_wait(bar(kBarODone + 2 * g + (hf ^ 1)), (n - 1) & 1, abort_flag, p.status, 21);
+      if (HOLES && p.splits > 1 && ok && n == 0 && r < rows && hf == 0) no_part(g * kTcRows + r);
       if (ok && n > 0) {
         tcgen05_fence_after();
         const float m_all = fmaxf(m_run, m_other);
@@ -519,13 +549,22 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         const float l0 = hf == 0 ? l_run : l_other, l1 = hf == 0 ? l_other : l_run;
         const float l_all = w0 * l0 + w1 * l1;
         const float inv = l_all > 0.f ? 1.0f / l_all : 0.f;
-        const float f0 = w0 * inv, f1 = w1 * inv;
+        const bool parts = HOLES && p.splits > 1;
+        const float f0 = parts ? w0 : w0 * inv, f1 = parts ? w1 : w1 * inv;
         const uint32_t acc0 = tmem_base + 2 * kTcRows + (g * 2) * 64 + lane_addr + d0;
         uint32_t a[32], b[32];
         tmem_load_32_nowait(acc0, a);
         tmem_load_32_nowait(acc0 + 64, b);
         tmem_wait_ld();
-        if (r < rows) {
+        if (parts && r < rows) {
+          const size_t at = ((size_t)(tok0 + g * kTcRows + r) * p.nq + h) * p.splits + blockIdx.z;
+          if (hf == 0) { p.part_ml[2 * at] = m_all; p.part_ml[2 * at + 1] = l_all; }
+          float4* dst = reinterpret_cast<float4*>(p.part_acc + at * kTcD + d0);
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            dst[e / 4] = make_float4(__uint_as_float(a[e]) * f0 + __uint_as_float(b[e]) * f1, __uint_as_float(a[e + 1]) * f0 + __uint_as_float(b[e + 1]) * f1,
+                                     __uint_as_float(a[e + 2]) * f0 + __uint_as_float(b[e + 2]) * f1, __uint_as_float(a[e + 3]) * f0 + __uint_as_float(b[e + 3]) * f1);
+        } else if (r < rows) {
           __nv_bfloat16* dst = p.out + (size_t)(tok0 + g * kTcRows + r) * p.out_stride + (size_t)h * kTcD + d0;
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4) {
@@ -542,14 +581,25 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
           }
         }
       }
+    } else if (HOLES && p.splits > 1 && ok && n == 0) {
+      if (r < rows) no_part(g * kTcRows + r);
     } else if (ok && n > 0) {
       tcgen05_fence_after();
       const float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
+      const size_t at = ((size_t)(tok0 + g * kTcRows + r) * p.nq + h) * (HOLES ? p.splits : 1) + (HOLES ? blockIdx.z : 0);
+      if (HOLES && p.splits > 1 && r < rows) { p.part_ml[2 * at] = m_run; p.part_ml[2 * at + 1] = l_run; }
 #pragma unroll 1
       for (int c0 = 0; c0 < kTcD; c0 += 32) {
         uint32_t v[32];
         tmem_load_32(tmem_o + lane_addr + c0, v);
-        if (r < rows) {
+        if (HOLES && p.splits > 1) {
+          if (r < rows) {
+            float4* dst = reinterpret_cast<float4*>(p.part_acc + at * kTcD + c0);
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              dst[e / 4] = make_float4(__uint_as_float(v[e]), __uint_as_float(v[e + 1]), __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+          }
+        } else if (r < rows) {
           __nv_bfloat16* dst = p.out + (size_t)(tok0 + g * kTcRows + r) * p.out_stride + (size_t)h * kTcD + c0;
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4) {
@@ -588,8 +638,8 @@ static int launch_prefill_tc(const void* q, const void* cache, int n_tiles, int 
   if (rc) return rc;
   rc = make_map(&mkv, cache, num_pages * 2 * nkv * page_size, D, page_size);     // cache as rows of one head's D values, boxes of 64 x page
   if (rc) return rc;
-  return launch_kernel("prefill_attention_tc", prefill_attention_tc_kernel<D, HOLES>, dim3(nq, n_tiles / 2), dim3(Cfg::kThreads), Cfg::kSmem,
-                       stream, mq, mkv, p);
+  return launch_kernel("prefill_attention_tc", prefill_attention_tc_kernel<D, HOLES>, dim3(nq, n_tiles / 2, HOLES ? p.splits : 1), dim3(Cfg::kThreads),
+                       Cfg::kSmem, stream, mq, mkv, p);
 }
 
 }  // namespace ptl
@@ -601,7 +651,8 @@ static int launch_prefill_tc(const void* q, const void* cache, int n_tiles, int 
 static int prefill_attention_tc_entry(void* out, const void* q, const void* cache, const int* block_table,
                                       const int* tiles, int n_tiles, int n_tokens, int q_stride, int out_stride,
                                       int bt_stride, int nq, int nkv, int d, int page_size, float scale,
-                                      int window, int num_pages, bool holes, int* status, void* stream) {
+                                      int window, int num_pages, bool holes, int splits, float* part_acc, float* part_ml, int* status,
+                                      void* stream) {
   using namespace ptl;
   PTL_REQUIRE(n_tiles >= 0 && nq > 0 && nkv > 0 && page_size > 0 && num_pages > 0, "prefill_attention_tc: bad sizes");
   PTL_REQUIRE(n_tiles % 2 == 0, "prefill_attention_tc: tiles come in pairs, %d is odd", n_tiles);
@@ -616,6 +667,7 @@ static int prefill_attention_tc_entry(void* out, const void* q, const void* cach
   p.out = (__nv_bfloat16*)out; p.block_table = block_table; p.tiles = tiles; p.status = status;
   p.out_stride = out_stride; p.bt_stride = bt_stride; p.nq = nq; p.nkv = nkv; p.page_size = page_size;
   p.window = window; p.num_pages = num_pages; p.scale_log2 = scale * 1.4426950408889634f;
+  p.splits = splits; p.part_acc = part_acc; p.part_ml = part_ml;
   if (holes)
     return d == 64 ? launch_prefill_tc<64, true>(q, cache, n_tiles, n_tokens, q_stride, nq, nkv, page_size, num_pages, p, as_stream(stream))
                    : launch_prefill_tc<128, true>(q, cache, n_tiles, n_tokens, q_stride, nq, nkv, page_size, num_pages, p, as_stream(stream));
@@ -628,14 +680,26 @@ PTL_EXPORT int ptl_prefill_attention_tc_bf16(void* out, const void* q, const voi
                                              int bt_stride, int nq, int nkv, int d, int page_size, float scale,
                                              int window, int num_pages, int* status, void* stream) {
   return prefill_attention_tc_entry(out, q, cache, block_table, tiles, n_tiles, n_tokens, q_stride, out_stride, bt_stride, nq, nkv, d, page_size,
-                                    scale, window, num_pages, false, status, stream);
+                                    scale, window, num_pages, false, 1, nullptr, nullptr, status, stream);
 }
 
-// The same where pages may be missing (-1) in the middle of a request; the cache's last page is zeros.
+namespace ptl {
+// defined in attention8_mma.cu
+int attention8_join_bf16(void* out, const float* part_acc, const float* part_ml, const int* tiles, int n_tiles, int out_stride, int nq, int d, int splits,
+                         void* stream);
+}  // namespace ptl
+
+// The same where pages may be missing (-1) in the middle of a request; the cache's last page is zeros.  splits > 1: of the keys, with part_acc
+// [n_tokens, nq, splits, d] and part_ml [n_tokens, nq, splits, 2] float32.
 PTL_EXPORT int ptl_prefill_attention_tc_holes_bf16(void* out, const void* q, const void* cache, const int* block_table,
                                                    const int* tiles, int n_tiles, int n_tokens, int q_stride, int out_stride,
                                                    int bt_stride, int nq, int nkv, int d, int page_size, float scale,
-                                                   int window, int num_pages, int* status, void* stream) {
-  return prefill_attention_tc_entry(out, q, cache, block_table, tiles, n_tiles, n_tokens, q_stride, out_stride, bt_stride, nq, nkv, d, page_size,
-                                    scale, window, num_pages, true, status, stream);
+                                                   int window, int num_pages, int splits, float* part_acc, float* part_ml, int* status,
+                                                   void* stream) {
+  PTL_REQUIRE(splits >= 1 && splits <= 65535 && (splits == 1 || (part_acc && part_ml && ptl::aligned16(part_acc))),
+              "prefill_attention_tc: splits > 1 need scratch buffers");
+  const int rc = prefill_attention_tc_entry(out, q, cache, block_table, tiles, n_tiles, n_tokens, q_stride, out_stride, bt_stride, nq, nkv, d,
+                                            page_size, scale, window, num_pages, true, splits, part_acc, part_ml, status, stream);
+  if (rc || splits == 1 || n_tiles == 0) return rc;
+  return ptl::attention8_join_bf16(out, part_acc, part_ml, tiles, n_tiles, out_stride, nq, d, splits, stream);
 }

@@ -94,8 +94,8 @@ _SIGNATURES = {
     "ptl_read_kv8": [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr],
     "ptl_attention8_single": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                               _c_int, _c_f, _c_int, _c_int, _c_int, _ptr, _ptr, _c_int, _ptr, _ptr],
-    "ptl_attention8_portion": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f, _c_int,
-                               _c_int, _ptr, _ptr],
+    "ptl_attention8_portion": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f,
+                               _c_int, _c_int, _c_int, _ptr, _ptr],
     "ptl_attention8_simt": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                             _c_int, _c_f, _c_int, _c_int, _c_int, _ptr],
     "ptl_paged_attention_simt": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int,
@@ -200,7 +200,7 @@ def load_library() -> ctypes.CDLL:
     lib.ptl_prefill_attention_tc_bf16.argtypes = [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                                   _c_int, _c_int, _c_int, _c_f, _c_int, _c_int, _ptr, _ptr]
     lib.ptl_prefill_attention_tc_bf16.restype = _c_int
-    lib.ptl_prefill_attention_tc_holes_bf16.argtypes = lib.ptl_prefill_attention_tc_bf16.argtypes
+    lib.ptl_prefill_attention_tc_holes_bf16.argtypes = lib.ptl_prefill_attention_tc_bf16.argtypes[:-2] + [_c_int, _ptr, _ptr, _ptr, _ptr]
     lib.ptl_prefill_attention_tc_holes_bf16.restype = _c_int
     lib.ptl_kv8_expand_bf16.argtypes = [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr]
     lib.ptl_kv8_expand_bf16.restype = _c_int
@@ -998,7 +998,7 @@ class CudaOps:
         dec, tiles = self._work(hints, "decode_items"), self._work(hints, "prefill_tiles")
         if d in (64, 128) and nq // nkv <= 16 and dec is not None and tiles is not None and q.shape[1] % 8 == 0:
             if self._attention8_tensor_cores(out, q, codes, words, block_table, tok_req, positions, nq, nkv, d, page_size, float(scale),
-                                             int(window), longest, dec, tiles):
+                                             int(window), longest, dec, tiles, getattr(hints, "split_portions", None)):
                 return out
         # blocks of 128 keys' turns: split until they fill the machine a few times
         splits = max(1, min(-(-longest // 256), 148 * 8 // max(1, tokens * nq), 64))
@@ -1013,7 +1013,7 @@ class CudaOps:
         return out
 
     def _attention8_tensor_cores(self, out, q, codes, words, block_table, tok_req, positions, nq, nkv, d, page_size, scale, window, longest,
-                                 dec, tiles) -> bool:
+                                 dec, tiles, split_portions=None) -> bool:
         """Single tokens and portions by the tensor-core kernels; False where they do not take the sizes (nothing has run then)."""
         stream, n, suffix = self._stream(), dec.items, _suffix(q.dtype)
         if tiles.items > 65535:
@@ -1041,18 +1041,32 @@ class CudaOps:
                 return False
             self._check(rc)
         if tiles.items:
-            if q.dtype == torch.bfloat16 and self._attention8_portions(out, q, codes, words, block_table, nq, nkv, d, page_size, scale, window,
-                                                                       tiles, stream):
+            # Short contexts on mma.sync: their pages made bfloat16 and the larger tiles' start cost more than they save (32 heads of 64 over 8: a
+            # portion of 16 tokens 8.7 us so and 12.8, of 131 15.0 and 15.7, of 256 21.5 and 16.0).  Portions of few rows at long contexts too: 128
+            # rows of a tile are multiplied whatever they hold (heads of 128: 16 tokens behind 6,000 41 and 46 us, behind 30,000 96 and 195).
+            rows = (q.shape[0] - n) / (tiles.items // 2)             # of a pair of tiles, on average
+            few = longest <= 192 or (rows <= 32 and longest >= 3000) if split_portions is None else bool(split_portions)
+            if q.dtype == torch.bfloat16 and not few and self._attention8_portions(out, q, codes, words, block_table, nq, nkv, d, page_size, scale,
+                                                                                   window, longest, tiles, stream):
                 return True
+            splits, part_acc, part_ml = 1, None, None
+            if few or q.dtype == torch.float32:
+                blocks = max(1, (q.shape[0] - n) * nq // (64 if q.dtype == torch.float32 or d == 128 else 128))
+                splits = max(1, min(self._sm_count * 3 // blocks, -(-longest // 256), 32))
+            if splits > 1:
+                scratch = self.empty((q.shape[0] * nq * splits * (d + 2),), torch.float32)
+                part_acc = scratch.data_ptr()
+                part_ml = part_acc + q.shape[0] * nq * splits * d * 4
             rc = getattr(self.lib, "ptl_attention8_portion" + suffix)(
-                _p(out), _p(q), _p(codes), _p(words), _p(block_table), _p(tiles.tensor), tiles.items, q.shape[1], nq * d, block_table.shape[1],
-                nq, nkv, d, page_size, scale, window, codes.shape[0], _p(self._tc_status_word()), stream)
-            self._check(rc)
+                out.data_ptr(), part_acc, part_ml, q.data_ptr(), codes.data_ptr(), words.data_ptr(), block_table.data_ptr(), tiles.tensor.data_ptr(),
+                tiles.items, q.shape[1], nq * d, block_table.shape[1], nq, nkv, d, page_size, scale, window, splits, codes.shape[0],
+                self._tc_status_word().data_ptr(), stream)
+            self._check(rc, kernels=2 if splits > 1 else 1)
         return True
 
     KV8_EXPAND_BYTES = 1 << 30       # of pages made bfloat16 for one call, at most
 
-    def _attention8_portions(self, out, q, codes, words, block_table, nq, nkv, d, page_size, scale, window, tiles, stream) -> bool:
+    def _attention8_portions(self, out, q, codes, words, block_table, nq, nkv, d, page_size, scale, window, longest, tiles, stream) -> bool:
         """bfloat16 portions on the fifth-generation tensor cores, over the pages they see made bfloat16 first; False where they are too many
         (a captured step counts its longest contexts) or of a size that those tiles do not take."""
         keys = 128 if d == 64 else 64
@@ -1063,6 +1077,18 @@ class CudaOps:
         pages = slots * width + 1
         if pages * 4 * nkv * page_size * d > self.KV8_EXPAND_BYTES:
             return False
+        # A block an SM, in rounds: a block starts and ends in about 6 us and takes 1.9 us a tile of keys with heads of 64, 1.4 with 128; with
+        # its keys split, what the parts leave is written and read at about 3 TB/s.  32 heads, one portion, us, whole and split: 131 tokens behind
+        # 6,000 (heads of 64) 108 and 42, 600 behind 30,000 485 and 357; 600 behind 1,000 37, and 50 in three parts.
+        blocks, sms, n_keys, tile_us = tiles.items // 2 * nq, self._sm_count, longest / keys, 1.9 if d == 64 else 1.4
+        most = max(1, min(16, longest // (4 * keys)))
+        splits = min(range(1, most + 1), key=lambda s: -(-blocks * s // sms) * (6 + n_keys / s * tile_us)
+                     + (5 + q.shape[0] * nq * s * (d + 2) * 8 / 3e6 if s > 1 else 0))
+        part_acc = part_ml = None
+        if splits > 1:
+            scratch = self.empty((q.shape[0] * nq * splits * (d + 2),), torch.float32)
+            part_acc = scratch.data_ptr()
+            part_ml = part_acc + q.shape[0] * nq * splits * d * 4
         place = self.empty((pages * 2 * nkv * page_size * d,), torch.bfloat16)
         table = self.empty((requests, width), torch.int32)
         self._check(self.lib.ptl_kv8_expand_bf16(place.data_ptr(), table.data_ptr(), codes.data_ptr(), words.data_ptr(), block_table.data_ptr(),
@@ -1070,7 +1096,8 @@ class CudaOps:
                                                  window, stream))
         self._check(self.lib.ptl_prefill_attention_tc_holes_bf16(out.data_ptr(), q.data_ptr(), place.data_ptr(), table.data_ptr(), tiles.tensor.data_ptr(),
                                                                  tiles.items, q.shape[0], q.shape[1], nq * d, width, nq, nkv, d, page_size, scale,
-                                                                 window, pages, self._tc_status_word().data_ptr(), stream))
+                                                                 window, pages, splits, part_acc, part_ml, self._tc_status_word().data_ptr(), stream),
+                    kernels=2 if splits > 1 else 1)
         return True
 
     def _decode8_unit_list(self, dec, tok_req, positions, rows: int, nq: int, nkv: int, d: int, window: int, per_head: int):
