@@ -153,41 +153,41 @@ template <int D, typename T, int NT> struct A8Rows {
     unit = 0;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      auto x = [&](int k, int i) { return raw.v[n][(16 * k + i) / Vec16<T>::N].get(i % Vec16<T>::N); };
       float big = 0.f;
 #pragma unroll
-      for (int k = 0; k < kSteps / 4; ++k)
+      for (int i = 0; i < kRaw; ++i)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(x(k, i)));
+        for (int j = 0; j < Vec16<T>::N; ++j) big = fmaxf(big, fabsf(raw.v[n][i].get(j)));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
       // 2^e with |x| < 2, within the powers of two whose inverse is a normal number
       const uint32_t e = min(max(__float_as_uint(big) >> 23, 2u), 252u);
       const float inverse = __uint_as_float((254u - e) << 23);
-      float sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < kSteps / 4; ++k)
+      for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float a = x(k, 4 * i + 2 * j) * inverse, b = x(k, 4 * i + 2 * j + 1) * inverse;
-#pragma unroll
-            for (int part = 0; part < kParts; ++part) {
-              const uint32_t half = a8_pack(a, b);
-              float fa, fb;
-              a8_unpack(half, fa, fb);
-              sum += fa + fb;
-              qb[part][4 * k + i][n][j] = half;
-              a -= fa; b -= fb;
-            }
+        for (int j = 0; j < 2; ++j) {
+          const int i = 4 * k + 2 * j;                       // of the lane's entries, 16 for each 64 dimensions
+          float a = raw.v[n][i / Vec16<T>::N].get(i % Vec16<T>::N) * inverse, b = raw.v[n][i / Vec16<T>::N].get(i % Vec16<T>::N + 1) * inverse;
+          const uint32_t half = a8_pack(a, b);
+          qb[0][k][n][j] = half;
+          if (kParts == 2) {
+            float fa, fb;
+            a8_unpack(half, fa, fb);
+            qb[kParts - 1][k][n][j] = a8_pack(a - fa, b - fb);
           }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        }
+      // sum(x) of rows 2c and 2c + 1, where the scores will be: the products with ones
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+#pragma unroll
+      for (int part = 0; part < kParts; ++part)
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) mma_f16_16816(sum, ones, qb[part][k][n][0], qb[part][k][n][1]);
       const float f = __uint_as_float(e << 23) * p.scale_log2;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {                          // row 8 n + 2c + j is held by the lanes of g = 2c + j here
-        half_sum[n][j] = 0.5f * __shfl_sync(0xffffffffu, sum, 4 * (2 * c + j));
+        half_sum[n][j] = 0.5f * sum[j];
         factor[n][j] = __shfl_sync(0xffffffffu, f, 4 * (2 * c + j));
         const int r = 8 * n + 2 * c + j;
         last[n][j] = r < tokens * group ? pos0 + r / group : -1;
@@ -411,7 +411,7 @@ __device__ __forceinline__ float a8_weight(float m, float l, float M) { return l
 __device__ __forceinline__ float a8_inverse(float l) { return l == 0.f ? 0.f : 1.0f / l; }
 
 template <int D, int NT> struct A8Single {
-  static constexpr int kRing = D == 64 ? 6 : 4;                            // slots a warp has
+  static constexpr int kRing = 4;                                          // slots a warp has
   static constexpr int kSlot = 2 * kKv8Block * D;
   static constexpr int kRingBytes = kA8Warps * kRing * kSlot;
   static constexpr int kJoinBytes = kA8Warps * 8 * NT * (D + 2) * 4 + 8 * NT * (D + 2) * 4;      // the warps' rows, and the block's: where the rings were
@@ -468,35 +468,41 @@ attention8_single_kernel(const A8Params p) {
   const int b0 = lo / kKv8Block, blocks = pos < 0 ? 0 : pos / kKv8Block - b0 + 1;
   const int per = (blocks + splits - 1) / splits;
   const int begin = b0 + min(blocks, split * per), end = b0 + min(blocks, (split + 1) * per);
-  // ---- this warp's blocks: begin + warp + 4 i, i < count.  A lane looks up every 32nd of them: its page, and its words
+  // ---- this warp's blocks: begin + warp + 4 i, i < count.  Lane l looks after blocks l, l + 32, ...: where they lie, their words, and their copies
+  static_assert(kRing == 4 && kA8Turn == 2, "blocks i + 4 and i + 5 follow blocks i and i + 1 into their slots");
   const int count = max(0, (end - begin - warp + kA8Warps - 1) / kA8Warps);
   const int* table = p.block_table + (size_t)r * p.bt_stride;
-  auto block_at = [&](int i) { return begin + warp + kA8Warps * i; };
-  auto page_at = [&](int i) { return i < count ? p.page_of(table, block_at(i)) : -1; };
-  auto word_at = [&](int i, int page) { return page >= 0 ? p.word(page, kvh, p.sub_of(block_at(i))) : make_uint2(0u, 0u); };
-  const uint32_t slot0 = smem_addr(smem) + warp * (kRing * Cfg::kSlot);
-  auto fetch = [&](int i, int page) {                         // (lane 0) block i into its slot
-    const uint32_t bar = full0 + 8 * (i % kRing), dst = slot0 + (i % kRing) * Cfg::kSlot;
-    if (page < 0) { mbar_arrive(bar); return; }
-    mbar_expect_tx(bar, Cfg::kSlot);
-    const unsigned char* src = p.keys<D>(page, kvh, p.sub_of(block_at(i)));
-    bulk_load(dst, src, Cfg::kSlot / 2, bar);
-    bulk_load(dst + Cfg::kSlot / 2, src + p.plane<D>(), Cfg::kSlot / 2, bar);
+  auto page_at = [&](int i) { return i < count ? p.page_of(table, begin + warp + kA8Warps * i) : -1; };
+  auto source = [&](int i, int page) { return page >= 0 ? p.keys<D>(page, kvh, p.sub_of(begin + warp + kA8Warps * i)) : nullptr; };
+  auto word_at = [&](int i, int page) {                       // with bit 8 of the keys' set: there is a page
+    uint2 w = page >= 0 ? p.word(page, kvh, p.sub_of(begin + warp + kA8Warps * i)) : make_uint2(0u, 0u);
+    if (page >= 0) w.x = (w.x & ~0xff00u) | 0x100u;
+    return w;
   };
-  int page_cur = page_at(lane), page_nxt = page_at(32 + lane);
+  const uint32_t slot0 = smem_addr(smem) + warp * (kRing * Cfg::kSlot);
+  const size_t plane = p.plane<D>();
+  auto fetch = [&](int slot, const unsigned char* src) {
+    const uint32_t bar = full0 + 8 * slot, dst = slot0 + slot * Cfg::kSlot;
+    if (!src) { mbar_arrive(bar); return; }
+    mbar_expect_tx(bar, Cfg::kSlot);
+    bulk_load(dst, src, Cfg::kSlot / 2, bar);
+    bulk_load(dst + Cfg::kSlot / 2, src + plane, Cfg::kSlot / 2, bar);
+  };
+  const int page0 = page_at(lane);
+  int page_nxt = page_at(32 + lane);
   A8Rows<D, T, NT> rows;
   typename A8Rows<D, T, NT>::Raw raw;
   rows.fetch(raw, p, t, 1, kvh, group);                       // (asked for beside the pages)
-  for (int i = 0; i < min(kRing, count); ++i) {
-    const int page = __shfl_sync(0xffffffffu, page_cur, i);
-    if (lane == 0) fetch(i, page);
-  }
-  uint2 word_cur = word_at(lane, page_cur);
+  const unsigned char* src_cur = source(lane, page0);
+  if (lane < min(kRing, count)) fetch(lane, src_cur);
+  __syncwarp();
+  uint2 word_cur = word_at(lane, page0);
   rows.load(raw, p, 1, pos, group);
   int gave_up = -1;                                           // the block whose wait ran out
   for (int base = 0; base < count; base += 32) {
     const uint2 word_nxt = word_at(base + 32 + lane, page_nxt);
-    const int page_nn = page_at(base + 64 + lane);
+    const unsigned char* src_nxt = source(base + 32 + lane, page_nxt);
+    page_nxt = page_at(base + 64 + lane);
     const int stop = min(32, count - base);
     for (int i = 0; i < stop; i += kA8Turn) {
       const unsigned char* slot[kA8Turn];
@@ -505,27 +511,22 @@ attention8_single_kernel(const A8Params p) {
       int key0[kA8Turn];
 #pragma unroll
       for (int b = 0; b < kA8Turn; ++b) {
-        const int at = base + i + b;
         word[b].x = __shfl_sync(0xffffffffu, word_cur.x, i + b);
         word[b].y = __shfl_sync(0xffffffffu, word_cur.y, i + b);
-        have[b] = __shfl_sync(0xffffffffu, page_cur, i + b) >= 0;        // (false behind the last block)
-        key0[b] = block_at(at) * kKv8Block;
-        slot[b] = smem + warp * (kRing * Cfg::kSlot) + (at % kRing) * Cfg::kSlot;
+        have[b] = (word[b].x >> 8) & 1u;                      // (not behind the last block)
+        key0[b] = (begin + warp + kA8Warps * (base + i + b)) * kKv8Block;
+        slot[b] = smem + warp * (kRing * Cfg::kSlot) + ((i + b) % kRing) * Cfg::kSlot;
         if (i + b < stop && gave_up < 0 &&
-            !__all_sync(0xffffffffu, mbar_wait(full0 + 8 * (at % kRing), (at / kRing) & 1, &s_abort, p.status, 9))) gave_up = at;
+            !__all_sync(0xffffffffu, mbar_wait(full0 + 8 * ((i + b) % kRing), ((base + i + b) / kRing) & 1, &s_abort, p.status, 9))) gave_up = base + i + b;
       }
       if (gave_up >= 0) break;
       rows.turn(slot, have, word, key0, lo, pos);
       __syncwarp();                                           // the slots are read: their next blocks
-#pragma unroll
-      for (int b = 0; b < kA8Turn; ++b) {
-        const int ahead = i + b + kRing;
-        const int page = __shfl_sync(0xffffffffu, ahead < 32 ? page_cur : page_nxt, ahead & 31);
-        if (lane == 0 && i + b < stop && base + ahead < count) fetch(base + ahead, page);
-      }
+      const int ahead = i + kRing + (lane & 1);
+      if ((lane & 30) == ((i + kRing) & 31) && base + ahead < count) fetch(ahead % kRing, ahead < 32 ? src_cur : src_nxt);
     }
     if (gave_up >= 0) break;
-    page_cur = page_nxt; page_nxt = page_nn; word_cur = word_nxt;
+    src_cur = src_nxt; word_cur = word_nxt;
   }
   if (gave_up >= 0)                                           // this warp's copies still under way end before the memory is used for something else
     for (int i = gave_up; i < min(gave_up + kRing, count); ++i) mbar_drain(full0 + 8 * (i % kRing), (i / kRing) & 1);
@@ -620,18 +621,29 @@ attention8_single_kernel(const A8Params p) {
   const size_t at0 = (size_t)(blockIdx.x - split) * group;   // the parts of a (token, kv head) lie side by side
   for (int e = tid; e < group * D; e += kA8Warps * 32) {
     const int row = e / D, col = e % D;
-    const float* ml = p.part_ml + 2 * (at0 + row);
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + at0 + row;
     const float* acc_of = p.part_acc + (at0 + row) * D + col;
     float M = -INFINITY, L = 0.f, acc = 0.f;
-#pragma unroll 8
-    for (int z = 0; z < splits; ++z) M = fmaxf(M, __ldcg(ml + 2 * (size_t)z * group));
-#pragma unroll 8
-    for (int z = 0; z < splits; ++z) {
-      const float mz = __ldcg(ml + 2 * (size_t)z * group), lz = __ldcg(ml + 2 * (size_t)z * group + 1), a = __ldcg(acc_of + (size_t)z * group * D);
-      const float f = a8_weight(mz, lz, M);
-      if (lz == 0.f) continue;
-      L = fmaf(f, lz, L);
-      acc = fmaf(f, a, acc);
+    for (int z0 = 0; z0 < splits; z0 += 8) {                 // eight parts are asked for at once
+      float2 part[8];
+      float a[8], top = M;
+#pragma unroll
+      for (int z = 0; z < 8; ++z) {
+        part[z] = z0 + z < splits ? __ldcg(ml + (size_t)(z0 + z) * group) : make_float2(-INFINITY, 0.f);
+        a[z] = z0 + z < splits ? __ldcg(acc_of + (size_t)(z0 + z) * group * D) : 0.f;
+        top = fmaxf(top, part[z].x);
+      }
+      const float before = a8_weight(M, L, top);
+      M = top;
+      L *= before;
+      acc *= before;
+#pragma unroll
+      for (int z = 0; z < 8; ++z) {
+        const float f = a8_weight(part[z].x, part[z].y, top);
+        if (part[z].y == 0.f) continue;
+        L = fmaf(f, part[z].y, L);
+        acc = fmaf(f, a[z], acc);
+      }
     }
     out[(size_t)t * p.out_stride + (size_t)(kvh * group + row) * D + col] = from_f32<T>(acc * a8_inverse(L));
   }
