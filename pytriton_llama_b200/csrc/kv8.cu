@@ -12,6 +12,7 @@
 namespace ptl {
 
 constexpr int kKv8Threads = 256;
+constexpr int kKv8WriteThreads = 128;
 
 template <int N> struct Kv8Packet;
 template <> struct Kv8Packet<8> { using type = uint2; };
@@ -63,7 +64,7 @@ __device__ __forceinline__ void kv8_turn(const Kv8WriteParams& p, float (&x)[Vec
 
 // D: the head size, or 0 for any (then the values are read twice).  TURN: there are frequencies.
 template <typename T, int D, bool TURN>
-__global__ void __launch_bounds__(kKv8Threads)
+__global__ void __launch_bounds__(kKv8WriteThreads)
 rope_kv8_write_kernel(const Kv8WriteParams p) {
   extern __shared__ float cs[];                  // [rows staged][cos[half], sin[half]]
   constexpr int N = Vec16<T>::N;
@@ -84,7 +85,7 @@ rope_kv8_write_kernel(const Kv8WriteParams p) {
     const int of_last = __shfl_sync(0xffffffffu, mine, last + 1);
     const unsigned same = __ballot_sync(0xffffffffu, lane > last && mine == of_last) >> (last + 1);
     staged = max(t1 - t0, leads ? last + min(kKv8Block, __ffs(~same) - 1) : 0);
-    for (int e = threadIdx.x; e < staged * half; e += kKv8Threads) {
+    for (int e = threadIdx.x; e < staged * half; e += kKv8WriteThreads) {
       if (t0 + e / half >= p.tokens) break;
       const float2 cos_sin = p.angle(t0 + e / half, e % half);
       cs[e / half * p.rot + e % half] = cos_sin.x;
@@ -95,7 +96,7 @@ rope_kv8_write_kernel(const Kv8WriteParams p) {
   pdl_launch_dependents();
   __syncthreads();
   if constexpr (TURN) {                          // q of these rows, in place
-    for (int e = blockIdx.y * kKv8Threads + threadIdx.x; e < (t1 - t0) * p.nq * half; e += gridDim.y * kKv8Threads) {
+    for (int e = blockIdx.y * kKv8WriteThreads + threadIdx.x; e < (t1 - t0) * p.nq * half; e += gridDim.y * kKv8WriteThreads) {
       const int r = e / (p.nq * half), j = e % half;
       T* head = qkv + (size_t)(t0 + r) * row_len + (size_t)(e / half % p.nq) * d;
       float o1, o2;
@@ -105,7 +106,7 @@ rope_kv8_write_kernel(const Kv8WriteParams p) {
     }
   }
   const int blocks_per_page = p.page_size / kKv8Block, units = 2 * p.nkv, packets = d / N;
-  for (int task = blockIdx.y * (kKv8Threads / 32) + warp; task < __popc(leads) * units; task += gridDim.y * (kKv8Threads / 32)) {
+  for (int task = blockIdx.y * (kKv8WriteThreads / 32) + warp; task < __popc(leads) * units; task += gridDim.y * (kKv8WriteThreads / 32)) {
     const int unit = task % units, g = unit >> 1, part = unit & 1;
     int first = t0 + __fns(leads, 0, task / units + 1);
     const int block = p.block_of(first);
@@ -125,43 +126,67 @@ rope_kv8_write_kernel(const Kv8WriteParams p) {
       Vec16<T> raw[kPackets];                    // (turned, once they have been looked at)
       auto fetch = [&](int e) { return load16(src + (size_t)(e / packets) * row_len + e % packets * N); };
       auto turn = [&](int e, Vec16<T>& v) {
-        if (!TURN || !turned) return;
-        float x[N];
+        if constexpr (TURN) {
+          if (!turned) return;
+          float x[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j) x[j] = v.get(j);
-        const int row = first + e / packets;
-        kv8_turn<T>(p, x, src + (size_t)(e / packets) * row_len, e % packets, row, row - t0 < staged ? cs + (row - t0) * p.rot : nullptr);
+          for (int j = 0; j < N; ++j) x[j] = v.get(j);
+          const int row = first + e / packets;
+          kv8_turn<T>(p, x, src + (size_t)(e / packets) * row_len, e % packets, row, row - t0 < staged ? cs + (row - t0) * p.rot : nullptr);
 #pragma unroll
-        for (int j = 0; j < N; ++j) v.set(j, x[j]);
+          for (int j = 0; j < N; ++j) v.set(j, x[j]);
+        }
       };
-      uint32_t amax = 0u, bad = 0u;              // bits of the largest magnitude; the marked tokens
-      auto look = [&](int e, const Vec16<T>& v) {
-        bool odd = false;
+      // Bits of the largest magnitude, marked values among them: those of infinity and NaN are larger than all others, so one look at
+      // the largest of the run tells whether there is one, and only then the tokens are looked through.
+      uint32_t amax = 0u, bad = 0u;
+      auto look = [&](const Vec16<T>& v) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) amax = max(amax, __float_as_uint(v.get(j)) & 0x7fffffffu);
+      };
+      constexpr uint32_t kInf = 0x7f800000u;
+      auto look_closely = [&](const Vec16<T>& v, int row_off) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
           const uint32_t mag = __float_as_uint(v.get(j)) & 0x7fffffffu;
-          odd |= mag >= 0x7f800000u;
-          amax = max(amax, mag >= 0x7f800000u ? 0u : mag);
+          if (mag >= kInf) bad |= 1u << row_off;
+          else amax = max(amax, mag);
         }
-        const int row_off = __ldg(p.slots + first + e / packets) % kKv8Block;
-        if (odd) bad |= 1u << row_off;
       };
+      int offs[kPackets];                        // of the packets' rows in the block of 16
       if constexpr (D != 0) {
 #pragma unroll
-        for (int i = 0; i < kPackets; ++i)
+        for (int i = 0; i < kPackets; ++i) {
           if (lane + 32 * i < rows * packets) raw[i] = fetch(lane + 32 * i);
+          offs[i] = __shfl_sync(0xffffffffu, off, (lane + 32 * i) / packets);
+        }
 #pragma unroll
         for (int i = 0; i < kPackets; ++i)
-          if (lane + 32 * i < rows * packets) { turn(lane + 32 * i, raw[i]); look(lane + 32 * i, raw[i]); }
+          if (lane + 32 * i < rows * packets) { turn(lane + 32 * i, raw[i]); look(raw[i]); }
       } else {
         for (int e = lane; e < rows * packets; e += 32) {
           Vec16<T> v = fetch(e);
           turn(e, v);
-          look(e, v);
+          look(v);
         }
       }
       amax = __reduce_max_sync(0xffffffffu, amax);
-      bad = __reduce_or_sync(0xffffffffu, bad);
+      if (amax >= kInf) {
+        amax = 0u;
+        if constexpr (D != 0) {
+#pragma unroll
+          for (int i = 0; i < kPackets; ++i)
+            if (lane + 32 * i < rows * packets) look_closely(raw[i], offs[i]);
+        } else {
+          for (int e = lane; e < rows * packets; e += 32) {
+            Vec16<T> v = fetch(e);
+            turn(e, v);
+            look_closely(v, __ldg(p.slots + first + e / packets) % kKv8Block);
+          }
+        }
+        amax = __reduce_max_sync(0xffffffffu, amax);
+        bad = __reduce_or_sync(0xffffffffu, bad);
+      }
       const bool anew = here & 1u;
       const int e_old = anew ? 0 : (int)(had & 255u);
       const int e_new = max(e_old, kv8_exponent(amax));
@@ -175,27 +200,31 @@ rope_kv8_write_kernel(const Kv8WriteParams p) {
       }
       __syncwarp();
       const float inverse = e_new ? kv8_inverse_step(e_new) : 0.f;
-      auto store = [&](int e, const Vec16<T>& v) {
+      auto store = [&](int e, const Vec16<T>& v, int row_off) {
         uint32_t out[N / 4];
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const float x = v.get(j);
-          const bool finite = (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u;
-          const uint32_t u = finite && e_new ? kv8_code(x, inverse) : 128u;
-          out[j / 4] = j % 4 ? out[j / 4] | u << (8 * (j % 4)) : u;
+        for (int j = 0; j < N; j += 4) {
+          uint32_t u[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) u[k] = kv8_code(v.get(j + k), inverse);
+          if (bad) {                             // (what is no finite number is kept as 128)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if ((__float_as_uint(v.get(j + k)) & 0x7fffffffu) >= kInf) u[k] = 128u;
+          }
+          out[j / 4] = __byte_perm(__byte_perm(u[0], u[1], 0x0040u), __byte_perm(u[2], u[3], 0x0040u), 0x5410u);
         }
-        const int row_off = __ldg(p.slots + first + e / packets) % kKv8Block;
         *reinterpret_cast<typename Kv8Packet<N>::type*>(dst + (size_t)row_off * d + e % packets * N) = *reinterpret_cast<typename Kv8Packet<N>::type*>(out);
       };
       if constexpr (D != 0) {
 #pragma unroll
         for (int i = 0; i < kPackets; ++i)
-          if (lane + 32 * i < rows * packets) store(lane + 32 * i, raw[i]);
+          if (lane + 32 * i < rows * packets) store(lane + 32 * i, raw[i], offs[i]);
       } else {
         for (int e = lane; e < rows * packets; e += 32) {
           Vec16<T> v = fetch(e);
           turn(e, v);
-          store(e, v);
+          store(e, v, __ldg(p.slots + first + e / packets) % kKv8Block);
         }
       }
       if (lane == 0) *word = (uint32_t)e_new | ((((anew ? 0u : had >> 16) & ~here) | bad) << 16);
@@ -206,8 +235,8 @@ rope_kv8_write_kernel(const Kv8WriteParams p) {
   }
 }
 
-// Keys and values of the first length[r] tokens of the requests as numbers, request after request: out [tokens][2][heads][d].  A block
-// takes 1,024 pieces of 8 codes of one request, four a thread.
+// Keys and values of the first length[r] tokens of the requests as numbers, request after request: out [tokens][2][heads][d].  A block of
+// threads takes 16 positions of a request, which lie in one page, packets of 16 codes in the order in which they lie there.
 constexpr int kKv8ReadRequests = 960;
 constexpr int kKv8ReadAhead = 4;
 struct Kv8ReadArgs {
@@ -221,45 +250,42 @@ __global__ void __launch_bounds__(kKv8Threads)
 read_kv8_kernel(T* __restrict__ out, const unsigned char* __restrict__ codes, const uint32_t* __restrict__ words,
                 const int* __restrict__ block_table, const __grid_constant__ Kv8ReadArgs args, int bt_stride, int nkv, int d, int page_size,
                 int num_pages) {
-  constexpr int N = 8;                     // codes of a piece
-  const int r = blockIdx.y;
-  const int t0 = r ? args.end[r - 1] : 0, tokens = args.end[r] - t0;
-  const int per_token = 2 * nkv * d / N;
-  const long long total = (long long)tokens * per_token;
-  const long long at = (long long)blockIdx.x * (kKv8Threads * kKv8ReadAhead) + threadIdx.x;
-  if (at - threadIdx.x >= total) return;
+  const int r = blockIdx.y, pos0 = blockIdx.x * kKv8Block;
+  const int t0 = r ? args.end[r - 1] : 0, tokens = min(kKv8Block, args.end[r] - t0 - pos0);
+  if (tokens <= 0) return;
   pdl_wait();
   pdl_launch_dependents();
-  const int* table = block_table + (size_t)(args.first_request + r) * bt_stride;
-  uint2 c[kKv8ReadAhead];
-  uint32_t w[kKv8ReadAhead];
-  bool have[kKv8ReadAhead];
+  const int page = __ldg(block_table + (size_t)(args.first_request + r) * bt_stride + pos0 / page_size), sub = pos0 % page_size / kKv8Block;
+  const bool here = page >= 0 && page < num_pages;           // (a position that has no page reads as 0)
+  const unsigned per_row = d / 16, total = 2u * nkv * d;     // packets of a row, and of the 16 positions
+  const unsigned char* src = codes + (size_t)(here ? page : 0) * 2 * nkv * page_size * d + (size_t)sub * kKv8Block * d;
+  const uint32_t* word0 = words + (size_t)(here ? page : 0) * nkv * (page_size / kKv8Block) * 2 + sub * 2;
+  T* dst0 = out + (args.first_row + t0 + pos0) * 2 * nkv * d;
+  for (unsigned x0 = threadIdx.x; x0 < total; x0 += kKv8Threads * kKv8ReadAhead) {
+    uint4 c[kKv8ReadAhead];
+    uint32_t w[kKv8ReadAhead];
 #pragma unroll
-  for (int i = 0; i < kKv8ReadAhead; ++i) {
-    const long long x = at + i * kKv8Threads;
-    have[i] = false;
-    if (x >= total) continue;
-    const int pos = (int)(x / per_token), e = (int)(x % per_token) * N;
-    const int page = __ldg(table + pos / page_size), part = e / (nkv * d), g = e / d % nkv, off = pos % page_size;
-    if (page < 0 || page >= num_pages) continue;             // a position that has no page
-    have[i] = true;
-    c[i] = __ldg(reinterpret_cast<const uint2*>(codes + ((((size_t)page * 2 + part) * nkv + g) * page_size + off) * d + e % d));
-    w[i] = __ldg(words + (((size_t)page * nkv + g) * (page_size / kKv8Block) + off / kKv8Block) * 2 + part);
-  }
+    for (int i = 0; i < kKv8ReadAhead; ++i) {
+      const unsigned x = x0 + i * kKv8Threads, head = x / d, part = head >= (unsigned)nkv, in_head = x - head * d;
+      if (x >= total || !here) continue;
+      c[i] = __ldg(reinterpret_cast<const uint4*>(src + (size_t)head * page_size * d) + in_head);
+      w[i] = __ldg(word0 + (head - part * nkv) * (page_size / kKv8Block) * 2 + part);
+    }
 #pragma unroll
-  for (int i = 0; i < kKv8ReadAhead; ++i) {
-    const long long x = at + i * kKv8Threads;
-    if (x >= total) continue;
-    const int pos = (int)(x / per_token);
-    const float half_step = have[i] ? kv8_half_step(w[i] & 255u) : 0.f;
-    const bool bad = have[i] && (w[i] >> (16 + pos % kKv8Block) & 1u);
-    T* dst = out + (args.first_row + t0) * 2 * nkv * d + x * N;
-    Vec16<T> p;
+    for (int i = 0; i < kKv8ReadAhead; ++i) {
+      const unsigned x = x0 + i * kKv8Threads, head = x / d, in_head = x - head * d, off = in_head / per_row, col = (in_head - off * per_row) * 16;
+      if (x >= total || off >= (unsigned)tokens) continue;
+      const float half_step = here ? kv8_half_step(w[i] & 255u) : 0.f;
+      const bool bad = here && ((w[i] >> (16 + off)) & 1u);
+      T* dst = dst0 + (size_t)off * 2 * nkv * d + head * d + col;
+      Vec16<T> p;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float v = have[i] ? (float)(2 * (int)(((j < 4 ? c[i].x : c[i].y) >> (8 * (j & 3))) & 255u) - 255) * half_step : 0.f;
-      p.set(j % Vec16<T>::N, bad ? __uint_as_float(0x7fc00000u) : v);
-      if (j % Vec16<T>::N == Vec16<T>::N - 1) store16(dst + j + 1 - Vec16<T>::N, p);
+      for (int j = 0; j < 16; ++j) {
+        const uint32_t four = j < 4 ? c[i].x : j < 8 ? c[i].y : j < 12 ? c[i].z : c[i].w;
+        const float v = here ? (float)(2 * (int)((four >> (8 * (j & 3))) & 255u) - 255) * half_step : 0.f;
+        p.set(j % Vec16<T>::N, bad ? __uint_as_float(0x7fc00000u) : v);
+        if (j % Vec16<T>::N == Vec16<T>::N - 1) store16(dst + j + 1 - Vec16<T>::N, p);
+      }
     }
   }
 }
@@ -346,7 +372,7 @@ static int rope_kv8_write(T* qkv, const int* positions, const float* inv_freq, c
                           int nkv, int d, int rot, int page_size, long long num_slots, void* stream) {
   PTL_REQUIRE(tokens >= 0 && nq >= 0 && nkv > 0 && d > 0 && page_size > 0 && num_slots >= 0, "rope_kv8_write: bad sizes");
   PTL_REQUIRE(d % 16 == 0 && d <= 256, "rope_kv8_write: head size %d is no multiple of 16 up to 256", d);
-  PTL_REQUIRE(nkv <= 65535 * 4, "rope_kv8_write: too many heads");
+  PTL_REQUIRE(nkv <= 65535, "rope_kv8_write: too many heads");
   PTL_REQUIRE(page_size % kKv8Block == 0, "rope_kv8_write: pages of %d positions are not whole blocks of %d", page_size, kKv8Block);
   PTL_REQUIRE(rot % 2 == 0 && rot >= 0 && rot <= d, "rope_kv8_write: rotary width %d of head size %d", rot, d);
   PTL_REQUIRE(aligned16(qkv) && aligned16(codes), "rope_kv8_write: qkv and codes must be 16-byte aligned");
@@ -358,7 +384,8 @@ static int rope_kv8_write(T* qkv, const int* positions, const float* inv_freq, c
   const size_t smem = inv_freq ? (size_t)(p.rows_per_block + kKv8Block - 1) * rot * sizeof(float) : 0;
   auto kernel = inv_freq ? (d == 64 ? rope_kv8_write_kernel<T, 64, true> : d == 128 ? rope_kv8_write_kernel<T, 128, true> : rope_kv8_write_kernel<T, 0, true>)
                          : (d == 64 ? rope_kv8_write_kernel<T, 64, false> : d == 128 ? rope_kv8_write_kernel<T, 128, false> : rope_kv8_write_kernel<T, 0, false>);
-  return launch_kernel("rope_kv8_write", kernel, dim3((tokens + p.rows_per_block - 1) / p.rows_per_block, (2 * nkv + 7) / 8), dim3(kKv8Threads), smem,
+  return launch_kernel("rope_kv8_write", kernel, dim3((tokens + p.rows_per_block - 1) / p.rows_per_block, (2 * nkv + kKv8WriteThreads / 32 - 1) / (kKv8WriteThreads / 32)),
+                       dim3(kKv8WriteThreads), smem,
                        as_stream(stream), p);
 }
 
@@ -384,9 +411,7 @@ static int read_kv8(T* out, const void* codes, const void* words, const int* blo
       args.end[i] = (int)sum;
     }
     if (sum > 0) {
-      const long long blocks = ((long long)longest * (2 * nkv * d / 8) + kKv8Threads * kKv8ReadAhead - 1) / (kKv8Threads * kKv8ReadAhead);
-      PTL_REQUIRE(blocks <= 0x7fffffffLL, "read_kv8: a request is too long");
-      if (int rc = launch_kernel("read_kv8", read_kv8_kernel<T>, dim3((unsigned)blocks, args.requests), dim3(kKv8Threads), 0, as_stream(stream), out,
+      if (int rc = launch_kernel("read_kv8", read_kv8_kernel<T>, dim3((longest + kKv8Block - 1) / kKv8Block, args.requests), dim3(kKv8Threads), 0, as_stream(stream), out,
                                  (const unsigned char*)codes, (const uint32_t*)words, block_table, args, bt_stride, nkv, d, page_size, num_pages))
         return rc;
     }

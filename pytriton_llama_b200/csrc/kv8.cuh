@@ -33,11 +33,9 @@ __device__ __forceinline__ float kv8_half_step(int e) {
 // 1 / step = 2^(133 - E), for E of 16 to 254 a normal number.
 __device__ __forceinline__ float kv8_inverse_step(int e) { return __uint_as_float((uint32_t)(260 - e) << 23); }
 
-__device__ __forceinline__ uint32_t kv8_code(float x, float inverse_step) {
-  const float y = x * inverse_step;                            // exact, or so small that only its sign is left
-  const int c = (y == 0.f && x < 0.f) ? -1 : (int)floorf(y);
-  return (uint32_t)(c + 128);
-}
+// The code of a finite x, in the low byte: x / step + 1.5 * 2^23 + 128 rounded down has the whole part of x / step, rounded down, plus 128 in its
+// last bits.  One rounding, so a tiny negative x counts as below 0 too.  With a step of 0 / 0 (inverse 0): 128.
+__device__ __forceinline__ uint32_t kv8_code(float x, float inverse_step) { return __float_as_uint(__fmaf_rd(x, inverse_step, 12583040.0f)); }
 // Four codes for steps 2^n times as large; from n = 7 on only the sign is left.
 __device__ __forceinline__ uint32_t kv8_coarser(uint32_t four, int n) {
   n = min(n, 7);

@@ -5,11 +5,12 @@
 //   log p(t) = x_t - m - log S          entropy = log S - U / S
 //
 // A row is cut into slices, one block of a cluster each.  A thread keeps (m, S, U) of what it has read; threads, then blocks are
-// brought to one maximum.  The largest logits are found on the way: a 64-bit key holds the logit in an order of
-// whole numbers and, below it, the index the other way round, so keys are unique and of equal logits the lowest index is
-// the largest.  Every 4,096 logits, those above the threshold (the smallest of the `top` best so far) go to a list in shared
-// memory.  Where more come than it has room for, the threshold is first raised to the `top`-th largest of the maxima of 64
-// groups of 64 logits: at most `top` * 64 logits can lie above that, and the list holds as many.
+// brought to one maximum.  The largest logits are found on the way, by every warp for itself, so that no barrier stands in the
+// loop: a 64-bit key holds the logit in an order of whole numbers and, below it, the index the other way round, so keys are
+// unique and of equal logits the lowest index is the largest.  A warp's lanes hold its best keys so far in order, one each; logits above
+// the block's threshold (the largest `top`-th best of any warp: as many are known to be no smaller) go to a list, and 32 of them
+// are ranked among the best by counting.  Where most lanes have one, as at the start, the threshold is first raised to the
+// `top`-th largest of the 32 lanes' maxima.  At the end the warps' best, then the blocks', are ranked the same way.
 //
 // Logits of -inf have no probability.  A row with a NaN, with +inf, or with -inf only has no distribution: its
 // log-probabilities and its entropy are NaN.  Its alternatives are the largest logits all the same, NaN behind all others.
@@ -17,13 +18,14 @@
 
 namespace ptl {
 
-constexpr int kTsThreads = 256;
+constexpr int kTsWarps = 8;
+constexpr int kTsThreads = kTsWarps * 32;
 constexpr int kTsPerThread = 16;                       // logits of a turn
 constexpr int kTsTurn = kTsThreads * kTsPerThread;
 constexpr int kTsMaxTop = 32;
-constexpr int kTsGroups = 64;                          // of a turn, 4 threads each
-constexpr int kTsRoom = kTsMaxTop * (kTsTurn / kTsGroups) + kTsMaxTop;      // of the list: the groups that may lie above a raised threshold, and what is there
+constexpr int kTsRoom = 32 * kTsPerThread + 31;        // of a warp's list: a turn's logits, and fewer than 32 that were left
 constexpr int kTsMaxCluster = 8;
+static_assert(kTsWarps <= kTsMaxCluster, "the warps' best and the blocks' have one place");
 
 typedef unsigned long long TsKey;
 // Larger logits have larger keys, equal ones larger keys at lower indices; NaN comes behind -inf.  No key is 0.
@@ -55,24 +57,44 @@ __device__ __forceinline__ void ts_move(float m, float to, float& S, float& U) {
 }
 
 struct TsShared {
-  TsKey list[kTsRoom];
-  TsKey best[kTsMaxTop];                               // of this block, sorted
-  TsKey group[kTsGroups];
+  TsKey list[kTsWarps][kTsRoom];
+  TsKey best[kTsWarps * kTsMaxTop];                    // 32 for every warp to merge through; then the block's
   TsKey threshold;
-  TsKey merged[kTsMaxCluster * kTsMaxTop];             // in the first block of a cluster: every block's best
+  TsKey merged[kTsMaxCluster * kTsMaxTop];             // every warp's best; then, in the first block of a cluster, every block's
   float sums[kTsMaxCluster][3];                        // ... and its m, S, U
   float red[33];
-  int count;
+  int count[kTsWarps];
 };
 
-// The `top` largest of n keys (unique, n >= top), sorted, to `best`: a key's place is the number of larger ones.
+// Places the `top` largest of n keys (unique but for zeros, which are none) in order in best[0 .. top): a key's place is the number of larger ones.
 __device__ __forceinline__ void ts_select(const TsKey* keys, int n, int top, TsKey* best) {
   for (int i = threadIdx.x; i < n; i += kTsThreads) {
     const TsKey k = keys[i];
+    if (k == 0) continue;
     int place = 0;
-    for (int j = 0; j < n && place < top; ++j) place += keys[j] > k;
+    for (int j = 0; j < n; ++j) place += keys[j] > k;
     if (place < top) best[place] = k;
   }
+}
+
+// The 32 best of the warp, lane by lane in order, and 32 more keys (0: none), through 32 keys of shared memory.
+__device__ __forceinline__ TsKey ts_merge(TsKey best, TsKey more, TsKey* through) {
+  const int lane = threadIdx.x & 31;
+  int place_best = lane, place_more = 0;
+  for (int j = 0; j < 32; ++j) {
+    const TsKey b = __shfl_sync(0xffffffffu, best, j), n = __shfl_sync(0xffffffffu, more, j);
+    place_more += (b > more) + (n > more);
+    place_best += n > best;
+  }
+  // (zeros share places behind all keys)
+  through[lane] = 0;
+  __syncwarp();
+  if (best != 0 && place_best < 32) through[place_best] = best;
+  if (more != 0 && place_more < 32) through[place_more] = more;
+  __syncwarp();
+  const TsKey r = through[lane];
+  __syncwarp();
+  return r;
 }
 
 template <bool TOP>
@@ -92,120 +114,128 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
   const int packets = (vocab + skew + 3) / 4;
   const int per = (packets + slices - 1) / slices;
   const int p0 = slice * per, p1 = min(packets, p0 + per);
-  if (TOP && tid == 0) { sh.count = 0; sh.threshold = 0; }
-  float m = -INFINITY, S = 0.f, U = 0.f;
-  const int want = TOP ? min(top, max(0, min(vocab, p1 * 4 - skew) - max(0, p0 * 4 - skew))) : 0;      // this block's share of the best
-  if (TOP) __syncthreads();
-  // a turn's logits are asked for while the turn before is worked on
-  float ahead[kTsPerThread];
-  auto ask = [&](int base) {
+  const int warp = tid >> 5, lane = tid & 31;
+  if (TOP) {
+    if (tid == 0) sh.threshold = 0;
+    if (lane == 0) sh.count[warp] = 0;
+    __syncthreads();
+  }
+  float m = -INFINITY;
+  float2 S2 = make_float2(0.f, 0.f), U2 = make_float2(0.f, 0.f);
+  TsKey best = 0;                                      // the warp's lane-th best
+  int have = 0;                                        // on the warp's list
+  // packet i of the lane in the warp's turn from packet `base` on
+  auto packet = [&](int base, int i) { return base + (warp * (kTsPerThread / 4) + i) * 32 + lane; };
+  auto ask = [&](int base, float2 (&v)[kTsPerThread / 2]) {
 #pragma unroll
     for (int i = 0; i < kTsPerThread / 4; ++i) {
-      const int p = base + i * kTsThreads + tid;
-      const int e = p * 4 - skew;
+      const int p = packet(base, i), e = p * 4 - skew;
       if (p < p1 && e >= 0 && e + 3 < vocab) {
         const float4 f = __ldcs(reinterpret_cast<const float4*>(x + e));
-        ahead[4 * i] = f.x; ahead[4 * i + 1] = f.y; ahead[4 * i + 2] = f.z; ahead[4 * i + 3] = f.w;
+        v[2 * i] = make_float2(f.x, f.y);
+        v[2 * i + 1] = make_float2(f.z, f.w);
       } else {
+        float one[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) ahead[4 * i + j] = p < p1 && e + j >= 0 && e + j < vocab ? x[e + j] : -INFINITY;
+        for (int j = 0; j < 4; ++j) one[j] = p < p1 && e + j >= 0 && e + j < vocab ? x[e + j] : -INFINITY;
+        v[2 * i] = make_float2(one[0], one[1]);
+        v[2 * i + 1] = make_float2(one[2], one[3]);
       }
     }
   };
-  ask(p0);
-  for (int base = p0; base < p1; base += kTsTurn / 4) {
-    float v[kTsPerThread];
+  auto flush = [&]() {                                 // the list into the best
+    for (int i = 0; i < have; i += 32) best = ts_merge(best, i + lane < have ? sh.list[warp][i + lane] : 0, sh.best + warp * kTsMaxTop);
+    have = 0;
+    if (lane == 0) sh.count[warp] = 0;
+    const TsKey last = __shfl_sync(0xffffffffu, best, top - 1);
+    if (lane == 0 && last != 0) atomicMax(&sh.threshold, last);
+    __syncwarp();
+  };
+  auto work = [&](int base, const float2 (&v)[kTsPerThread / 2]) {
+    auto at = [&](int i) { return i % 2 ? v[i / 2].y : v[i / 2].x; };
+    float mx = fmaxf(v[0].x, v[0].y);
 #pragma unroll
-    for (int i = 0; i < kTsPerThread; ++i) v[i] = ahead[i];
-    if (base + kTsTurn / 4 < p1) ask(base + kTsTurn / 4);
-    float mx = v[0];
-#pragma unroll
-    for (int i = 1; i < kTsPerThread; ++i) mx = fmaxf(mx, v[i]);
+    for (int i = 1; i < kTsPerThread / 2; ++i) mx = fmaxf(mx, fmaxf(v[i].x, v[i].y));
     if (mx > m) {                                      // (never at +inf twice)
-      ts_move(m, mx, S, U);
+      ts_move(m, mx, S2.x, U2.x);
+      ts_move(m, mx, S2.y, U2.y);
       m = mx;
     }
     const float ref = m == -INFINITY ? 0.f : m;
+    const float2 ref2 = make_float2(ref, ref), log2e = make_float2(1.4426950408889634f, 1.4426950408889634f);
 #pragma unroll
-    for (int i = 0; i < kTsPerThread; ++i) {
-      const float z = v[i] - ref, e = ts_exp2(z * 1.4426950408889634f);
-      S += e;                                          // (a NaN stays in it; +inf shows in the maximum)
-      U = fmaf(e, fmaxf(z, -200.f), U);                // e^-200 is 0, and 0 * -200 is no NaN
+    for (int i = 0; i < kTsPerThread / 2; ++i) {
+      const float2 z = sub2(v[i], ref2), y = mul2(z, log2e);
+      const float2 e = make_float2(ts_exp2(y.x), ts_exp2(y.y));
+      S2 = add2(S2, e);                                // (a NaN stays in it; +inf shows in the maximum)
+      U2 = fma2(e, make_float2(fmaxf(z.x, -200.f), fmaxf(z.y, -200.f)), U2);      // e^-200 is 0, and 0 * -200 is no NaN
     }
-    if (TOP && want > 0) {
-      // indices of this thread's logits: 4 * (base + i * kTsThreads + tid) - skew + j
-      auto key_at = [&](int i) {
-        const int e = 4 * (base + (i >> 2) * kTsThreads + tid) - skew + (i & 3);
-        const bool here = base + (i >> 2) * kTsThreads + tid < p1 && e >= 0 && e < vocab;
-        return here ? ts_key(v[i], e) : (TsKey)0;
-      };
-      TsKey threshold = sh.threshold;
-      float least = ts_logit(threshold);               // (NaN, a threshold that is no number or none: everything comes in)
-      const int threads_with = __syncthreads_count(!(mx < least));
-      if (threads_with == 0) continue;                 // (the same in every thread)
-      if (threads_with * kTsPerThread + sh.count > kTsRoom) {
-        // raise the threshold: what the list holds down to the best, then the turn's group maxima
-        if (sh.count > want) {
-          const int n = sh.count;
-          ts_select(sh.list, n, want, sh.best);
-          __syncthreads();
-          if (tid < want) sh.list[tid] = sh.best[tid];
-          if (tid == 0) { sh.count = want; sh.threshold = max(sh.threshold, sh.best[want - 1]); }
-        }
-        TsKey mine = 0;
-        if (mx > -INFINITY) {                          // the first of the thread's largest (what is behind the row is -inf)
+    if (!TOP) return;
+    TsKey threshold = *const_cast<volatile TsKey*>(&sh.threshold);
+    float least = ts_logit(threshold);                 // (NaN, a threshold that is no number or none: everything comes in)
+    const int lanes_with = __popc(__ballot_sync(0xffffffffu, !(mx < least)));
+    if (lanes_with == 0) return;
+    auto key_at = [&](int i) {
+      const int p = packet(base, i / 4), e = 4 * p - skew + i % 4;
+      return p < p1 && e >= 0 && e < vocab ? ts_key(at(i), e) : (TsKey)0;
+    };
+    if (lanes_with > 16) {
+      TsKey mine = 0;
+      if (mx > -INFINITY) {                            // the first of the lane's largest (what is behind the row is -inf)
 #pragma unroll
-          for (int i = kTsPerThread - 1; i >= 0; --i)
-            if (v[i] == mx) mine = key_at(i);
-        } else {
+        for (int i = kTsPerThread - 1; i >= 0; --i)
+          if (at(i) == mx) mine = key_at(i);
+      } else {
 #pragma unroll
-          for (int i = 0; i < kTsPerThread; ++i) mine = max(mine, key_at(i));
-        }
-#pragma unroll
-        for (int o = 1; o < kTsThreads / kTsGroups; o <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
-        if (tid % (kTsThreads / kTsGroups) == 0) sh.group[tid / (kTsThreads / kTsGroups)] = mine;
-        __syncthreads();
-        if (tid < kTsGroups) {
-          // the want-th largest group maximum (groups without logits have 0: no bound)
-          const TsKey k = sh.group[tid];
-          int place = 0;
-          for (int j = 0; j < kTsGroups; ++j) place += sh.group[j] > k || (sh.group[j] == k && j < tid);
-          // a logit equal to the threshold has to come in as well: the threshold is one less
-          if (place == want - 1 && k > 0) atomicMax(&sh.threshold, k - 1);
-        }
-        __syncthreads();
-        threshold = sh.threshold;
-        least = ts_logit(threshold);
+        for (int i = 0; i < kTsPerThread; ++i) mine = max(mine, key_at(i));
       }
-      if (!(mx < least)) {
-#pragma unroll
-        for (int i = 0; i < kTsPerThread; ++i) {
-          if (v[i] < least) continue;
-          const TsKey k = key_at(i);
-          if (k > threshold) {
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < kTsRoom) sh.list[at] = k;
-          }
-        }
+      int place = 0;
+      for (int j = 0; j < 32; ++j) place += __shfl_sync(0xffffffffu, mine, j) > mine;
+      // (lanes without logits have 0 and come last; one less, so that the key itself comes in)
+      const unsigned who = __ballot_sync(0xffffffffu, place == top - 1 && mine != 0);
+      if (who) {
+        const TsKey raised = __shfl_sync(0xffffffffu, mine, __ffs(who) - 1) - 1;
+        if (raised > threshold) { threshold = raised; least = ts_logit(raised); }
       }
-      __syncthreads();
-      if (sh.count >= 2 * want) {                      // an exact threshold keeps the list short
-        const int n = min(sh.count, kTsRoom);
-        ts_select(sh.list, n, want, sh.best);
-        __syncthreads();
-        if (tid < want) sh.list[tid] = sh.best[tid];
-        if (tid == 0) { sh.count = want; sh.threshold = sh.best[want - 1]; }
-      }
-      __syncthreads();
     }
+    if (!(mx < least)) {
+#pragma unroll
+      for (int i = 0; i < kTsPerThread; ++i) {
+        if (at(i) < least) continue;
+        const TsKey k = key_at(i);
+        if (k > threshold) sh.list[warp][atomicAdd(&sh.count[warp], 1)] = k;
+      }
+    }
+    __syncwarp();
+    have = *const_cast<volatile int*>(&sh.count[warp]);
+    // with no threshold yet the first of them gives one
+    if (have >= 32 || (have > 0 && *const_cast<volatile TsKey*>(&sh.threshold) == 0)) flush();
+  };
+  // a turn's logits are asked for while the turn before is worked on
+  constexpr int kStep = kTsTurn / 4;
+  float2 a[kTsPerThread / 2], b[kTsPerThread / 2];
+  ask(p0, a);
+  for (int base = p0; base < p1; base += 2 * kStep) {
+    if (base + kStep < p1) ask(base + kStep, b);
+    work(base, a);
+    if (base + kStep >= p1) break;
+    if (base + 2 * kStep < p1) ask(base + 2 * kStep, a);
+    work(base + kStep, b);
+  }
+  float S = S2.x + S2.y, U = U2.x + U2.y;
+  if (TOP) {
+    flush();
+    if (lane < top) sh.merged[warp * top + lane] = best;        // (barriers follow, and no other block writes here yet)
   }
   // ---- threads to one maximum
   const float bm = block_max(m, sh.red);
   ts_move(m, bm, S, U);
   const float bU = block_sum(U, sh.red);
   const float bS = block_sum(S, sh.red);
-  if (TOP && want > 0) {
-    ts_select(sh.list, sh.count, want, sh.best);
+  if (TOP) {
+    if (tid < kTsMaxTop) sh.best[tid] = 0;
+    __syncthreads();
+    ts_select(sh.merged, kTsWarps * top, top, sh.best);
     __syncthreads();
   }
   // ---- blocks to the first of the cluster
@@ -214,7 +244,7 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
     cluster_wait();
     if (tid < 3) st_peer_f32(map_to_peer((uint32_t)__cvta_generic_to_shared(&sh.sums[slice][tid]), 0), tid == 0 ? bm : tid == 1 ? bS : bU);
     if (TOP && tid < top) {
-      const TsKey k = tid < want ? sh.best[tid] : 0;
+      const TsKey k = sh.best[tid];
       const uint32_t to = map_to_peer((uint32_t)__cvta_generic_to_shared(&sh.merged[slice * top + tid]), 0);
       asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(to), "l"(k) : "memory");
     }
@@ -245,21 +275,15 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
   }
   if (TOP) {
     TsKey* all = sh.merged;
-    const TsKey* best = sh.best;
+    const TsKey* found = sh.best;
     if (slices > 1) {
-      // empty places (key 0) are the smallest: a place below `top` is a real key's, for top <= vocab
-      for (int i = tid; i < slices * top; i += kTsThreads) {
-        const TsKey k = all[i];
-        if (k == 0) continue;
-        int place = 0;
-        for (int j = 0; j < slices * top; ++j) place += all[j] > k;
-        if (place < top) sh.list[place] = k;
-      }
-      best = sh.list;
+      // (a place below `top` is a real key's: top <= vocab)
+      ts_select(all, slices * top, top, sh.list[0]);
+      found = sh.list[0];
       __syncthreads();
     }
     if (tid < top) {
-      const int id = (int)~(uint32_t)best[tid];
+      const int id = (int)~(uint32_t)found[tid];
       top_id[row * top + tid] = id;
       top_logprob[row * top + tid] = bad ? nan : x[id] - M - log_sum;
     }
