@@ -5,12 +5,14 @@
 //   log p(t) = x_t - m - log S          entropy = log S - U / S
 //
 // A row is cut into slices, one block of a cluster each.  A thread keeps (m, S, U) of what it has read; threads, then blocks are
-// brought to one maximum.  The largest logits are found on the way, by every warp for itself, so that no barrier stands in the
-// loop: a 64-bit key holds the logit in an order of whole numbers and, below it, the index the other way round, so keys are
-// unique and of equal logits the lowest index is the largest.  A warp's lanes hold its best keys so far in order, one each; logits above
-// the block's threshold (the largest `top`-th best of any warp: as many are known to be no smaller) go to a list, and 32 of them
-// are ranked among the best by counting.  Where most lanes have one, as at the start, the threshold is first raised to the
-// `top`-th largest of the 32 lanes' maxima.  At the end the warps' best, then the blocks', are ranked the same way.
+// brought to one maximum.  The largest logits are found on the way: a 64-bit key holds the logit in an order of
+// whole numbers and, below it, the index the other way round, so keys are unique and of equal logits the lowest index is the
+// largest.  Logits above the block's threshold go to a list of their warp's; where that grows to 32, they are ranked among the warp's best, which
+// its lanes hold in order, by counting.  The threshold follows from what the threads know anyway: of 64 groups of four threads the
+// `top`-th largest maximum so far is no larger than the `top`-th best logit, and little smaller; it is taken after 1, 4, 16, ... turns, and
+// between those turns no barrier stands in the loop.  Where most lanes of a warp have a logit above it all the same (logits in ascending
+// order, or equal ones), it is raised for them to the `top`-th largest of the lanes' own.  At the end what the warps have, then what
+// the blocks have, is ranked the same way.
 //
 // Logits of -inf have no probability.  A row with a NaN, with +inf, or with -inf only has no distribution: its
 // log-probabilities and its entropy are NaN.  Its alternatives are the largest logits all the same, NaN behind all others.
@@ -25,6 +27,8 @@ constexpr int kTsTurn = kTsThreads * kTsPerThread;
 constexpr int kTsMaxTop = 32;
 constexpr int kTsRoom = 32 * kTsPerThread + 31;        // of a warp's list: a turn's logits, and fewer than 32 that were left
 constexpr int kTsMaxCluster = 8;
+constexpr int kTsGroups = kTsThreads / 4;
+static_assert(kTsGroups == 64, "six bits number the groups");
 static_assert(kTsWarps <= kTsMaxCluster, "the warps' best and the blocks' have one place");
 
 typedef unsigned long long TsKey;
@@ -58,11 +62,13 @@ __device__ __forceinline__ void ts_move(float m, float to, float& S, float& U) {
 
 struct TsShared {
   TsKey list[kTsWarps][kTsRoom];
-  TsKey best[kTsWarps * kTsMaxTop];                    // 32 for every warp to merge through; then the block's
+  TsKey all[kTsWarps * 64];                            // 32 for every warp to merge through; then what the warps have
+  TsKey best[kTsMaxTop];                               // of the block
   TsKey threshold;
-  TsKey merged[kTsMaxCluster * kTsMaxTop];             // every warp's best; then, in the first block of a cluster, every block's
+  TsKey merged[kTsMaxCluster * kTsMaxTop];             // in the first block of a cluster: every block's best
   float sums[kTsMaxCluster][3];                        // ... and its m, S, U
-  float red[33];
+  __align__(16) uint32_t group[kTsGroups];
+  float warp_sums[kTsWarps][3];
   int count[kTsWarps];
 };
 
@@ -72,6 +78,7 @@ __device__ __forceinline__ void ts_select(const TsKey* keys, int n, int top, TsK
     const TsKey k = keys[i];
     if (k == 0) continue;
     int place = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) place += keys[j] > k;
     if (place < top) best[place] = k;
   }
@@ -81,6 +88,7 @@ __device__ __forceinline__ void ts_select(const TsKey* keys, int n, int top, TsK
 __device__ __forceinline__ TsKey ts_merge(TsKey best, TsKey more, TsKey* through) {
   const int lane = threadIdx.x & 31;
   int place_best = lane, place_more = 0;
+#pragma unroll 4
   for (int j = 0; j < 32; ++j) {
     const TsKey b = __shfl_sync(0xffffffffu, best, j), n = __shfl_sync(0xffffffffu, more, j);
     place_more += (b > more) + (n > more);
@@ -98,7 +106,7 @@ __device__ __forceinline__ TsKey ts_merge(TsKey best, TsKey more, TsKey* through
 }
 
 template <bool TOP>
-__global__ void __launch_bounds__(kTsThreads, 3)
+__global__ void __launch_bounds__(kTsThreads, 4)
 token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, float* __restrict__ top_logprob, int* __restrict__ top_id,
                     const float* __restrict__ logits, const int* __restrict__ tokens, int vocab, int top, int slices) {
   extern __shared__ __align__(16) unsigned char smem[];
@@ -115,9 +123,10 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
   const int per = (packets + slices - 1) / slices;
   const int p0 = slice * per, p1 = min(packets, p0 + per);
   const int warp = tid >> 5, lane = tid & 31;
+  if (slices > 1) cluster_arrive();                    // (waited for before a peer is written to: every block of the cluster runs by then)
   if (TOP) {
     if (tid == 0) sh.threshold = 0;
-    if (lane == 0) sh.count[warp] = 0;
+    if (tid < kTsMaxTop) sh.best[tid] = 0;
     __syncthreads();
   }
   float m = -INFINITY;
@@ -144,14 +153,13 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
     }
   };
   auto flush = [&]() {                                 // the list into the best
-    for (int i = 0; i < have; i += 32) best = ts_merge(best, i + lane < have ? sh.list[warp][i + lane] : 0, sh.best + warp * kTsMaxTop);
+    for (int i = 0; i < have; i += 32) best = ts_merge(best, i + lane < have ? sh.list[warp][i + lane] : 0, sh.all + warp * 32);
     have = 0;
-    if (lane == 0) sh.count[warp] = 0;
     const TsKey last = __shfl_sync(0xffffffffu, best, top - 1);
     if (lane == 0 && last != 0) atomicMax(&sh.threshold, last);
     __syncwarp();
   };
-  auto work = [&](int base, const float2 (&v)[kTsPerThread / 2]) {
+  auto work = [&](int base, int turn, const float2 (&v)[kTsPerThread / 2]) {
     auto at = [&](int i) { return i % 2 ? v[i / 2].y : v[i / 2].x; };
     float mx = fmaxf(v[0].x, v[0].y);
 #pragma unroll
@@ -171,6 +179,28 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
       U2 = fma2(e, make_float2(fmaxf(z.x, -200.f), fmaxf(z.y, -200.f)), U2);      // e^-200 is 0, and 0 * -200 is no NaN
     }
     if (!TOP) return;
+    if ((turn & 0x55555555) == turn && (turn & (turn - 1)) == 0) {      // 1, 4, 16, ...: the same in every thread
+      float g = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 2));
+      // the maximum in the order of whole numbers, its last six bits the group's number: unique, and no larger
+      const uint32_t mine = ((uint32_t)(ts_key(g, 0) >> 32) & ~63u) | (uint32_t)(tid / 4);
+      if (tid % 4 == 0) sh.group[tid / 4] = mine;
+      __syncthreads();
+      int place = 0;                                   // each of a group's four threads looks at a quarter of the others
+#pragma unroll
+      for (int j = 0; j < kTsGroups / 16; ++j) {
+        const uint4 o = reinterpret_cast<const uint4*>(sh.group)[tid % 4 * (kTsGroups / 16) + j];
+        place += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+      }
+      place += __shfl_xor_sync(0xffffffffu, place, 1);
+      place += __shfl_xor_sync(0xffffffffu, place, 2);
+      // (-inf: a group without logits, or of no probability: no bound)
+      if (tid % 4 == 0 && place == top - 1 && g > -INFINITY) {
+        const TsKey bound = (TsKey)(mine & ~63u) << 32;          // below every key with that logit
+        if (bound > sh.threshold) sh.threshold = bound;          // (the one thread that writes between the barriers)
+      }
+      __syncthreads();
+    }
     TsKey threshold = *const_cast<volatile TsKey*>(&sh.threshold);
     float least = ts_logit(threshold);                 // (NaN, a threshold that is no number or none: everything comes in)
     const int lanes_with = __popc(__ballot_sync(0xffffffffu, !(mx < least)));
@@ -198,49 +228,63 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
         if (raised > threshold) { threshold = raised; least = ts_logit(raised); }
       }
     }
-    if (!(mx < least)) {
 #pragma unroll
-      for (int i = 0; i < kTsPerThread; ++i) {
-        if (at(i) < least) continue;
-        const TsKey k = key_at(i);
-        if (k > threshold) sh.list[warp][atomicAdd(&sh.count[warp], 1)] = k;
-      }
+    for (int i = 0; i < kTsPerThread; ++i) {
+      if (!__any_sync(0xffffffffu, !(at(i) < least))) continue;
+      const TsKey k = key_at(i);
+      const unsigned who = __ballot_sync(0xffffffffu, k > threshold);
+      if (k > threshold) sh.list[warp][have + __popc(who & ((1u << lane) - 1u))] = k;
+      have += __popc(who);
     }
     __syncwarp();
-    have = *const_cast<volatile int*>(&sh.count[warp]);
-    // with no threshold yet the first of them gives one
-    if (have >= 32 || (have > 0 && *const_cast<volatile TsKey*>(&sh.threshold) == 0)) flush();
+    if (have >= 32) flush();
   };
   // a turn's logits are asked for while the turn before is worked on
   constexpr int kStep = kTsTurn / 4;
   float2 a[kTsPerThread / 2], b[kTsPerThread / 2];
   ask(p0, a);
-  for (int base = p0; base < p1; base += 2 * kStep) {
+  int turn = 1;
+  for (int base = p0; base < p1; base += 2 * kStep, turn += 2) {
     if (base + kStep < p1) ask(base + kStep, b);
-    work(base, a);
+    work(base, turn, a);
     if (base + kStep >= p1) break;
     if (base + 2 * kStep < p1) ask(base + 2 * kStep, a);
-    work(base + kStep, b);
+    work(base + kStep, turn + 1, b);
   }
+  // ---- threads, then warps to one maximum; what the warps have side by side
   float S = S2.x + S2.y, U = U2.x + U2.y;
-  if (TOP) {
-    flush();
-    if (lane < top) sh.merged[warp * top + lane] = best;        // (barriers follow, and no other block writes here yet)
+  const float wm = warp_max(m);
+  ts_move(m, wm, S, U);
+  S = warp_sum(S);
+  U = warp_sum(U);
+  if (lane == 0) { sh.warp_sums[warp][0] = wm; sh.warp_sums[warp][1] = S; sh.warp_sums[warp][2] = U; }
+  const int kept = TOP ? __popc(__ballot_sync(0xffffffffu, best != 0)) : 0;
+  if (TOP && lane == 0) sh.count[warp] = kept + have;
+  __syncthreads();
+  float bm = -INFINITY, bS = 0.f, bU = 0.f;
+  int before = 0, found_all = 0;
+#pragma unroll
+  for (int w = 0; w < kTsWarps; ++w) bm = fmaxf(bm, sh.warp_sums[w][0]);
+#pragma unroll
+  for (int w = 0; w < kTsWarps; ++w) {
+    float s = sh.warp_sums[w][1], u = sh.warp_sums[w][2];
+    ts_move(sh.warp_sums[w][0], bm, s, u);
+    bS += s;
+    bU += u;
+    if (TOP) {
+      if (w < warp) before += sh.count[w];
+      found_all += sh.count[w];
+    }
   }
-  // ---- threads to one maximum
-  const float bm = block_max(m, sh.red);
-  ts_move(m, bm, S, U);
-  const float bU = block_sum(U, sh.red);
-  const float bS = block_sum(S, sh.red);
   if (TOP) {
-    if (tid < kTsMaxTop) sh.best[tid] = 0;
+    if (lane < kept) sh.all[before + lane] = best;
+    if (lane < have) sh.all[before + kept + lane] = sh.list[warp][lane];
     __syncthreads();
-    ts_select(sh.merged, kTsWarps * top, top, sh.best);
+    ts_select(sh.all, found_all, top, sh.best);
     __syncthreads();
   }
   // ---- blocks to the first of the cluster
   if (slices > 1) {
-    cluster_arrive();                                  // every block of the cluster runs before a peer writes into it
     cluster_wait();
     if (tid < 3) st_peer_f32(map_to_peer((uint32_t)__cvta_generic_to_shared(&sh.sums[slice][tid]), 0), tid == 0 ? bm : tid == 1 ? bS : bU);
     if (TOP && tid < top) {
@@ -303,7 +347,7 @@ PTL_EXPORT int ptl_token_scores(float* logprob, float* entropy, float* top_logpr
   PTL_REQUIRE((reinterpret_cast<uintptr_t>(logits) & 3u) == 0, "token_scores: logits must be 4-byte aligned");
   if (rows == 0) return 0;
   int slices = 1;
-  while (slices < kTsMaxCluster && (long long)rows * slices * 2 <= 1184 && vocab / (slices * 2) >= 4096) slices *= 2;
+  while (slices < kTsMaxCluster && (long long)rows * slices * 2 <= 592 && vocab / (slices * 2) >= 4096) slices *= 2;
   PTL_REQUIRE((long long)rows * slices <= 0x7fffffffLL, "token_scores: too many rows");
   static SmemRaised raised[2] = {};
   constexpr int kSmem = (int)sizeof(TsShared);
