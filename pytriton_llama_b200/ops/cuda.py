@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from array import array
 from typing import Optional, Tuple
 
 import numpy as np
@@ -958,18 +959,18 @@ class CudaOps:
         pages, _, nkv, page_size, d = codes.shape
         self._want_kv8(codes, words, nkv, d, page_size)
         self._want(block_table, "block_table", torch.int32)
-        contexts = np.ascontiguousarray(np.asarray(contexts, dtype=np.int64).reshape(-1))
-        if block_table.dim() != 2 or contexts.size > block_table.shape[0]:
-            raise KernelError(f"read_kv8: {contexts.size} requests, the table has {tuple(block_table.shape)} entries")
-        total = 0
-        if contexts.size:
-            low, high, total = int(contexts.min()), int(contexts.max()), int(contexts.sum())
-            if low < 0 or high > block_table.shape[1] * page_size:
-                raise KernelError(f"read_kv8: a request of {low if low < 0 else high} tokens does not fit its row of the table")
-        contexts = contexts.astype(np.int32)
+        contexts = contexts if isinstance(contexts, list) else np.asarray(contexts, dtype=np.int64).reshape(-1).tolist()
+        n = len(contexts)
+        if block_table.dim() != 2 or n > block_table.shape[0]:
+            raise KernelError(f"read_kv8: {n} requests, the table has {tuple(block_table.shape)} entries")
+        width = block_table.shape[1]
+        if n and (min(contexts) < 0 or max(contexts) > width * page_size):
+            raise KernelError(f"read_kv8: a request of {min(contexts) if min(contexts) < 0 else max(contexts)} tokens does not fit its row of the table")
+        total = sum(contexts)
+        lengths = array("i", contexts)
         out = self.empty((total, 2, nkv, d), dtype)
         fn = getattr(self.lib, "ptl_read_kv8" + _suffix(dtype))
-        self._check(fn(_p(out), _p(codes), _p(words), _p(block_table), contexts.ctypes.data, contexts.size, block_table.shape[1], nkv, d,
+        self._check(fn(out.data_ptr(), codes.data_ptr(), words.data_ptr(), block_table.data_ptr(), lengths.buffer_info()[0], n, width, nkv, d,
                        page_size, pages, self._stream()), kernels=1 if total else 0)
         return out
 
@@ -991,7 +992,7 @@ class CudaOps:
             raise KernelError("paged_attention8: fewer requests or positions than rows")
         if window < 0:
             raise KernelError(f"paged_attention8: a window of {window} positions")
-        out = self.empty((tokens, nq * d), q.dtype)
+        out = q.new_empty((tokens, nq * d))
         longest = getattr(hints, "max_ctx_len", 0) or block_table.shape[1] * page_size
         if window:
             longest = min(longest, window)
@@ -1029,7 +1030,7 @@ class CudaOps:
                 per_head = per_head if units is not None else 0
                 parts = 1
             if per_head:
-                scratch = self.empty((nkv * per_head * group * (d + 2),), torch.float32)      # partial outputs, then their maxima and sums
+                scratch = tok_req.new_empty(nkv * per_head * group * (d + 2))      # float32: partial outputs, then their maxima and sums
                 part_acc = scratch.data_ptr()
                 part_ml = part_acc + nkv * per_head * group * d * 4
                 counters = units.data_ptr() + nkv * per_head * 32
@@ -1054,7 +1055,7 @@ class CudaOps:
                 blocks = max(1, (q.shape[0] - n) * nq // (64 if q.dtype == torch.float32 or d == 128 else 128))
                 splits = max(1, min(self._sm_count * 3 // blocks, -(-longest // 256), 32))
             if splits > 1:
-                scratch = self.empty((q.shape[0] * nq * splits * (d + 2),), torch.float32)
+                scratch = tok_req.new_empty(q.shape[0] * nq * splits * (d + 2))      # float32
                 part_acc = scratch.data_ptr()
                 part_ml = part_acc + q.shape[0] * nq * splits * d * 4
             rc = getattr(self.lib, "ptl_attention8_portion" + suffix)(
@@ -1086,11 +1087,10 @@ class CudaOps:
                      + (5 + q.shape[0] * nq * s * (d + 2) * 8 / 3e6 if s > 1 else 0))
         part_acc = part_ml = None
         if splits > 1:
-            scratch = self.empty((q.shape[0] * nq * splits * (d + 2),), torch.float32)
+            scratch = block_table.new_empty(q.shape[0] * nq * splits * (d + 2))      # float32
             part_acc = scratch.data_ptr()
             part_ml = part_acc + q.shape[0] * nq * splits * d * 4
-        place = self.empty((pages * 2 * nkv * page_size * d,), torch.bfloat16)
-        table = self.empty((requests, width), torch.int32)
+        place, table = q.new_empty(pages * 2 * nkv * page_size * d), block_table.new_empty((requests, width))
         self._check(self.lib.ptl_kv8_expand_bf16(place.data_ptr(), table.data_ptr(), codes.data_ptr(), words.data_ptr(), block_table.data_ptr(),
                                                  tiles.tensor.data_ptr(), tiles.items, slots, width, width, nkv, d, page_size, codes.shape[0],
                                                  window, stream))
@@ -1110,7 +1110,7 @@ class CudaOps:
             key = (stream, dec.items, dec.in_order, *(x for t in integers for x in (t.data_ptr(), t._version)), rows, nq, nkv, d, int(window), per_head)
             if key in memo:
                 return memo[key][0]
-        units = self.empty((nkv * per_head * 8 + rows * nkv,), torch.int32)
+        units = tok_req.new_empty(nkv * per_head * 8 + rows * nkv)
         rc = self.lib.ptl_decode_units_zeroed(units.data_ptr(), units.data_ptr() + nkv * per_head * 32, rows * nkv,
                                               None if dec.in_order else _p(dec.tensor), _p(tok_req), _p(positions), dec.items, nq, nkv, d,
                                               int(window), per_head, stream)
@@ -1139,22 +1139,25 @@ class CudaOps:
         if not written.isdisjoint(src):
             raise KernelError("copy_pages: a row that is read is written too")
         low, high = min(min(src), min(dst)), max(max(src), max(dst))
-        held, device = [], self.device
+        device, held = self.device, []
         for t in tensors:
             if not t.is_contiguous() or t.device != device:
                 self._want(t, "a tensor of pages")
-            rows = t.shape[0] if t.dim() else 0
-            if low < 0 or high >= rows or high > 0x7fffffff:
-                raise KernelError(f"copy_pages: rows {low}..{high} of a tensor {tuple(t.shape)}")
+            shape = t.shape
+            if low < 0 or not shape or high >= shape[0] or high > 0x7fffffff:
+                raise KernelError(f"copy_pages: rows {low}..{high} of a tensor {tuple(shape)}")
             size = t.nbytes
             if size:
-                held.append((t.data_ptr(), size, size // rows))
-        in_order = sorted(held)
-        if any(a[0] + a[1] > b[0] for a, b in zip(in_order, in_order[1:])):
-            raise KernelError("copy_pages: two tensors share memory")
-        k = len(held)
+                held.append((t.data_ptr(), size, size // shape[0]))
+        end = 0
+        for at, size, _ in sorted(held):
+            if at < end:
+                raise KernelError("copy_pages: two tensors share memory")
+            end = at + size
+        base, row = array("Q", [x[0] for x in held]), array("q", [x[2] for x in held])
+        rows = array("i", src), array("i", dst)
         launches = _c_int(0)
-        self._check(self.lib.ptl_copy_pages((_ptr * k)(*[x[0] for x in held]), (_c_ll * k)(*[x[2] for x in held]), k, (_c_int * n)(*src), (_c_int * n)(*dst),
+        self._check(self.lib.ptl_copy_pages(base.buffer_info()[0], row.buffer_info()[0], len(held), rows[0].buffer_info()[0], rows[1].buffer_info()[0],
                                             n, ctypes.byref(launches), self._stream()), kernels=0)
         self.launches += launches.value
 
@@ -2648,9 +2651,10 @@ class CudaOps:
             raise KernelError(f"token_scores: {tokens.numel()} tokens for {rows} rows")
         if not 0 <= top <= self.SCORES_MAX_TOP:
             raise KernelError(f"token_scores: {top} alternatives, at most {self.SCORES_MAX_TOP}")
-        k, device = min(int(top), vocab), self.device
-        logprob, entropy = torch.empty((rows,), dtype=torch.float32, device=device), torch.empty((rows,), dtype=torch.float32, device=device)
-        best, ids = torch.empty((rows, k), dtype=torch.float32, device=device), torch.empty((rows, k), dtype=torch.int32, device=device)
+        k = min(int(top), vocab)
+        logprob = logits.new_empty(rows)                     # (half the host's time of torch.empty with a type and a device)
+        entropy = torch.empty_like(logprob)
+        best, ids = logits.new_empty((rows, k)), tokens.new_empty((rows, k))
         self._check(self.lib.ptl_token_scores(logprob.data_ptr(), entropy.data_ptr(), best.data_ptr(), ids.data_ptr(), logits.data_ptr(),
                                               tokens.data_ptr(), rows, vocab, k, self._stream()), kernels=1 if rows else 0)
         return logprob, entropy, best, ids
