@@ -410,24 +410,26 @@ template <int D, typename T, int NT> struct A8Rows {
 __device__ __forceinline__ float a8_weight(float m, float l, float M) { return l == 0.f ? 0.f : a8_exp2(m - M); }
 __device__ __forceinline__ float a8_inverse(float l) { return l == 0.f ? 0.f : 1.0f / l; }
 
-template <int D, int NT> struct A8Single {
+template <int D, int NT, int WARPS> struct A8Single {
   static constexpr int kRing = 4;                                          // slots a warp has
   static constexpr int kSlot = 2 * kKv8Block * D;
-  static constexpr int kRingBytes = kA8Warps * kRing * kSlot;
-  static constexpr int kJoinBytes = kA8Warps * 8 * NT * (D + 2) * 4 + 8 * NT * (D + 2) * 4;      // the warps' rows, and the block's: where the rings were
+  static constexpr int kRingBytes = WARPS * kRing * kSlot;
+  static constexpr int kJoinBytes = WARPS * 8 * NT * (D + 2) * 4;          // the warps' rows, where the rings were
+  static constexpr int kPartBytes = 8 * NT * D * 12 + 8 * 12;              // what a cluster's blocks send: (output, maximum, sum) of a share's entries
   static constexpr int kSmem = kRingBytes > kJoinBytes ? kRingBytes : kJoinBytes;
 };
 
-// Single tokens: the four warps of a block take turns through the keys of one (token, kv head), or of a part of them, and join
+// Single tokens: the warps of a block take turns through the keys of one (token, kv head), or of a part of them, and join
 // through shared memory.  The parts of a (token, kv head) join in a cluster, or, where the contexts are cut into parts of equal
-// length (the list of decode_units_kernel), in the block that ends last.  Every warp fetches its own keys, kRing blocks ahead.
-template <int D, typename T, int NT>
-__global__ void __launch_bounds__(kA8Warps * 32, NT == 1 && sizeof(T) == 2 ? (D == 64 ? 4 : 3) : 1)
+// length (the list of attention8_units_kernel), in the block that ends last.  Every warp fetches its own keys, kRing blocks ahead.  Eight warps
+// where there are fewer blocks than SMs: half the turns.
+template <int D, typename T, int NT, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, NT == 1 && sizeof(T) == 2 && WARPS == 4 ? (D == 64 ? 4 : 3) : 1)
 attention8_single_kernel(const A8Params p) {
-  using Cfg = A8Single<D, NT>;
+  using Cfg = A8Single<D, NT, WARPS>;
   constexpr int kRows = 8 * NT, kRing = Cfg::kRing;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ __align__(8) uint64_t s_full[kA8Warps][kRing];
+  __shared__ __align__(8) uint64_t s_full[WARPS][kRing];
   __shared__ int s_last;
   __shared__ volatile int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
@@ -438,6 +440,7 @@ attention8_single_kernel(const A8Params p) {
   }
   if (tid == 0) s_abort = 0;
   __syncthreads();
+  if (p.cluster) cluster_arrive();                           // (waited for before anything is sent: every block runs by then)
   pdl_wait();
   pdl_launch_dependents();
   const int group = p.nq / p.nkv;
@@ -447,7 +450,7 @@ attention8_single_kernel(const A8Params p) {
     const int4 a = p.units[2 * blockIdx.x], b = p.units[2 * blockIdx.x + 1];
     t = a.x; r = a.y; pos = a.z; kvh = a.w; split = b.x; splits = b.y;
     if (b.z >= 0)                                            // a row without a request: zeros
-      for (int e = tid; e < group * D; e += kA8Warps * 32) out[(size_t)b.z * p.out_stride + (size_t)b.w * group * D + e] = from_f32<T>(0.f);
+      for (int e = tid; e < group * D; e += WARPS * 32) out[(size_t)b.z * p.out_stride + (size_t)b.w * group * D + e] = from_f32<T>(0.f);
     if (t < 0) return;
     pair = t * p.nkv + kvh;
   } else {
@@ -460,7 +463,8 @@ attention8_single_kernel(const A8Params p) {
     pos = p.positions[t];
     if (r < 0) {                                             // (every block of a cluster alike)
       if (split == 0)
-        for (int e = tid; e < group * D; e += kA8Warps * 32) out[(size_t)t * p.out_stride + (size_t)kvh * group * D + e] = from_f32<T>(0.f);
+        for (int e = tid; e < group * D; e += WARPS * 32) out[(size_t)t * p.out_stride + (size_t)kvh * group * D + e] = from_f32<T>(0.f);
+      if (p.cluster) cluster_wait();
       return;
     }
   }
@@ -470,15 +474,11 @@ attention8_single_kernel(const A8Params p) {
   const int begin = b0 + min(blocks, split * per), end = b0 + min(blocks, (split + 1) * per);
   // ---- this warp's blocks: begin + warp + 4 i, i < count.  Lane l looks after blocks l, l + 32, ...: where they lie, their words, and their copies
   static_assert(kRing == 4 && kA8Turn == 2, "blocks i + 4 and i + 5 follow blocks i and i + 1 into their slots");
-  const int count = max(0, (end - begin - warp + kA8Warps - 1) / kA8Warps);
+  const int count = max(0, (end - begin - warp + WARPS - 1) / WARPS);
   const int* table = p.block_table + (size_t)r * p.bt_stride;
-  auto page_at = [&](int i) { return i < count ? p.page_of(table, begin + warp + kA8Warps * i) : -1; };
-  auto source = [&](int i, int page) { return page >= 0 ? p.keys<D>(page, kvh, p.sub_of(begin + warp + kA8Warps * i)) : nullptr; };
-  auto word_at = [&](int i, int page) {                       // with bit 8 of the keys' set: there is a page
-    uint2 w = page >= 0 ? p.word(page, kvh, p.sub_of(begin + warp + kA8Warps * i)) : make_uint2(0u, 0u);
-    if (page >= 0) w.x = (w.x & ~0xff00u) | 0x100u;
-    return w;
-  };
+  auto page_at = [&](int i) { return i < count ? p.page_of(table, begin + warp + WARPS * i) : -1; };
+  auto source = [&](int i, int page) { return page >= 0 ? p.keys<D>(page, kvh, p.sub_of(begin + warp + WARPS * i)) : nullptr; };
+  auto word_at = [&](int i, int page) { return page >= 0 ? p.word(page, kvh, p.sub_of(begin + warp + WARPS * i)) : make_uint2(0u, 0u); };
   const uint32_t slot0 = smem_addr(smem) + warp * (kRing * Cfg::kSlot);
   const size_t plane = p.plane<D>();
   auto fetch = [&](int slot, const unsigned char* src) {
@@ -493,10 +493,10 @@ attention8_single_kernel(const A8Params p) {
   A8Rows<D, T, NT> rows;
   typename A8Rows<D, T, NT>::Raw raw;
   rows.fetch(raw, p, t, 1, kvh, group);                       // (asked for beside the pages)
+  uint2 word_cur = word_at(lane, page0);                      // (before the copies, behind which it would wait)
   const unsigned char* src_cur = source(lane, page0);
   if (lane < min(kRing, count)) fetch(lane, src_cur);
   __syncwarp();
-  uint2 word_cur = word_at(lane, page0);
   rows.load(raw, p, 1, pos, group);
   int gave_up = -1;                                           // the block whose wait ran out
   for (int base = 0; base < count; base += 32) {
@@ -504,6 +504,7 @@ attention8_single_kernel(const A8Params p) {
     const unsigned char* src_nxt = source(base + 32 + lane, page_nxt);
     page_nxt = page_at(base + 64 + lane);
     const int stop = min(32, count - base);
+    const unsigned there = __ballot_sync(0xffffffffu, src_cur != nullptr);      // blocks with a page (none behind the last)
     for (int i = 0; i < stop; i += kA8Turn) {
       const unsigned char* slot[kA8Turn];
       bool have[kA8Turn];
@@ -513,8 +514,8 @@ attention8_single_kernel(const A8Params p) {
       for (int b = 0; b < kA8Turn; ++b) {
         word[b].x = __shfl_sync(0xffffffffu, word_cur.x, i + b);
         word[b].y = __shfl_sync(0xffffffffu, word_cur.y, i + b);
-        have[b] = (word[b].x >> 8) & 1u;                      // (not behind the last block)
-        key0[b] = (begin + warp + kA8Warps * (base + i + b)) * kKv8Block;
+        have[b] = (there >> (i + b)) & 1u;
+        key0[b] = (begin + warp + WARPS * (base + i + b)) * kKv8Block;
         slot[b] = smem + warp * (kRing * Cfg::kSlot) + ((i + b) % kRing) * Cfg::kSlot;
         if (i + b < stop && gave_up < 0 &&
             !__all_sync(0xffffffffu, mbar_wait(full0 + 8 * ((i + b) % kRing), ((base + i + b) / kRing) & 1, &s_abort, p.status, 9))) gave_up = base + i + b;
@@ -533,11 +534,11 @@ attention8_single_kernel(const A8Params p) {
   rows.finish();
   __syncthreads();                                            // the rings are read
   float(*s_o)[kRows][D] = reinterpret_cast<float(*)[kRows][D]>(smem);
-  float(*s_m)[kRows] = reinterpret_cast<float(*)[kRows]>(smem + kA8Warps * kRows * D * 4);
-  float(*s_l)[kRows] = s_m + kA8Warps;
-  float* s_part = reinterpret_cast<float*>(s_l + kA8Warps);
-  float* s_pm = s_part + kRows * D;
-  float* s_pl = s_pm + kRows;
+  float(*s_m)[kRows] = reinterpret_cast<float(*)[kRows]>(smem + WARPS * kRows * D * 4);
+  float(*s_l)[kRows] = s_m + WARPS;
+  // behind them, what the cluster's blocks send: [part][entry of this block's share] outputs, then maxima, then sums
+  float* s_part = reinterpret_cast<float*>(smem + Cfg::kSmem);
+  const int share = p.cluster ? (group * D + splits - 1) / splits : 0, shares = share * splits;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -551,13 +552,14 @@ attention8_single_kernel(const A8Params p) {
     }
   __syncthreads();
   const bool whole = splits == 1;
-  for (int e = tid; e < group * D; e += kA8Warps * 32) {
+  if (p.cluster) cluster_wait();                             // (every block of the cluster runs)
+  for (int e = tid; e < group * D; e += WARPS * 32) {
     const int row = e / D, col = e % D;
     float M = -INFINITY, L = 0.f, acc = 0.f;
 #pragma unroll
-    for (int i = 0; i < kA8Warps; ++i) M = fmaxf(M, s_m[i][row]);
+    for (int i = 0; i < WARPS; ++i) M = fmaxf(M, s_m[i][row]);
 #pragma unroll
-    for (int i = 0; i < kA8Warps; ++i) {
+    for (int i = 0; i < WARPS; ++i) {
       const float f = a8_weight(s_m[i][row], s_l[i][row], M);
       if (s_l[i][row] == 0.f) continue;
       L = fmaf(f, s_l[i][row], L);
@@ -566,8 +568,10 @@ attention8_single_kernel(const A8Params p) {
     if (whole) {
       out[(size_t)t * p.out_stride + (size_t)(kvh * group + row) * D + col] = from_f32<T>(acc * a8_inverse(L));
     } else if (p.cluster) {
-      s_part[e] = acc;
-      if (col == 0) { s_pm[row] = M; s_pl[row] = L; }
+      const uint32_t to = map_to_peer(smem_addr(s_part + split * share + e % share), e / share);
+      st_peer_f32(to, acc);
+      st_peer_f32(to + 4 * shares, M);
+      st_peer_f32(to + 8 * shares, L);
     } else {
       const size_t at = (size_t)blockIdx.x * group + row;
       p.part_acc[at * D + col] = acc;
@@ -576,38 +580,23 @@ attention8_single_kernel(const A8Params p) {
   }
   if (whole) return;
   if (p.cluster) {
-    // every block of the cluster finishes its share of the outputs from all of them
+    // every block of the cluster finishes its share of the outputs
     __syncwarp();
     cluster_arrive();
     cluster_wait();
-    const uint32_t at_o = smem_addr(s_part), at_m = smem_addr(s_pm), at_l = smem_addr(s_pl);
-    const int share = (group * D + splits - 1) / splits;
-    for (int e = split * share + tid; e < min(group * D, (split + 1) * share); e += kA8Warps * 32) {
-      const int row = e / D;
+    for (int e = tid; e < min(share, group * D - split * share); e += WARPS * 32) {
+      const int row = (split * share + e) / D, col = (split * share + e) % D;
       float M = -INFINITY, L = 0.f, acc = 0.f;
-      float ms[8], ls[8], os[8];
-#pragma unroll
-      for (int z = 0; z < 8; ++z) {
-        if (z < splits) {
-          ms[z] = ld_peer_f32(map_to_peer(at_m + 4 * row, z));
-          ls[z] = ld_peer_f32(map_to_peer(at_l + 4 * row, z));
-          os[z] = ld_peer_f32(map_to_peer(at_o + 4 * e, z));
-          M = fmaxf(M, ms[z]);
-        }
+      for (int z = 0; z < splits; ++z) M = fmaxf(M, s_part[shares + z * share + e]);
+      for (int z = 0; z < splits; ++z) {
+        const float m = s_part[shares + z * share + e], l = s_part[2 * shares + z * share + e];
+        if (l == 0.f) continue;
+        const float f = a8_weight(m, l, M);
+        L = fmaf(f, l, L);
+        acc = fmaf(f, s_part[z * share + e], acc);
       }
-#pragma unroll
-      for (int z = 0; z < 8; ++z) {
-        if (z < splits && ls[z] != 0.f) {
-          const float f = a8_weight(ms[z], ls[z], M);
-          L = fmaf(f, ls[z], L);
-          acc = fmaf(f, os[z], acc);
-        }
-      }
-      out[(size_t)t * p.out_stride + (size_t)(kvh * group + row) * D + e % D] = from_f32<T>(acc * a8_inverse(L));
+      out[(size_t)t * p.out_stride + (size_t)(kvh * group + row) * D + col] = from_f32<T>(acc * a8_inverse(L));
     }
-    __syncwarp();
-    cluster_arrive();
-    cluster_wait();                                          // nobody leaves while a peer still reads
     return;
   }
   // ---- the block that ends last among the parts joins them; nobody waits
@@ -619,7 +608,7 @@ attention8_single_kernel(const A8Params p) {
   if (tid == 0) p.counters[pair] = 0;                        // ready for the next layer
   __threadfence();
   const size_t at0 = (size_t)(blockIdx.x - split) * group;   // the parts of a (token, kv head) lie side by side
-  for (int e = tid; e < group * D; e += kA8Warps * 32) {
+  for (int e = tid; e < group * D; e += WARPS * 32) {
     const int row = e / D, col = e % D;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + at0 + row;
     const float* acc_of = p.part_acc + (at0 + row) * D + col;
@@ -830,22 +819,83 @@ int attention8_join_bf16(void* out, const float* part_acc, const float* part_ml,
                        dim3((128 * nq + kA8Warps - 1) / kA8Warps, n_tiles), dim3(kA8Warps * 32), 0, as_stream(stream), p);
 }
 
-template <int D, typename T, int NT>
+// The units that a step's single tokens are dealt out in: see decode_units_kernel (attention_decode.cu), whose list this is.  c is
+// ceil(tiles / (units - tokens)), which always suffices, and not the smallest that does: no search, three barriers in all; and the counters
+// that the parts join by are set to zero.  Tiles are 64 keys.  5.6 us by the search (64 tokens), 3 so.
+constexpr int kA8PlanItems = 1024;
+__global__ void __launch_bounds__(kA8PlanItems)
+attention8_units_kernel(int4* __restrict__ units, const int* __restrict__ items, const int* __restrict__ tok_req, const int* __restrict__ positions,
+                        int n_items, int nkv, int window, int per_head, int* __restrict__ counters, int n_counters) {
+  __shared__ int s_t[kA8PlanItems], s_r[kA8PlanItems], s_p[kA8PlanItems], s_first[kA8PlanItems + 1], s_sum[32], s_units[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_wait();
+  pdl_launch_dependents();
+  int t = -1, r = -1, p = -1, tiles = 0;
+  if (tid < n_items) {
+    t = items ? __ldg(items + tid) : tid;
+    r = __ldg(tok_req + t);
+    p = __ldg(positions + t);
+    const int keys = window > 0 && p + 1 > window ? window : p + 1;
+    tiles = r < 0 ? 0 : max(1, (keys + 63) / 64);
+  }
+  for (int i = tid; i < n_counters; i += kA8PlanItems) counters[i] = 0;
+  s_t[tid] = t; s_r[tid] = r; s_p[tid] = p;
+  const int sum = __reduce_add_sync(0xffffffffu, tiles);
+  if (lane == 0) s_sum[warp] = sum;
+  __syncthreads();
+  const int total = __reduce_add_sync(0xffffffffu, s_sum[lane]);
+  const int c = max(1, per_head > n_items ? (total + per_head - n_items - 1) / (per_head - n_items) : total);
+  const int mine = (tiles + c - 1) / c;
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int below = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += below;
+  }
+  if (lane == 31) s_units[warp] = incl;
+  __syncthreads();
+  const int before = __reduce_add_sync(0xffffffffu, lane < warp ? s_units[lane] : 0);
+  s_first[tid] = before + incl - mine;                       // units of the tokens before, per kv head
+  if (tid == kA8PlanItems - 1) s_first[kA8PlanItems] = before + incl;
+  __syncthreads();
+  const int units_per_head = s_first[kA8PlanItems];
+  for (int u = tid; u < nkv * per_head; u += kA8PlanItems) {
+    int4 a = make_int4(-1, -1, -1, 0), b = make_int4(0, 1, -1, 0);
+    if (u / nkv < units_per_head) {
+      int i = 0;                                             // the last token that begins at or before this unit
+#pragma unroll
+      for (int half = kA8PlanItems / 2; half; half >>= 1)
+        if (s_first[i + half] <= u / nkv) i += half;
+      const int n = s_first[i + 1] - s_first[i], at = u - s_first[i] * nkv;
+      a = make_int4(s_t[i], s_r[i], s_p[i], at / n);
+      b.x = at % n;
+      b.y = n;
+    }
+    if (u < n_items * nkv && s_r[u / nkv] < 0) { b.z = s_t[u / nkv]; b.w = u % nkv; }
+    units[2 * u] = a;
+    units[2 * u + 1] = b;
+  }
+}
+
+template <int D, typename T, int NT, int WARPS>
 static int launch_single(const A8Params& p, unsigned blocks, cudaStream_t stream) {
-  using Cfg = A8Single<D, NT>;
+  using Cfg = A8Single<D, NT, WARPS>;
   static SmemRaised raised = {};
-  if (int rc = raise_shared_memory("attention8_single", attention8_single_kernel<D, T, NT>, Cfg::kSmem, raised)) return rc;
-  return launch_kernel_cluster("attention8_single", attention8_single_kernel<D, T, NT>, dim3(blocks), dim3(kA8Warps * 32), Cfg::kSmem, stream,
-                               p.cluster ? p.splits : 1, p);
+  constexpr int kMost = Cfg::kSmem + Cfg::kPartBytes;
+  if (int rc = raise_shared_memory("attention8_single", attention8_single_kernel<D, T, NT, WARPS>, kMost, raised)) return rc;
+  const int share = (p.nq / p.nkv * D + p.splits - 1) / p.splits;
+  return launch_kernel_cluster("attention8_single", attention8_single_kernel<D, T, NT, WARPS>, dim3(blocks), dim3(WARPS * 32),
+                               Cfg::kSmem + (p.cluster ? share * p.splits * 12 : 0), stream, p.cluster ? p.splits : 1, p);
 }
 
 template <int D, typename T>
-static int launch_attention8(const A8Params& p, int singles, int tiles, int per_head, cudaStream_t stream) {
+static int launch_attention8(const A8Params& p, int singles, int tiles, int per_head, int warps, cudaStream_t stream) {
   const int group = p.nq / p.nkv;
   if (singles) {
     const long long blocks = per_head ? (long long)p.nkv * per_head : (long long)singles * p.nkv * p.splits;
     PTL_REQUIRE(blocks <= 0x7fffffffLL, "attention8: too many blocks");
-    return group <= 8 ? launch_single<D, T, 1>(p, (unsigned)blocks, stream) : launch_single<D, T, 2>(p, (unsigned)blocks, stream);
+    if (group > 8) return launch_single<D, T, 2, 4>(p, (unsigned)blocks, stream);
+    return warps == 8 ? launch_single<D, T, 1, 8>(p, (unsigned)blocks, stream) : launch_single<D, T, 1, 4>(p, (unsigned)blocks, stream);
   }
   using Cfg = A8Portion<D, T>;
   static SmemRaised raised = {};
@@ -858,7 +908,7 @@ static int launch_attention8(const A8Params& p, int singles, int tiles, int per_
 }
 
 template <typename T>
-static int attention8_mma(A8Params p, int singles, int tiles, int d, int page_size, int per_head, void* stream) {
+static int attention8_mma(A8Params p, int singles, int tiles, int d, int page_size, int per_head, int warps, void* stream) {
   PTL_REQUIRE(p.nq > 0 && p.nkv > 0 && page_size > 0 && p.num_pages > 0 && p.bt_stride > 0 && singles >= 0 && tiles >= 0, "attention8: bad sizes");
   PTL_REQUIRE(p.nq % p.nkv == 0, "attention8: %d query heads are no multiple of %d kv heads", p.nq, p.nkv);
   PTL_REQUIRE(page_size % kKv8Block == 0, "attention8: pages of %d positions are not whole blocks of %d", page_size, kKv8Block);
@@ -873,26 +923,27 @@ static int attention8_mma(A8Params p, int singles, int tiles, int d, int page_si
   p.page_shift = -1;
   for (int b = 0; b < 20; ++b) if ((1 << b) == p.blocks_per_page) p.page_shift = b;
   if (singles == 0 && tiles == 0) return 0;
-  return d == 64 ? launch_attention8<64, T>(p, singles, tiles, per_head, as_stream(stream)) : launch_attention8<128, T>(p, singles, tiles, per_head, as_stream(stream));
+  return d == 64 ? launch_attention8<64, T>(p, singles, tiles, per_head, warps, as_stream(stream))
+                 : launch_attention8<128, T>(p, singles, tiles, per_head, warps, as_stream(stream));
 }
 
 }  // namespace ptl
 
 // Single tokens: `items` their rows (null: 0..n_items-1).  With per_head > 0 the keys are dealt out in units (`units` from
-// ptl_decode_units_zeroed with the same sizes and with `counters`, one int per (row, kv head) of q), part_acc [nkv * per_head, nq / nkv, d] and part_ml
-// [..., 2]; else every (token, kv head) has `splits` parts, up to 8, which join in a cluster.  -2: sizes this kernel does not take.
+// ptl_attention8_units with the same sizes and with `counters`, one int per (row, kv head) of q), part_acc [nkv * per_head, nq / nkv, d] and part_ml
+// [..., 2]; else every (token, kv head) has `splits` parts, up to 8, which join in a cluster.  `warps` of a block: 4 or 8.  -2: sizes this kernel does not take.
 // *status: raised when a wait for a copy gave up.
 // Portions: with splits > 1 part_acc [rows of q, nq, splits, d] and part_ml [rows of q, nq, splits, 2], float32.
 #define PTL_ATTENTION8_MMA(NAME, T)                                                                                                         \
   PTL_EXPORT int ptl_attention8_single_##NAME(void* out, float* part_acc, float* part_ml, const void* q, const void* codes,                 \
                                               const void* words, const int* block_table, const int* items, const int* tok_req,             \
                                               const int* positions, int n_items, int q_stride, int out_stride, int bt_stride, int nq,       \
-                                              int nkv, int d, int page_size, float scale, int window, int splits, int per_head,             \
+                                              int nkv, int d, int page_size, float scale, int window, int splits, int warps, int per_head,  \
                                               const int* units, int* counters, int num_pages, int* status, void* stream) {                  \
     ptl::A8Params p{out, part_acc, part_ml, counters, q, (const unsigned char*)codes, (const uint32_t*)words, block_table, items, tok_req,  \
                     positions, (const int4*)units, status, q_stride, out_stride, bt_stride, nq, nkv, 0, 0, num_pages, window, splits,       \
                     per_head == 0 && splits > 1, scale * 1.4426950408889634f};                                                              \
-    return ptl::attention8_mma<T>(p, n_items, 0, d, page_size, per_head, stream);                                                           \
+    return ptl::attention8_mma<T>(p, n_items, 0, d, page_size, per_head, warps, stream);                                                    \
   }                                                                                                                                         \
   PTL_EXPORT int ptl_attention8_portion_##NAME(void* out, float* part_acc, float* part_ml, const void* q, const void* codes,                \
                                                const void* words, const int* block_table, const int* tiles, int n_tiles, int q_stride,      \
@@ -901,7 +952,18 @@ static int attention8_mma(A8Params p, int singles, int tiles, int d, int page_si
     ptl::A8Params p{out, part_acc, part_ml, nullptr, q, (const unsigned char*)codes, (const uint32_t*)words, block_table, tiles, nullptr,    \
                     nullptr, nullptr, status, q_stride, out_stride, bt_stride, nq, nkv, 0, 0, num_pages, window, splits, 0,                 \
                     scale * 1.4426950408889634f};                                                                                           \
-    return ptl::attention8_mma<T>(p, 0, n_tiles, d, page_size, 0, stream);                                                                  \
+    return ptl::attention8_mma<T>(p, 0, n_tiles, d, page_size, 0, 4, stream);                                                               \
   }
 PTL_ATTENTION8_MMA(f32, float)
 PTL_ATTENTION8_MMA(bf16, __nv_bfloat16)
+
+// units: 8 ints for each of nkv * per_head blocks, per_head at least n_items; counters: n_counters ints, set to zero.  -2: more tokens than one block lays out.
+PTL_EXPORT int ptl_attention8_units(int* units, int* counters, int n_counters, const int* items, const int* tok_req, const int* positions, int n_items,
+                                    int nkv, int window, int per_head, void* stream) {
+  using namespace ptl;
+  if (n_items > kA8PlanItems) return -2;
+  PTL_REQUIRE(n_items > 0 && nkv > 0 && per_head >= n_items && (long long)nkv * per_head <= (1 << 24) && units && aligned16(units) && counters && n_counters >= 0,
+              "attention8_units: bad sizes");
+  return launch_kernel("attention8_units", attention8_units_kernel, dim3(1), dim3(kA8PlanItems), 0, as_stream(stream), (int4*)units, items, tok_req,
+                       positions, n_items, nkv, window, per_head, counters, n_counters);
+}

@@ -66,14 +66,12 @@ constexpr int kDecPlanItems = 1024;
 
 __global__ void __launch_bounds__(kDecPlanItems)
 decode_units_kernel(int4* __restrict__ units, const int* __restrict__ items, const int* __restrict__ tok_req,
-                    const int* __restrict__ positions, int n_items, int nkv, int window, int per_head, int tile_keys, int max_splits,
-                    int* __restrict__ zeros, int n_zeros) {
+                    const int* __restrict__ positions, int n_items, int nkv, int window, int per_head, int tile_keys, int max_splits) {
   __shared__ int s_t[kDecPlanItems], s_r[kDecPlanItems], s_p[kDecPlanItems], s_tiles[kDecPlanItems], s_first[kDecPlanItems + 1];
   __shared__ int s_sum[32], s_max[32], s_fits[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_wait();
   pdl_launch_dependents();
-  for (int i = tid; i < n_zeros; i += kDecPlanItems) zeros[i] = 0;
   int t = -1, r = -1, p = -1, tiles = 0;
   if (tid < n_items) {
     t = items ? items[tid] : tid;
@@ -854,18 +852,7 @@ PTL_EXPORT int ptl_decode_units(int* units, const int* items, const int* tok_req
   static_assert(DecodeCfg<64, 1, 3>::kKeys == DecodeCfg<128, 1, 2>::kKeys, "the forms that take units have tiles of one size");
   const int max_splits = (d == 64 ? DecodeCfg<64, 1, 3>::kMaxSums : DecodeCfg<128, 1, 2>::kMaxSums) / (nq / nkv);
   return launch_kernel("decode_units", decode_units_kernel, dim3(1), dim3(kDecPlanItems), 0, as_stream(stream), (int4*)units, items, tok_req,
-                       positions, n_items, nkv, window, per_head, (int)DecodeCfg<64, 1, 3>::kKeys, max_splits, (int*)nullptr, 0);
-}
-
-// The same, with counters that the blocks of an attention over these units join by set to zero: `counters` n_counters ints.
-PTL_EXPORT int ptl_decode_units_zeroed(int* units, int* counters, int n_counters, const int* items, const int* tok_req, const int* positions,
-                                       int n_items, int nq, int nkv, int d, int window, int per_head, void* stream) {
-  using namespace ptl;
-  if (n_items > kDecPlanItems || (d != 64 && d != 128)) return -2;
-  PTL_REQUIRE(n_items > 0 && nkv > 0 && nq % nkv == 0 && nq / nkv <= 16 && per_head >= n_items && (long long)nkv * per_head <= (1 << 24) &&
-                  units && aligned16(units) && counters && n_counters >= 0, "decode_units: bad sizes");
-  return launch_kernel("decode_units", decode_units_kernel, dim3(1), dim3(kDecPlanItems), 0, as_stream(stream), (int4*)units, items, tok_req,
-                       positions, n_items, nkv, window, per_head, (int)DecodeCfg<64, 1, 3>::kKeys, 1 << 20, counters, n_counters);
+                       positions, n_items, nkv, window, per_head, (int)DecodeCfg<64, 1, 3>::kKeys, max_splits);
 }
 
 // Either form (fused != 0: as ptl_decode_attention_rope_bf16) for pages of whole sixteens of positions, fetched by TMA; -2 for

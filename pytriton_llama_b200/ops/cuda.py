@@ -10,6 +10,7 @@ or loaded, raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from array import array
 from typing import Optional, Tuple
@@ -94,7 +95,7 @@ _SIGNATURES = {
     "ptl_rope_kv8_write": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ll, _ptr],
     "ptl_read_kv8": [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr],
     "ptl_attention8_single": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
-                              _c_int, _c_f, _c_int, _c_int, _c_int, _ptr, _ptr, _c_int, _ptr, _ptr],
+                              _c_int, _c_f, _c_int, _c_int, _c_int, _c_int, _ptr, _ptr, _c_int, _ptr, _ptr],
     "ptl_attention8_portion": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f,
                                _c_int, _c_int, _c_int, _ptr, _ptr],
     "ptl_attention8_simt": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
@@ -173,8 +174,8 @@ def load_library() -> ctypes.CDLL:
                                                     _c_int, _ptr, _ptr, _ptr, _ptr]
     lib.ptl_decode_units.argtypes = [_ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr]
     lib.ptl_decode_units.restype = _c_int
-    lib.ptl_decode_units_zeroed.argtypes = [_ptr, _ptr, _c_int, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr]
-    lib.ptl_decode_units_zeroed.restype = _c_int
+    lib.ptl_attention8_units.argtypes = [_ptr, _ptr, _c_int, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _ptr]
+    lib.ptl_attention8_units.restype = _c_int
     lib.ptl_decode_attention_pages_bf16.restype = _c_int
     lib.ptl_prefill_attention_bf16.argtypes = [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                                _c_int, _c_int, _c_f, _c_int, _c_int, _ptr]
@@ -999,7 +1000,7 @@ class CudaOps:
         dec, tiles = self._work(hints, "decode_items"), self._work(hints, "prefill_tiles")
         if d in (64, 128) and nq // nkv <= 16 and dec is not None and tiles is not None and q.shape[1] % 8 == 0:
             if self._attention8_tensor_cores(out, q, codes, words, block_table, tok_req, positions, nq, nkv, d, page_size, float(scale),
-                                             int(window), longest, dec, tiles, getattr(hints, "split_portions", None)):
+                                             int(window), longest, dec, tiles, getattr(hints, "split_portions", None), getattr(hints, "single_form", None)):
                 return out
         # blocks of 128 keys' turns: split until they fill the machine a few times
         splits = max(1, min(-(-longest // 256), 148 * 8 // max(1, tokens * nq), 64))
@@ -1013,22 +1014,59 @@ class CudaOps:
                        self._stream()), kernels=(2 if splits > 1 else 1) if tokens else 0)
         return out
 
+    @staticmethod
+    def _kv8_fit(d: int, float32: bool, wide: bool, warps: int = 4) -> int:
+        """Blocks of single tokens' attention over an 8-bit cache that run at once (by their registers)."""
+        if warps == 8:
+            return 296 if d == 64 and not float32 else 148
+        return 296 if wide or (d == 128 and float32) else 444 if d == 128 or float32 else 592
+
+    @staticmethod
+    @functools.lru_cache(maxsize=4096)
+    def _kv8_single_form(n: int, nkv: int, keys256: int, d: int, float32: bool, wide: bool):
+        """(parts of a token's keys that join in a cluster, warps of a block) of n single tokens with up to 256 * keys256 keys, or (0, 4): their
+        keys dealt out in units of equal length.  By what the forms take: a block 5 us with heads of 64 and 7 with 128, 2 more for
+        every further round of blocks; a cluster 1.2, and 0.3 for every doubling of the parts (more than run at once are taken only
+        whole: clusters wait for room); a turn of 32 keys a warp 1.5 and 2.0 us where the machine is full and 1.1 and 1.5 where it is
+        not; units 7 us for their list and the join, and 0.08 a part.  Measured (bfloat16, heads of 64 over 8 kv heads), us, by units, whole with 8
+        warps, and the best: one token of 4,000 19, 24 and 8.1 (8 parts, 8 warps), of 16,000 21, 85 and 16, of 120,000 42, 617 and 42; 8 of
+        4,096 17, 25 and 13 (8 parts, 4 warps); 16 of 1,000 14, 9.4 and 9.4; 64 of 256 to 2,560 36, 28 and 28; 128 of 300 to 600 26, 31 and 22
+        (whole, 4 warps).  Heads of 128: 8 of 20,011 to 30,011 80 by units, 113 by the next best."""
+        pairs = n * nkv
+        base, turn = (5.0, 1.5) if d == 64 else (7.0, 2.0)
+        best = None
+        for warps in (4,) if wide else (8, 4):
+            fit = CudaOps._kv8_fit(d, float32, wide, warps)
+            for parts in (1, 2, 4, 8):
+                blocks = pairs * parts
+                if parts > 1 and blocks > fit:
+                    break
+                turns = max(1, -(-keys256 * 8 // (parts * warps)))
+                cost = base + (0.9 + 0.3 * parts.bit_length() if parts > 1 else 0) + max(1.0, blocks / fit) * turns * turn * (
+                    0.73 + 0.27 * min(1.0, blocks / fit)) + 2 * (-(-blocks // fit) - 1)
+                if best is None or cost < best[0]:
+                    best = (cost, parts, warps)
+        fit = CudaOps._kv8_fit(d, float32, wide)
+        if pairs <= fit and n <= 1024 and base + 7 + -(-pairs * keys256 * 8 // (fit * 4)) * turn + 0.08 * fit / pairs < best[0]:
+            return 0, 4
+        return best[1], best[2]
+
     def _attention8_tensor_cores(self, out, q, codes, words, block_table, tok_req, positions, nq, nkv, d, page_size, scale, window, longest,
-                                 dec, tiles, split_portions=None) -> bool:
+                                 dec, tiles, split_portions=None, force=None) -> bool:
         """Single tokens and portions by the tensor-core kernels; False where they do not take the sizes (nothing has run then)."""
         stream, n, suffix = self._stream(), dec.items, _suffix(q.dtype)
         if tiles.items > 65535:
             return False
         if n:
             pairs = n * nkv
-            fit = self.DECODE_UNITS[d]               # blocks that fit at once
-            parts = max(1, min(8, 296 // pairs, -(-longest // 128)))
-            per_head, units, counters, part_acc, part_ml, group = 0, None, None, None, None, nq // nkv
-            if (parts < 2 or longest > 1024 * parts) and pairs <= fit * 7 // 8 and longest > 64:
-                per_head = max(fit // nkv, n)
+            group = nq // nkv
+            per_head, units, counters, part_acc, part_ml = 0, None, None, None, None
+            parts, warps = force or self._kv8_single_form(n, nkv, -(-longest // 256), d, q.dtype == torch.float32, group > 8)
+            if not parts:
+                per_head = max(self._kv8_fit(d, q.dtype == torch.float32, group > 8) // nkv, n)
                 units = self._decode8_unit_list(dec, tok_req, positions, q.shape[0], nq, nkv, d, window, per_head)
                 per_head = per_head if units is not None else 0
-                parts = 1
+                parts, warps = 1, 4
             if per_head:
                 scratch = tok_req.new_empty(nkv * per_head * group * (d + 2))      # float32: partial outputs, then their maxima and sums
                 part_acc = scratch.data_ptr()
@@ -1037,7 +1075,7 @@ class CudaOps:
             rc = getattr(self.lib, "ptl_attention8_single" + suffix)(
                 out.data_ptr(), part_acc, part_ml, q.data_ptr(), codes.data_ptr(), words.data_ptr(), block_table.data_ptr(),
                 None if dec.in_order else dec.tensor.data_ptr(), tok_req.data_ptr(), positions.data_ptr(), n, q.shape[1], nq * d,
-                block_table.shape[1], nq, nkv, d, page_size, scale, window, parts, per_head, _p(units), counters, codes.shape[0], _p(self._tc_status_word()), stream)
+                block_table.shape[1], nq, nkv, d, page_size, scale, window, parts, warps, per_head, _p(units), counters, codes.shape[0], _p(self._tc_status_word()), stream)
             if rc == -2:
                 return False
             self._check(rc)
@@ -1111,9 +1149,9 @@ class CudaOps:
             if key in memo:
                 return memo[key][0]
         units = tok_req.new_empty(nkv * per_head * 8 + rows * nkv)
-        rc = self.lib.ptl_decode_units_zeroed(units.data_ptr(), units.data_ptr() + nkv * per_head * 32, rows * nkv,
-                                              None if dec.in_order else _p(dec.tensor), _p(tok_req), _p(positions), dec.items, nq, nkv, d,
-                                              int(window), per_head, stream)
+        rc = self.lib.ptl_attention8_units(units.data_ptr(), units.data_ptr() + nkv * per_head * 32, rows * nkv,
+                                           None if dec.in_order else dec.tensor.data_ptr(), tok_req.data_ptr(), positions.data_ptr(), dec.items, nkv,
+                                           int(window), per_head, stream)
         if rc == -2:
             return None
         self._check(rc)
