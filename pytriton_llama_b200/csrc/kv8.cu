@@ -78,7 +78,10 @@ rope_kv8_write_kernel(const Kv8WriteParams p) {
   const int mine = p.block_of(t0 - 1 + lane);                  // (rows t0 - 1 .. t0 + 30)
   const int before = __shfl_up_sync(0xffffffffu, mine, 1);
   const unsigned leads = __ballot_sync(0xffffffffu, lane >= 1 && t0 - 1 + lane < t1 && mine >= 0 && mine != before) >> 1;      // bit i: row t0 + i begins a run
-  if (!leads && (p.nq == 0 || !TURN)) return;
+  if (!leads && (p.nq == 0 || !TURN)) {
+    pdl_wait();                                  // (what comes after this kernel counts on the one before it being through)
+    return;
+  }
   int staged = 0;                                              // rows from t0 on whose angles are in shared memory
   if constexpr (TURN) {
     const int last = 31 - __clz(leads | 1u);                   // the last run's first row, and up to 16 of its rows
