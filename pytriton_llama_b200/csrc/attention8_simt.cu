@@ -44,7 +44,7 @@ attention8_simt_kernel(T* __restrict__ out, float* __restrict__ part_acc, float*
     float s = -INFINITY, vstep = 0.f;
     const unsigned char* vrow = nullptr;
     if (key <= p) {
-      const int page = block_table[(size_t)r * bt_stride + key / page_size], off = key % page_size;
+      const int block = key / page_size, page = block < bt_stride ? block_table[(size_t)r * bt_stride + block] : -1, off = key % page_size;
       if (page >= 0 && page < num_pages) {
         const unsigned char* krow = codes + (size_t)page * 2 * plane + ((size_t)kvh * page_size + off) * d;
         vrow = krow + plane;

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import os
 from array import array
 from typing import Optional, Tuple
@@ -993,6 +994,8 @@ class CudaOps:
             raise KernelError("paged_attention8: fewer requests or positions than rows")
         if window < 0:
             raise KernelError(f"paged_attention8: a window of {window} positions")
+        if not 0 <= scale < math.inf:
+            raise KernelError(f"paged_attention8: scores times {scale}")
         out = q.new_empty((tokens, nq * d))
         longest = getattr(hints, "max_ctx_len", 0) or block_table.shape[1] * page_size
         if window:

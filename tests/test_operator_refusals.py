@@ -78,6 +78,8 @@ def test_tensors_of_another_device(ops):
     (dict(page_size=24), "no whole blocks"),
     (dict(d=512), "up to 256"),
     (dict(window=-1), "window"),
+    (dict(scale=-0.125), "scores times"),
+    (dict(scale=float("nan")), "scores times"),
 ])
 def test_attention(ops, over, message):
     a = dict(q=torch.zeros((3, 256), dtype=BF), block_table=torch.zeros((1, 2), dtype=I32), tok_req=torch.zeros(3, dtype=I32),
