@@ -19,7 +19,8 @@
 // normal numbers, is multiplied by itself and added with its step, as every block of a warp of one tile is.
 //
 // A row's reference maximum only moves when a score is above it by more than 2^8: the comparison is one vote a turn, and
-// the reduction over the keys' lanes and the rescaling of the output happen a few times a row.
+// the reduction over the keys' lanes and the rescaling of the output happen a few times a row.  Weights count in units of 2^-7, so that
+// the largest are 2^15, and those that half floats hold with fewer bits are below 2^-21 of e^reference (2^-13 in a block of small steps).
 //
 // Keys and values of 16 positions and a head are 16 D bytes each in one piece, and come by bulk copies into rings of slots in shared memory.
 // Waits for them are bounded: one that gives up says so in *status, and the block ends once its copies have.
@@ -30,6 +31,7 @@ namespace ptl {
 
 constexpr int kA8Warps = 4;
 constexpr int kA8Turn = 2;                                    // blocks of 16 keys a turn
+constexpr float kA8Lift = 7.0f;                               // weights are 2^7 e^(score - reference), at most 2^15
 
 struct A8Params {
   void* out;
@@ -313,7 +315,7 @@ template <int D, typename T, int NT> struct A8Rows {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float pr[4];
-        const float use[2] = {(m[n][0] == -INFINITY ? 0.f : m[n][0]) - shift, (m[n][1] == -INFINITY ? 0.f : m[n][1]) - shift};
+        const float use[2] = {(m[n][0] == -INFINITY ? 0.f : m[n][0]) - (shift + kA8Lift), (m[n][1] == -INFINITY ? 0.f : m[n][1]) - (shift + kA8Lift)};
 #pragma unroll
         for (int e = 0; e < 4; ++e) pr[e] = a8_exp2(fmaf(s[b][n][e], f[b][n][e & 1], -use[e & 1]));
 #pragma unroll

@@ -72,13 +72,18 @@ def attend(q, values, bad, positions, scale, window=0):
     return out, size, score
 
 
-def tolerance(dtype, out, size, score, d, keys, weights=torch.float16):
+def tolerance(dtype, out, size, score, d, keys, weights=torch.float16, largest=0.0):
     """How far a kernel may be off: the output's rounding, half a step of the type; weights rounded to ``weights`` (bfloat16 rows: half floats for
     single tokens, bfloat16 for portions on the fifth-generation tensor cores), half a step of each, 2^-11 or 2^-8
     (and 2^-25 of the largest where half floats leave the normal numbers, keys of them at most); 2 eps for a relative error eps of
     e^s, where a score's d products and sums in float32, two more for its scale and the exponential's few ulps, err by
-    (d + 8) 2^-24 of |q| |k| scale; and the float32 sums over the keys."""
+    (d + 8) 2^-24 of |q| |k| scale; and the float32 sums over the keys.
+
+    ``largest``: the largest |v| of the request, where values lie so far apart that the smallest weights matter.  Weights are half floats (float32:
+    two, the second of what the first leaves) in units of 2^-7, and half floats are 2^-24 apart below 2^-14, so a weight is off by up to
+    2^-25 of those units, 2^-32 of the largest weight, which is at least 1 of the row's sum's terms; in blocks whose weights carry their
+    step, by as much in units of the largest step, whose block has a value of at least 64 of its steps where codes count up to 128: 2^-31 |v| a key."""
     half = torch.finfo(dtype).eps / 2
     eps = (d + 8) * 2.0 ** -24 * (1 + score[..., None])
     rounding = torch.finfo(weights).eps / 2 + keys * 2.0 ** -25 if dtype == torch.bfloat16 else 2.0 ** -22
-    return half * out.abs() + size * (2 * eps + 2 * rounding + (keys + 64) * 2.0 ** -24) + 1e-30
+    return half * out.abs() + size * (2 * eps + 2 * rounding + (keys + 64) * 2.0 ** -24) + keys * 2.0 ** -31 * largest + 1e-30

@@ -216,7 +216,7 @@ STEPS = {  # (new tokens, tokens cached before) of the requests
 }
 
 
-def run_attention(ops, nq, G, d, ps, step, dtype, window=0, spoil=None, extra=0, seed=0, gain=1.0):
+def run_attention(ops, nq, G, d, ps, step, dtype, window=0, spoil=None, extra=0, seed=0, gain=1.0, far=False):
     t = DTYPES[dtype]
     lens = [n + c for n, c in step]
     pool = Pool(ops, G, d, ps, lens, seed=seed + d)
@@ -246,7 +246,8 @@ def run_attention(ops, nq, G, d, ps, step, dtype, window=0, spoil=None, extra=0,
         mine = got[at:at + n].double().cpu().view(n, nq, d)
         assert torch.equal(torch.isnan(mine), torch.isnan(out)), (r, n, c)
         fine = ~torch.isnan(out)
-        off = (mine - out).abs()[fine] / tolerance(t, out, size, score, d, n + c, torch.float16 if n == 1 else torch.bfloat16)[fine]
+        off = (mine - out).abs()[fine] / tolerance(t, out, size, score, d, n + c, torch.float16 if n == 1 else torch.bfloat16,
+                                                   v[:, 1].abs().max() if far else 0.0)[fine]
         assert off.numel() == 0 or off.max() <= 1, (r, n, c, float(off.max()))
         at += n
     return got, pool, qkv, req, pos, hints
