@@ -86,7 +86,7 @@ struct PrefillTcParams {
   int* status;
   int out_stride, bt_stride, nq, nkv, page_size, window, num_pages;
   float scale_log2;
-  int splits;                      // HOLES: of the keys; with more than one
+  int splits, split_tiles;         // HOLES: parts that the keys are cut into and key tiles of one (more where that would leave some out); with more than one
   float* part_acc;                 // [rows of q][nq][splits][D]
   float* part_ml;                  // [rows of q][nq][splits][2], the maximum in units of log2
 };
@@ -160,7 +160,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
   int tiles_of_split = 0x7fffffff;
   if (HOLES && p.splits > 1) {
     const int all = (max(k_end[0], rows_g[1] > 0 ? k_end[1] : 0) - k_base + kTcKeys - 1) / kTcKeys;
-    tiles_of_split = (all + p.splits - 1) / p.splits;
+    tiles_of_split = max(p.split_tiles, (all + p.splits - 1) / p.splits);
     k_base += blockIdx.z * tiles_of_split * kTcKeys;
   }
 #pragma unroll
@@ -651,7 +651,7 @@ static int launch_prefill_tc(const void* q, const void* cache, int n_tiles, int 
 static int prefill_attention_tc_entry(void* out, const void* q, const void* cache, const int* block_table,
                                       const int* tiles, int n_tiles, int n_tokens, int q_stride, int out_stride,
                                       int bt_stride, int nq, int nkv, int d, int page_size, float scale,
-                                      int window, int num_pages, bool holes, int splits, float* part_acc, float* part_ml, int* status,
+                                      int window, int num_pages, bool holes, int splits, int split_tiles, float* part_acc, float* part_ml, int* status,
                                       void* stream) {
   using namespace ptl;
   PTL_REQUIRE(n_tiles >= 0 && nq > 0 && nkv > 0 && page_size > 0 && num_pages > 0, "prefill_attention_tc: bad sizes");
@@ -667,7 +667,7 @@ static int prefill_attention_tc_entry(void* out, const void* q, const void* cach
   p.out = (__nv_bfloat16*)out; p.block_table = block_table; p.tiles = tiles; p.status = status;
   p.out_stride = out_stride; p.bt_stride = bt_stride; p.nq = nq; p.nkv = nkv; p.page_size = page_size;
   p.window = window; p.num_pages = num_pages; p.scale_log2 = scale * 1.4426950408889634f;
-  p.splits = splits; p.part_acc = part_acc; p.part_ml = part_ml;
+  p.splits = splits; p.split_tiles = split_tiles; p.part_acc = part_acc; p.part_ml = part_ml;
   if (holes)
     return d == 64 ? launch_prefill_tc<64, true>(q, cache, n_tiles, n_tokens, q_stride, nq, nkv, page_size, num_pages, p, as_stream(stream))
                    : launch_prefill_tc<128, true>(q, cache, n_tiles, n_tokens, q_stride, nq, nkv, page_size, num_pages, p, as_stream(stream));
@@ -680,7 +680,7 @@ PTL_EXPORT int ptl_prefill_attention_tc_bf16(void* out, const void* q, const voi
                                              int bt_stride, int nq, int nkv, int d, int page_size, float scale,
                                              int window, int num_pages, int* status, void* stream) {
   return prefill_attention_tc_entry(out, q, cache, block_table, tiles, n_tiles, n_tokens, q_stride, out_stride, bt_stride, nq, nkv, d, page_size,
-                                    scale, window, num_pages, false, 1, nullptr, nullptr, status, stream);
+                                    scale, window, num_pages, false, 1, 0, nullptr, nullptr, status, stream);
 }
 
 namespace ptl {
@@ -689,17 +689,17 @@ int attention8_join_bf16(void* out, const float* part_acc, const float* part_ml,
                          void* stream);
 }  // namespace ptl
 
-// The same where pages may be missing (-1) in the middle of a request; the cache's last page is zeros.  splits > 1: of the keys, with part_acc
-// [n_tokens, nq, splits, d] and part_ml [n_tokens, nq, splits, 2] float32.
+// The same where pages may be missing (-1) in the middle of a request; the cache's last page is zeros.  splits > 1: of the keys, split_tiles tiles of
+// them each, with part_acc [n_tokens, nq, splits, d] and part_ml [n_tokens, nq, splits, 2] float32.
 PTL_EXPORT int ptl_prefill_attention_tc_holes_bf16(void* out, const void* q, const void* cache, const int* block_table,
                                                    const int* tiles, int n_tiles, int n_tokens, int q_stride, int out_stride,
                                                    int bt_stride, int nq, int nkv, int d, int page_size, float scale,
-                                                   int window, int num_pages, int splits, float* part_acc, float* part_ml, int* status,
-                                                   void* stream) {
+                                                   int window, int num_pages, int splits, int split_tiles, float* part_acc, float* part_ml,
+                                                   int* status, void* stream) {
   PTL_REQUIRE(splits >= 1 && splits <= 65535 && (splits == 1 || (part_acc && part_ml && ptl::aligned16(part_acc))),
               "prefill_attention_tc: splits > 1 need scratch buffers");
   const int rc = prefill_attention_tc_entry(out, q, cache, block_table, tiles, n_tiles, n_tokens, q_stride, out_stride, bt_stride, nq, nkv, d,
-                                            page_size, scale, window, num_pages, true, splits, part_acc, part_ml, status, stream);
+                                            page_size, scale, window, num_pages, true, splits, split_tiles, part_acc, part_ml, status, stream);
   if (rc || splits == 1 || n_tiles == 0) return rc;
   return ptl::attention8_join_bf16(out, part_acc, part_ml, tiles, n_tiles, out_stride, nq, d, splits, stream);
 }

@@ -299,7 +299,8 @@ read_kv8_kernel(T* __restrict__ out, const unsigned char* __restrict__ codes, co
 // mma.sync, 44 from bfloat16).  The j-th request with portions, counted in the order of the tiles (pairs of {request, first row,
 // rows, first position}, as the attention takes them), has pages j * width .. of `pages` in the order of its positions;
 // table[request] says so, -1 where it has no page.  Page slots * width is zeros.  A marked token's key is NaN and its value
-// the finite part, so that it reaches the rows that see it and no other.  One block of threads a page and pair; a request's first pair works.
+// the finite part, so that it reaches the rows that see it and no other.  Blocks of threads a page (a thread has four
+// packets of 16 codes of it) and pair; a request's first pair works.
 struct Kv8ExpandParams {
   __nv_bfloat16* pages;
   int* table;
@@ -310,59 +311,69 @@ struct Kv8ExpandParams {
   int pairs, slots, width, bt_stride, nkv, d, page_size, num_pages, window;
 };
 
+constexpr int kKv8ExpandChunk = kKv8Threads * kKv8ReadAhead;      // packets of a page a block takes
+
 __global__ void __launch_bounds__(kKv8Threads)
 kv8_expand_kernel(const Kv8ExpandParams p) {
-  __shared__ int s_first[kKv8Threads / 32], s_end[kKv8Threads / 32];
+  // tiles and the block table are inputs of the step, not results of the kernel before this one
+  const int page_codes = 2 * p.nkv * p.page_size * p.d, lane = threadIdx.x & 31;
+  const int pair = blockIdx.y, chunk = blockIdx.z * kKv8ExpandChunk;      // of the page's packets of 16 codes
+  auto request = [&](int i) { return i >= 0 && i < p.pairs && __ldg(p.tiles + 8 * i + 2) > 0 ? __ldg(p.tiles + 8 * i) : -1; };
+  const int r = request(pair);
+  const bool works = r >= 0 && request(pair - 1) != r;
+  int before = 0, lo = 0, hi = 0;
+  if (works) {
+    // requests before this one, and the end of this one's last portion (every warp for itself)
+    int end = 0;
+    for (int i = lane; i < p.pairs; i += 32) {
+      const int ri = request(i);
+      if (i < pair && ri >= 0 && request(i - 1) != ri) ++before;
+      if (i >= pair && ri == r) end = max(end, __ldg(p.tiles + 8 * i + 3) + __ldg(p.tiles + 8 * i + 2) + max(0, __ldg(p.tiles + 8 * i + 6)));
+    }
+    before = __reduce_add_sync(0xffffffffu, before);
+    end = __reduce_max_sync(0xffffffffu, end);
+    const int pos0 = __ldg(p.tiles + 8 * pair + 3);
+    lo = p.window > 0 && pos0 + 1 > p.window ? (pos0 + 1 - p.window) / p.page_size : 0;
+    hi = before < p.slots ? min((end + p.page_size - 1) / p.page_size, p.width) : 0;      // (there are as many slots as such requests)
+  }
+  auto page_at = [&](int b) { return b < hi && b < p.bt_stride ? __ldg(p.block_table + (size_t)r * p.bt_stride + b) : -1; };
+  int b = lo + blockIdx.x, page = page_at(b);
   pdl_wait();
   pdl_launch_dependents();
-  const int page_codes = 2 * p.nkv * p.page_size * p.d;
   if (blockIdx.x == 0 && blockIdx.y == 0)
-    for (int i = threadIdx.x; i < page_codes / 8; i += kKv8Threads)
+    for (int i = 2 * chunk + threadIdx.x; i < min(page_codes / 8, 2 * (chunk + kKv8ExpandChunk)); i += kKv8Threads)
       reinterpret_cast<uint4*>(p.pages + (size_t)p.slots * p.width * page_codes)[i] = make_uint4(0u, 0u, 0u, 0u);
-  const int pair = blockIdx.y;
-  auto request = [&](int i) { return i >= 0 && i < p.pairs && p.tiles[8 * i + 2] > 0 ? p.tiles[8 * i] : -1; };
-  const int r = request(pair);
-  if (r < 0 || request(pair - 1) == r) return;
-  // requests before this one, and the end of this one's last portion
-  int before = 0, end = 0;
-  for (int i = threadIdx.x; i < p.pairs; i += kKv8Threads) {
-    const int ri = request(i);
-    if (i < pair && ri >= 0 && request(i - 1) != ri) ++before;
-    if (i >= pair && ri == r) end = max(end, p.tiles[8 * i + 3] + p.tiles[8 * i + 2] + max(0, p.tiles[8 * i + 6]));
-  }
-  before = __reduce_add_sync(0xffffffffu, before);
-  end = __reduce_max_sync(0xffffffffu, end);
-  if (threadIdx.x % 32 == 0) { s_first[threadIdx.x / 32] = before; s_end[threadIdx.x / 32] = end; }
-  __syncthreads();
-  before = 0;
-  end = 0;
-  for (int i = 0; i < kKv8Threads / 32; ++i) { before += s_first[i]; end = max(end, s_end[i]); }
-  if (before >= p.slots) return;                       // (never: there are as many slots as such requests)
-  const int pos0 = p.tiles[8 * pair + 3];
-  const int lo = p.window > 0 && pos0 + 1 > p.window ? (pos0 + 1 - p.window) / p.page_size : 0, hi = min((end + p.page_size - 1) / p.page_size, p.width);
   const int blocks = p.page_size / kKv8Block, per_row = p.d / 16;
-  for (int b = lo + blockIdx.x; b < hi; b += gridDim.x) {
-    const int page = b < p.bt_stride ? p.block_table[(size_t)r * p.bt_stride + b] : -1, to = before * p.width + b;
+  for (; b < hi; b += gridDim.x) {
+    const int to = before * p.width + b;
     const bool here = page >= 0 && page < p.num_pages;
-    if (threadIdx.x == 0) p.table[(size_t)r * p.width + b] = here ? to : -1;
-    if (!here) continue;
-    const uint4* src = reinterpret_cast<const uint4*>(p.codes + (size_t)page * page_codes);
+    if (threadIdx.x == 0 && blockIdx.z == 0) p.table[(size_t)r * p.width + b] = here ? to : -1;
+    const uint4* src = reinterpret_cast<const uint4*>(p.codes + (size_t)(here ? page : 0) * page_codes);
     uint4* dst = reinterpret_cast<uint4*>(p.pages + (size_t)to * page_codes);
-    const uint2* words = reinterpret_cast<const uint2*>(p.words) + (size_t)page * p.nkv * blocks;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < page_codes / 16; i += kKv8Threads) {
-      const int row = i / per_row, part = row / (p.nkv * p.page_size), g = row / p.page_size - part * p.nkv, off = row % p.page_size;
-      const uint4 c = __ldg(src + i);
-      const uint2 w = __ldg(words + g * blocks + off / kKv8Block);
-      const float step = 2.0f * kv8_half_step((part ? w.y : w.x) & 255u);
-      const bool marked = part == 0 && (((w.x | w.y) >> (16 + off % kKv8Block)) & 1u);
+    const uint2* words = reinterpret_cast<const uint2*>(p.words) + (size_t)(here ? page : 0) * p.nkv * blocks;
+    uint4 c[kKv8ReadAhead];
+    uint2 w[kKv8ReadAhead];
+#pragma unroll
+    for (int k = 0; k < kKv8ReadAhead; ++k) {
+      const int i = chunk + k * kKv8Threads + threadIdx.x, row = i / per_row, g = row / p.page_size % p.nkv, off = row % p.page_size;
+      if (!here || i >= page_codes / 16) continue;
+      c[k] = __ldg(src + i);
+      w[k] = __ldg(words + g * blocks + off / kKv8Block);
+    }
+    page = page_at(b + gridDim.x);
+#pragma unroll
+    for (int k = 0; k < kKv8ReadAhead; ++k) {
+      const int i = chunk + k * kKv8Threads + threadIdx.x, row = i / per_row, part = row / (p.nkv * p.page_size), off = row % p.page_size;
+      if (!here || i >= page_codes / 16) continue;
+      const float step = 2.0f * kv8_half_step((part ? w[k].y : w[k].x) & 255u);
+      const bool marked = part == 0 && (((w[k].x | w[k].y) >> (16 + off % kKv8Block)) & 1u);
       uint32_t out[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t four = k < 2 ? c.x : k < 4 ? c.y : k < 6 ? c.z : c.w;
-        const float lo2 = (float)((four >> (16 * (k & 1))) & 255u) - 127.5f, hi2 = (float)((four >> (16 * (k & 1) + 8)) & 255u) - 127.5f;
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t four = j < 2 ? c[k].x : j < 4 ? c[k].y : j < 6 ? c[k].z : c[k].w;
+        const float lo2 = (float)((four >> (16 * (j & 1))) & 255u) - 127.5f, hi2 = (float)((four >> (16 * (j & 1) + 8)) & 255u) - 127.5f;
         const __nv_bfloat162 two = __floats2bfloat162_rn(lo2 * step, hi2 * step);
-        out[k] = marked ? 0x7fc07fc0u : *reinterpret_cast<const uint32_t*>(&two);
+        out[j] = marked ? 0x7fc07fc0u : *reinterpret_cast<const uint32_t*>(&two);
       }
       dst[2 * i] = make_uint4(out[0], out[1], out[2], out[3]);
       dst[2 * i + 1] = make_uint4(out[4], out[5], out[6], out[7]);
@@ -448,8 +459,9 @@ PTL_EXPORT int ptl_kv8_expand_bf16(void* pages, int* table, const void* codes, c
   PTL_REQUIRE(d % 16 == 0 && d > 0 && page_size % kKv8Block == 0, "kv8_expand: head size %d and pages of %d must be multiples of 16", d, page_size);
   PTL_REQUIRE(aligned16(pages) && aligned16(codes) && (reinterpret_cast<uintptr_t>(words) & 7u) == 0 && n_tiles / 2 <= 65535, "kv8_expand: alignment");
   if (n_tiles == 0) return 0;
-  const int x = width < 1024 ? width : 1024;
-  return launch_kernel("kv8_expand", kv8_expand_kernel, dim3(x, n_tiles / 2), dim3(kKv8Threads), 0, as_stream(stream),
+  const int x = width < 1024 ? width : 1024, chunks = (nkv * page_size * d / 8 + kKv8ExpandChunk - 1) / kKv8ExpandChunk;
+  PTL_REQUIRE(chunks <= 65535, "kv8_expand: pages are too large");
+  return launch_kernel("kv8_expand", kv8_expand_kernel, dim3(x, n_tiles / 2, chunks), dim3(kKv8Threads), 0, as_stream(stream),
                        Kv8ExpandParams{(__nv_bfloat16*)pages, table, (const unsigned char*)codes, (const uint32_t*)words, block_table, tiles,
                                        n_tiles / 2, slots, width, bt_stride, nkv, d, page_size, num_pages, window});
 }

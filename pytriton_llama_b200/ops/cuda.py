@@ -203,7 +203,7 @@ def load_library() -> ctypes.CDLL:
     lib.ptl_prefill_attention_tc_bf16.argtypes = [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                                   _c_int, _c_int, _c_int, _c_f, _c_int, _c_int, _ptr, _ptr]
     lib.ptl_prefill_attention_tc_bf16.restype = _c_int
-    lib.ptl_prefill_attention_tc_holes_bf16.argtypes = lib.ptl_prefill_attention_tc_bf16.argtypes[:-2] + [_c_int, _ptr, _ptr, _ptr, _ptr]
+    lib.ptl_prefill_attention_tc_holes_bf16.argtypes = lib.ptl_prefill_attention_tc_bf16.argtypes[:-2] + [_c_int, _c_int, _ptr, _ptr, _ptr, _ptr]
     lib.ptl_prefill_attention_tc_holes_bf16.restype = _c_int
     lib.ptl_kv8_expand_bf16.argtypes = [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr]
     lib.ptl_kv8_expand_bf16.restype = _c_int
@@ -1003,7 +1003,7 @@ class CudaOps:
         dec, tiles = self._work(hints, "decode_items"), self._work(hints, "prefill_tiles")
         if d in (64, 128) and nq // nkv <= 16 and dec is not None and tiles is not None and q.shape[1] % 8 == 0:
             if self._attention8_tensor_cores(out, q, codes, words, block_table, tok_req, positions, nq, nkv, d, page_size, float(scale),
-                                             int(window), longest, dec, tiles, getattr(hints, "split_portions", None), getattr(hints, "single_form", None)):
+                                             int(window), longest, dec, tiles, hints):
                 return out
         # blocks of 128 keys' turns: split until they fill the machine a few times
         splits = max(1, min(-(-longest // 256), 148 * 8 // max(1, tokens * nq), 64))
@@ -1055,8 +1055,10 @@ class CudaOps:
         return best[1], best[2]
 
     def _attention8_tensor_cores(self, out, q, codes, words, block_table, tok_req, positions, nq, nkv, d, page_size, scale, window, longest,
-                                 dec, tiles, split_portions=None, force=None) -> bool:
-        """Single tokens and portions by the tensor-core kernels; False where they do not take the sizes (nothing has run then)."""
+                                 dec, tiles, hints) -> bool:
+        """Single tokens and portions by the tensor-core kernels; False where they do not take the sizes (nothing has run then).  ``hints`` may
+        name the form of single tokens, ``single_form``, and of portions, ``split_portions``."""
+        force, split_portions = getattr(hints, "single_form", None), getattr(hints, "split_portions", None)
         stream, n, suffix = self._stream(), dec.items, _suffix(q.dtype)
         if tiles.items > 65535:
             return False
@@ -1089,7 +1091,7 @@ class CudaOps:
             rows = (q.shape[0] - n) / (tiles.items // 2)             # of a pair of tiles, on average
             few = longest <= 192 or (rows <= 32 and longest >= 3000) if split_portions is None else bool(split_portions)
             if q.dtype == torch.bfloat16 and not few and self._attention8_portions(out, q, codes, words, block_table, nq, nkv, d, page_size, scale,
-                                                                                   window, longest, tiles, stream):
+                                                                                   window, longest, tiles, hints, stream):
                 return True
             splits, part_acc, part_ml = 1, None, None
             if few or q.dtype == torch.float32:
@@ -1108,7 +1110,7 @@ class CudaOps:
 
     KV8_EXPAND_BYTES = 1 << 30       # of pages made bfloat16 for one call, at most
 
-    def _attention8_portions(self, out, q, codes, words, block_table, nq, nkv, d, page_size, scale, window, longest, tiles, stream) -> bool:
+    def _attention8_portions(self, out, q, codes, words, block_table, nq, nkv, d, page_size, scale, window, longest, tiles, hints, stream) -> bool:
         """bfloat16 portions on the fifth-generation tensor cores, over the pages they see made bfloat16 first; False where they are too many
         (a captured step counts its longest contexts) or of a size that those tiles do not take."""
         keys = 128 if d == 64 else 64
@@ -1119,13 +1121,10 @@ class CudaOps:
         pages = slots * width + 1
         if pages * 4 * nkv * page_size * d > self.KV8_EXPAND_BYTES:
             return False
-        # A block an SM, in rounds: a block starts and ends in about 6 us and takes 1.9 us a tile of keys with heads of 64, 1.4 with 128; with
-        # its keys split, what the parts leave is written and read at about 3 TB/s.  32 heads, one portion, us, whole and split: 131 tokens behind
-        # 6,000 (heads of 64) 108 and 42, 600 behind 30,000 485 and 357; 600 behind 1,000 37, and 50 in three parts.
-        blocks, sms, n_keys, tile_us = tiles.items // 2 * nq, self._sm_count, longest / keys, 1.9 if d == 64 else 1.4
-        most = max(1, min(16, longest // (4 * keys)))
-        splits = min(range(1, most + 1), key=lambda s: -(-blocks * s // sms) * (6 + n_keys / s * tile_us)
-                     + (5 + q.shape[0] * nq * s * (d + 2) * 8 / 3e6 if s > 1 else 0))
+        pairs = self._portion_pairs(hints, keys, page_size, window)
+        if pairs is None or len(pairs) != tiles.items // 2:      # (a captured step: as if all were the longest)
+            pairs = ((-(-(longest + page_size) // keys), 256),) * (tiles.items // 2)
+        splits, split_tiles = self._kv8_split_plan(pairs, nq, d, self._sm_count)
         part_acc = part_ml = None
         if splits > 1:
             scratch = block_table.new_empty(q.shape[0] * nq * splits * (d + 2))      # float32
@@ -1137,9 +1136,53 @@ class CudaOps:
                                                  window, stream))
         self._check(self.lib.ptl_prefill_attention_tc_holes_bf16(out.data_ptr(), q.data_ptr(), place.data_ptr(), table.data_ptr(), tiles.tensor.data_ptr(),
                                                                  tiles.items, q.shape[0], q.shape[1], nq * d, width, nq, nkv, d, page_size, scale,
-                                                                 window, pages, splits, part_acc, part_ml, self._tc_status_word().data_ptr(), stream),
+                                                                 window, pages, splits, split_tiles, part_acc, part_ml, self._tc_status_word().data_ptr(), stream),
                     kernels=2 if splits > 1 else 1)
         return True
+
+    def _portion_pairs(self, hints, keys: int, page_size: int, window: int):
+        """(tiles of ``keys`` keys it sees, rows) of every pair of tiles of a step whose lengths the host knows, or None."""
+        if not getattr(hints, "host_lengths_exact", False):
+            return None
+        memo = getattr(hints, "portion_pairs", None)
+        if memo is None or memo[0] != (keys, page_size, window):
+            pairs = []
+            for n, c in zip(hints.q_lens, hints.ctx_lens):
+                for a in range(0, n if n > 1 else 0, 2 * self.QUERY_TILE):
+                    first, rows = c - n + a, min(n - a, 2 * self.QUERY_TILE)
+                    lo = max(0, first + 1 - window) // page_size * page_size if window else 0
+                    pairs.append((-(-(first + rows - lo) // keys), rows))
+            memo = (keys, page_size, window), tuple(pairs)
+            hints.portion_pairs = memo
+        return memo[1]
+
+    @staticmethod
+    @functools.lru_cache(maxsize=4096)
+    def _kv8_split_plan(pairs, nq: int, d: int, sms: int):
+        """(parts that the keys of portions are cut into, tiles of keys of a part): what the tensor-memory kernel over pages made bfloat16
+        takes for pairs of (tiles of keys, rows).  An SM works on a block at a time, which starts and ends in about 6 us and takes 1.9 us a
+        tile of keys with heads of 64, 1.4 with 128; what the parts leave is written and read at about 3 TB/s.  Parts are of one length, so a short
+        context has fewer of them.  32 heads, one portion, us, whole and so: 131 tokens behind 6,000 (heads of 64) 108 and 42, 600 behind 30,000 485
+        and 357."""
+        tile = 1.9 if d == 64 else 1.4
+        longest = max(t for t, _ in pairs)
+        best = None
+        for s in range(1, max(1, min(16, longest // 4)) + 1):
+            length = -(-longest // s)
+            blocks, left = [], 0
+            for t, rows in pairs:
+                full, rest = divmod(t, length)
+                blocks += [(6 + length * tile, full * nq)] * (full > 0) + [(6 + rest * tile, nq)] * (rest > 0)
+                left += rows * nq * (full + (rest > 0)) * (d + 2) * 8
+            blocks.sort(reverse=True)
+            done, cost = 0, sum(us * k for us, k in blocks) / sms
+            for us, k in blocks:             # some SM has this many blocks of at least this length
+                done += k
+                cost = max(cost, us * -(-done // sms))
+            cost += 5 + left / 3e6 if s > 1 else 0
+            if best is None or cost < best[0]:
+                best = (cost, s, length)
+        return best[1:]
 
     def _decode8_unit_list(self, dec, tok_req, positions, rows: int, nq: int, nkv: int, d: int, window: int, per_head: int):
         """The units of the step's single tokens, 8 integers each, and behind them a counter per (row, kv head), zero: as ``_decode_unit_list``, but
