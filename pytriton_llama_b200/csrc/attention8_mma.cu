@@ -784,32 +784,57 @@ attention8_portion_kernel(const A8Params p) {
     }
 }
 
-// The splits of portions joined: a warp a row of the tiles and query head.
+// The splits of portions joined: D / 4 lanes a row of the tiles and query head, four dimensions each.
+constexpr int kA8JoinThreads = 256;
 template <int D, typename T>
-__global__ void __launch_bounds__(kA8Warps * 32)
+__global__ void __launch_bounds__(kA8JoinThreads)
 attention8_join_kernel(const A8Params p) {
+  const int* tl = p.items + 4 * blockIdx.y;
+  const int first = __ldg(tl + 1), rows = __ldg(tl + 2);       // (inputs of the step)
   pdl_wait();
   pdl_launch_dependents();
-  const int* tl = p.items + 4 * blockIdx.y;
-  const int i = blockIdx.x * kA8Warps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (i / p.nq >= tl[2]) return;
-  const size_t row = (size_t)(tl[1] + i / p.nq), at = (row * p.nq + i % p.nq) * p.splits;
-  float M = -INFINITY, L = 0.f, acc[D / 32];
+  const int i = blockIdx.x * (kA8JoinThreads / (D / 4)) + threadIdx.x / (D / 4), col = threadIdx.x % (D / 4) * 4;
+  if (i / p.nq >= rows) return;
+  const size_t row = (size_t)(first + i / p.nq), at = (row * p.nq + i % p.nq) * p.splits;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + at;
+  const float4* part = reinterpret_cast<const float4*>(p.part_acc + at * D + col);
+  constexpr int kAhead = 4;
+  float M = -INFINITY, L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int z0 = 0; z0 < p.splits; z0 += kAhead) {              // kAhead parts are asked for at once; those without keys hold nothing
+    float2 s[kAhead];
+    float4 a[kAhead];
+    float top = M;
 #pragma unroll
-  for (int k = 0; k < D / 32; ++k) acc[k] = 0.f;
-  for (int z = 0; z < p.splits; ++z) M = fmaxf(M, __ldg(p.part_ml + 2 * (at + z)));
-#pragma unroll 4
-  for (int z = 0; z < p.splits; ++z) {
-    const float m = __ldg(p.part_ml + 2 * (at + z)), l = __ldg(p.part_ml + 2 * (at + z) + 1), f = a8_weight(m, l, M);
-    if (l == 0.f) continue;
-    L = fmaf(f, l, L);
+    for (int z = 0; z < kAhead; ++z) {
+      s[z] = z0 + z < p.splits ? __ldg(ml + z0 + z) : make_float2(-INFINITY, 0.f);
+      a[z] = z0 + z < p.splits ? __ldg(part + (size_t)(z0 + z) * (D / 4)) : acc;
+      top = fmaxf(top, s[z].x);
+    }
+    const float before = a8_weight(M, L, top);
+    M = top;
+    L *= before;
+    acc.x *= before; acc.y *= before; acc.z *= before; acc.w *= before;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) acc[k] = fmaf(f, __ldg(p.part_acc + (at + z) * D + k * 32 + lane), acc[k]);
+    for (int z = 0; z < kAhead; ++z) {
+      if (s[z].y == 0.f) continue;
+      const float f = a8_weight(s[z].x, s[z].y, top);
+      L = fmaf(f, s[z].y, L);
+      acc.x = fmaf(f, a[z].x, acc.x); acc.y = fmaf(f, a[z].y, acc.y); acc.z = fmaf(f, a[z].z, acc.z); acc.w = fmaf(f, a[z].w, acc.w);
+    }
   }
   const float inv = a8_inverse(L);
-  T* dst = static_cast<T*>(p.out) + row * p.out_stride + (size_t)(i % p.nq) * D + lane;
-#pragma unroll
-  for (int k = 0; k < D / 32; ++k) dst[k * 32] = from_f32<T>(acc[k] * inv);
+  T* dst = static_cast<T*>(p.out) + row * p.out_stride + (size_t)(i % p.nq) * D + col;
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  } else {
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  }
+}
+template <int D, typename T> static int launch_a8_join(const A8Params& p, int tiles, cudaStream_t stream) {
+  constexpr int kPer = kA8JoinThreads / (D / 4);
+  return launch_kernel("attention8_join", attention8_join_kernel<D, T>, dim3((128 * p.nq + kPer - 1) / kPer, tiles), dim3(kA8JoinThreads), 0, stream, p);
 }
 
 int attention8_join_bf16(void* out, const float* part_acc, const float* part_ml, const int* tiles, int n_tiles, int out_stride, int nq, int d, int splits,
@@ -817,8 +842,7 @@ int attention8_join_bf16(void* out, const float* part_acc, const float* part_ml,
   A8Params p{};
   p.out = out; p.part_acc = const_cast<float*>(part_acc); p.part_ml = const_cast<float*>(part_ml); p.items = tiles;
   p.out_stride = out_stride; p.nq = nq; p.splits = splits;
-  return launch_kernel("attention8_join", d == 64 ? attention8_join_kernel<64, __nv_bfloat16> : attention8_join_kernel<128, __nv_bfloat16>,
-                       dim3((128 * nq + kA8Warps - 1) / kA8Warps, n_tiles), dim3(kA8Warps * 32), 0, as_stream(stream), p);
+  return d == 64 ? launch_a8_join<64, __nv_bfloat16>(p, n_tiles, as_stream(stream)) : launch_a8_join<128, __nv_bfloat16>(p, n_tiles, as_stream(stream));
 }
 
 // The units that a step's single tokens are dealt out in: see decode_units_kernel (attention_decode.cu), whose list this is.  c is
@@ -906,7 +930,7 @@ static int launch_attention8(const A8Params& p, int singles, int tiles, int per_
   if (int rc = launch_kernel("attention8_portion", attention8_portion_kernel<D, T>, dim3(p.nkv * ((128 + per_block - 1) / per_block), tiles, p.splits),
                              dim3(kA8Warps * 32), Cfg::kSmem, stream, p)) return rc;
   if (p.splits == 1) return 0;
-  return launch_kernel("attention8_join", attention8_join_kernel<D, T>, dim3((128 * p.nq + kA8Warps - 1) / kA8Warps, tiles), dim3(kA8Warps * 32), 0, stream, p);
+  return launch_a8_join<D, T>(p, tiles, stream);
 }
 
 template <typename T>

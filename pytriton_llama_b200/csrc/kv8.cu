@@ -240,18 +240,17 @@ rope_kv8_write_kernel(const Kv8WriteParams p) {
 
 // Keys and values of the first length[r] tokens of the requests as numbers, request after request: out [tokens][2][heads][d].  A block of
 // threads takes 16 positions of a request, which lie in one page, packets of 16 codes in the order in which they lie there.
-constexpr int kKv8ReadRequests = 960;
 constexpr int kKv8ReadAhead = 4;
-struct Kv8ReadArgs {
+template <int REQUESTS> struct Kv8ReadArgs {
   long long first_row;                     // of the output
   int requests, first_request;
-  int end[kKv8ReadRequests];               // tokens of this launch's requests up to and with each
+  int end[REQUESTS];                       // tokens of this launch's requests up to and with each
 };
 
-template <typename T>
+template <typename T, int REQUESTS>
 __global__ void __launch_bounds__(kKv8Threads)
 read_kv8_kernel(T* __restrict__ out, const unsigned char* __restrict__ codes, const uint32_t* __restrict__ words,
-                const int* __restrict__ block_table, const __grid_constant__ Kv8ReadArgs args, int bt_stride, int nkv, int d, int page_size,
+                const int* __restrict__ block_table, const __grid_constant__ Kv8ReadArgs<REQUESTS> args, int bt_stride, int nkv, int d, int page_size,
                 int num_pages) {
   const int r = blockIdx.y, pos0 = blockIdx.x * kKv8Block;
   const int t0 = r ? args.end[r - 1] : 0, tokens = min(kKv8Block, args.end[r] - t0 - pos0);
@@ -403,17 +402,14 @@ static int rope_kv8_write(T* qkv, const int* positions, const float* inv_freq, c
                        as_stream(stream), p);
 }
 
-template <typename T>
-static int read_kv8(T* out, const void* codes, const void* words, const int* block_table, const int* lengths, int requests, int bt_stride,
-                    int nkv, int d, int page_size, int num_pages, void* stream) {
-  PTL_REQUIRE(requests >= 0 && nkv > 0 && d > 0 && page_size > 0 && num_pages > 0 && bt_stride > 0, "read_kv8: bad sizes");
-  PTL_REQUIRE(d % 16 == 0 && page_size % kKv8Block == 0, "read_kv8: head size %d and pages of %d must be multiples of 16", d, page_size);
-  PTL_REQUIRE(aligned16(out) && aligned16(codes), "read_kv8: out and codes must be 16-byte aligned");
-  Kv8ReadArgs args;
+template <typename T, int REQUESTS>
+static int launch_read_kv8(T* out, const void* codes, const void* words, const int* block_table, const int* lengths, int requests, int bt_stride,
+                           int nkv, int d, int page_size, int num_pages, void* stream) {
+  Kv8ReadArgs<REQUESTS> args;
   args.first_row = 0;
-  for (int r0 = 0; r0 < requests; r0 += kKv8ReadRequests) {
+  for (int r0 = 0; r0 < requests; r0 += REQUESTS) {
     args.first_request = r0;
-    args.requests = requests - r0 < kKv8ReadRequests ? requests - r0 : kKv8ReadRequests;
+    args.requests = requests - r0 < REQUESTS ? requests - r0 : REQUESTS;
     long long sum = 0;
     int longest = 0;
     for (int i = 0; i < args.requests; ++i) {
@@ -425,13 +421,25 @@ static int read_kv8(T* out, const void* codes, const void* words, const int* blo
       args.end[i] = (int)sum;
     }
     if (sum > 0) {
-      if (int rc = launch_kernel("read_kv8", read_kv8_kernel<T>, dim3((longest + kKv8Block - 1) / kKv8Block, args.requests), dim3(kKv8Threads), 0, as_stream(stream), out,
-                                 (const unsigned char*)codes, (const uint32_t*)words, block_table, args, bt_stride, nkv, d, page_size, num_pages))
+      if (int rc = launch_kernel("read_kv8", read_kv8_kernel<T, REQUESTS>, dim3((longest + kKv8Block - 1) / kKv8Block, args.requests), dim3(kKv8Threads), 0,
+                                 as_stream(stream), out, (const unsigned char*)codes, (const uint32_t*)words, block_table, args, bt_stride, nkv, d,
+                                 page_size, num_pages))
         return rc;
     }
     args.first_row += sum;
   }
   return 0;
+}
+
+template <typename T>
+static int read_kv8(T* out, const void* codes, const void* words, const int* block_table, const int* lengths, int requests, int bt_stride,
+                    int nkv, int d, int page_size, int num_pages, void* stream) {
+  PTL_REQUIRE(requests >= 0 && nkv > 0 && d > 0 && page_size > 0 && num_pages > 0 && bt_stride > 0, "read_kv8: bad sizes");
+  PTL_REQUIRE(d % 16 == 0 && page_size % kKv8Block == 0, "read_kv8: head size %d and pages of %d must be multiples of 16", d, page_size);
+  PTL_REQUIRE(aligned16(out) && aligned16(codes), "read_kv8: out and codes must be 16-byte aligned");
+  // (the host copies the arguments of a launch, however many are used)
+  return (requests <= 64 ? launch_read_kv8<T, 64> : launch_read_kv8<T, 960>)(out, codes, words, block_table, lengths, requests, bt_stride, nkv, d, page_size,
+                                                                             num_pages, stream);
 }
 
 }  // namespace ptl

@@ -911,19 +911,24 @@ class CudaOps:
     # ------------------------------------------------------------------ keys and values in 8 bits
     KV8_BLOCK = 16         # positions that share a scale
 
-    def _want_kv8(self, codes: torch.Tensor, words: torch.Tensor, nkv: int, d: int, page_size: int) -> None:
+    def _want_kv8(self, codes: torch.Tensor, words: torch.Tensor, nkv: int, d: int, page_size: int) -> int:
+        """Looks an 8-bit cache over; its pages."""
+        device, shape = self.device, words.shape
+        if (words.dtype is torch.int32 and codes.dtype is torch.uint8 and len(shape) == 4 and shape[0] and page_size % 16 == 0 and d % 16 == 0
+                and 0 < d <= 256 and shape[1] == nkv and shape[2] * 16 == page_size and shape[3] == 2 and codes.shape[0] == shape[0]
+                and codes.numel() == shape[0] * 2 * nkv * page_size * d and codes.is_contiguous() and words.is_contiguous() and codes.device == device
+                and words.device == device):
+            return shape[0]
         self._want_all(torch.uint8, codes=codes)
         self._want_all(torch.int32, words=words)
         if page_size % self.KV8_BLOCK:
             raise KernelError(f"8-bit cache: pages of {page_size} positions are no whole blocks of {self.KV8_BLOCK}")
         if d % 16 or d <= 0 or d > 256:
             raise KernelError(f"8-bit cache: head size {d} is no multiple of 16 up to 256")
-        shape = codes.shape
-        pages = shape[0] if shape else 0
+        pages = codes.shape[0] if codes.dim() else 0
         if not pages or codes.numel() != pages * 2 * nkv * page_size * d:
-            raise KernelError(f"8-bit cache: pages of {tuple(shape)} do not fit {nkv} heads of {d} and {page_size} positions")
-        if words.shape != (pages, nkv, page_size // self.KV8_BLOCK, 2):
-            raise KernelError(f"8-bit cache: words {tuple(words.shape)}, expected {(codes.shape[0], nkv, page_size // self.KV8_BLOCK, 2)}")
+            raise KernelError(f"8-bit cache: pages of {tuple(codes.shape)} do not fit {nkv} heads of {d} and {page_size} positions")
+        raise KernelError(f"8-bit cache: words {tuple(shape)}, expected {(pages, nkv, page_size // self.KV8_BLOCK, 2)}")
 
     def rope_kv8_write(self, qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optional[torch.Tensor], rot: int,
                        slots: torch.Tensor, codes: torch.Tensor, words: torch.Tensor, nq: int, nkv: int, d: int, page_size: int) -> None:
@@ -939,33 +944,35 @@ class CudaOps:
         negative or behind the pool write nothing."""
         self._want(qkv, "qkv")
         self._want_all(torch.int32, positions=positions, slots=slots)
-        self._want_kv8(codes, words, nkv, d, page_size)
-        if qkv.dim() != 2 or qkv.shape[1] != (nq + 2 * nkv) * d:
-            raise KernelError(f"qkv is {tuple(qkv.shape)}, expected rows of {(nq + 2 * nkv) * d} elements")
-        if positions.numel() < qkv.shape[0] or slots.numel() < qkv.shape[0]:
+        pages, shape = self._want_kv8(codes, words, nkv, d, page_size), qkv.shape
+        if len(shape) != 2 or shape[1] != (nq + 2 * nkv) * d:
+            raise KernelError(f"qkv is {tuple(shape)}, expected rows of {(nq + 2 * nkv) * d} elements")
+        rows = shape[0]
+        if positions.numel() < rows or slots.numel() < rows:
             raise KernelError("rope_kv8_write: fewer positions or slots than rows")
         if inv_freq is not None:
             self._want(inv_freq, "inv_freq", torch.float32)
             if inv_freq.numel() < rot // 2:
                 raise KernelError("inv_freq shorter than half the rotary width")
         fn = getattr(self.lib, "ptl_rope_kv8_write" + _suffix(qkv.dtype))
-        self._check(fn(_p(qkv), _p(positions), _p(inv_freq), _p(slots), _p(codes), _p(words), qkv.shape[0], nq, nkv, d, rot, page_size,
-                       codes.shape[0] * page_size, self._stream()), kernels=1 if qkv.shape[0] else 0)
+        self._check(fn(qkv.data_ptr(), positions.data_ptr(), _p(inv_freq), slots.data_ptr(), codes.data_ptr(), words.data_ptr(), rows, nq, nkv, d, rot,
+                       page_size, pages * page_size, self._stream()), kernels=1 if rows else 0)
 
     def read_kv8(self, codes: torch.Tensor, words: torch.Tensor, block_table: torch.Tensor, contexts, dtype: torch.dtype) -> torch.Tensor:
         """What an 8-bit cache holds of the first ``contexts[r]`` (host integers) positions of the requests in the table's rows,
         request after request: [tokens, 2 (k, v), nkv, d].  bfloat16 holds every value exactly.  A marked token reads as NaN, a
         position without a page as 0."""
-        if codes.dim() != 5:
-            raise KernelError(f"codes are {tuple(codes.shape)}, expected [pages, 2, heads, positions, d]")
-        pages, _, nkv, page_size, d = codes.shape
+        shape = codes.shape
+        if len(shape) != 5:
+            raise KernelError(f"codes are {tuple(shape)}, expected [pages, 2, heads, positions, d]")
+        pages, _, nkv, page_size, d = shape
         self._want_kv8(codes, words, nkv, d, page_size)
         self._want(block_table, "block_table", torch.int32)
         contexts = contexts if isinstance(contexts, list) else np.asarray(contexts, dtype=np.int64).reshape(-1).tolist()
-        n = len(contexts)
-        if block_table.dim() != 2 or n > block_table.shape[0]:
-            raise KernelError(f"read_kv8: {n} requests, the table has {tuple(block_table.shape)} entries")
-        width = block_table.shape[1]
+        n, shape = len(contexts), block_table.shape
+        if len(shape) != 2 or n > shape[0]:
+            raise KernelError(f"read_kv8: {n} requests, the table has {tuple(shape)} entries")
+        width = shape[1]
         if n and (min(contexts) < 0 or max(contexts) > width * page_size):
             raise KernelError(f"read_kv8: a request of {min(contexts) if min(contexts) < 0 else max(contexts)} tokens does not fit its row of the table")
         total = sum(contexts)
@@ -985,11 +992,12 @@ class CudaOps:
         self._want(q, "q")
         self._want_kv8(codes, words, nkv, d, page_size)
         self._want_all(torch.int32, block_table=block_table, tok_req=tok_req, positions=positions)
-        if q.dim() != 2 or q.shape[1] < nq * d or nq <= 0 or nq % nkv:
-            raise KernelError(f"paged_attention8: q {tuple(q.shape)} for {nq} heads of {d} over {nkv} kv heads")
-        tokens = q.shape[0]
-        if block_table.dim() != 2:
-            raise KernelError(f"paged_attention8: the block table is {tuple(block_table.shape)}, expected a row per request")
+        shape, width = q.shape, block_table.shape
+        if len(shape) != 2 or shape[1] < nq * d or nq <= 0 or nq % nkv:
+            raise KernelError(f"paged_attention8: q {tuple(shape)} for {nq} heads of {d} over {nkv} kv heads")
+        tokens = shape[0]
+        if len(width) != 2:
+            raise KernelError(f"paged_attention8: the block table is {tuple(width)}, expected a row per request")
         if tok_req.numel() < tokens or positions.numel() < tokens:
             raise KernelError("paged_attention8: fewer requests or positions than rows")
         if window < 0:
@@ -997,11 +1005,11 @@ class CudaOps:
         if not 0 <= scale < math.inf:
             raise KernelError(f"paged_attention8: scores times {scale}")
         out = q.new_empty((tokens, nq * d))
-        longest = getattr(hints, "max_ctx_len", 0) or block_table.shape[1] * page_size
+        longest = getattr(hints, "max_ctx_len", 0) or width[1] * page_size
         if window:
             longest = min(longest, window)
         dec, tiles = self._work(hints, "decode_items"), self._work(hints, "prefill_tiles")
-        if d in (64, 128) and nq // nkv <= 16 and dec is not None and tiles is not None and q.shape[1] % 8 == 0:
+        if (d == 64 or d == 128) and nq // nkv <= 16 and dec is not None and tiles is not None and shape[1] % 8 == 0:
             if self._attention8_tensor_cores(out, q, codes, words, block_table, tok_req, positions, nq, nkv, d, page_size, float(scale),
                                              int(window), longest, dec, tiles, hints):
                 return out
@@ -1217,29 +1225,43 @@ class CudaOps:
             raise KernelError(f"copy_pages: {n} rows to read, {len(dst)} to write")
         if not n or not tensors:
             return
-        written = set(dst)
-        if len(written) != n:
-            raise KernelError("copy_pages: a row is written twice")
-        if not written.isdisjoint(src):
-            raise KernelError("copy_pages: a row that is read is written too")
-        low, high = min(min(src), min(dst)), max(max(src), max(dst))
+        try:
+            rows = array("i", src), array("i", dst)
+        except OverflowError:
+            raise KernelError(f"copy_pages: rows {min(*src, *dst)}..{max(*src, *dst)} of a tensor") from None
+        read, written = src, dst
+        if n > 64:                                           # (many: looked over by numpy)
+            read, written = (np.frombuffer(r, np.int32) for r in rows)
+            low, high = int(min(read.min(), written.min())), int(max(read.max(), written.max()))
+        else:
+            low, high = min(min(src), min(dst)), max(max(src), max(dst))
         device, held = self.device, []
         for t in tensors:
             if not t.is_contiguous() or t.device != device:
                 self._want(t, "a tensor of pages")
             shape = t.shape
-            if low < 0 or not shape or high >= shape[0] or high > 0x7fffffff:
+            if low < 0 or not shape or high >= shape[0]:
                 raise KernelError(f"copy_pages: rows {low}..{high} of a tensor {tuple(shape)}")
             size = t.nbytes
             if size:
                 held.append((t.data_ptr(), size, size // shape[0]))
+        if n > 64:
+            mark = np.zeros(high + 1, dtype=bool)
+            mark[written] = True
+            twice, both = np.count_nonzero(mark) != n, mark[read].any()
+        else:
+            of = set(dst)
+            twice, both = len(of) != n, not of.isdisjoint(src)
+        if twice:
+            raise KernelError("copy_pages: a row is written twice")
+        if both:
+            raise KernelError("copy_pages: a row that is read is written too")
         end = 0
         for at, size, _ in sorted(held):
             if at < end:
                 raise KernelError("copy_pages: two tensors share memory")
             end = at + size
         base, row = array("Q", [x[0] for x in held]), array("q", [x[2] for x in held])
-        rows = array("i", src), array("i", dst)
         launches = _c_int(0)
         self._check(self.lib.ptl_copy_pages(base.buffer_info()[0], row.buffer_info()[0], len(held), rows[0].buffer_info()[0], rows[1].buffer_info()[0],
                                             n, ctypes.byref(launches), self._stream()), kernels=0)
