@@ -1239,10 +1239,9 @@ class CudaOps:
         for t in tensors:
             if not t.is_contiguous() or t.device != device:
                 self._want(t, "a tensor of pages")
-            shape = t.shape
+            shape, size = t.shape, t.nbytes
             if low < 0 or not shape or high >= shape[0]:
                 raise KernelError(f"copy_pages: rows {low}..{high} of a tensor {tuple(shape)}")
-            size = t.nbytes
             if size:
                 held.append((t.data_ptr(), size, size // shape[0]))
         if n > 64:
@@ -1256,12 +1255,13 @@ class CudaOps:
             raise KernelError("copy_pages: a row is written twice")
         if both:
             raise KernelError("copy_pages: a row that is read is written too")
-        end = 0
-        for at, size, _ in sorted(held):
-            if at < end:
-                raise KernelError("copy_pages: two tensors share memory")
-            end = at + size
-        base, row = array("Q", [x[0] for x in held]), array("q", [x[2] for x in held])
+        if not held:
+            return
+        held.sort()
+        base, size, row = zip(*held)
+        if any(at + n_bytes > after for at, n_bytes, after in zip(base, size, base[1:])):
+            raise KernelError("copy_pages: two tensors share memory")
+        base, row = array("Q", base), array("q", row)
         launches = _c_int(0)
         self._check(self.lib.ptl_copy_pages(base.buffer_info()[0], row.buffer_info()[0], len(held), rows[0].buffer_info()[0], rows[1].buffer_info()[0],
                                             n, ctypes.byref(launches), self._stream()), kernels=0)
