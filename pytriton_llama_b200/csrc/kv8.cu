@@ -64,7 +64,7 @@ __device__ __forceinline__ void kv8_turn(const Kv8WriteParams& p, float (&x)[Vec
 
 // D: the head size, or 0 for any (then the values are read twice).  TURN: there are frequencies.
 template <typename T, int D, bool TURN>
-__global__ void __launch_bounds__(kKv8WriteThreads)
+__global__ void __launch_bounds__(kKv8WriteThreads, 5)
 rope_kv8_write_kernel(const Kv8WriteParams p) {
   extern __shared__ float cs[];                  // [rows staged][cos[half], sin[half]]
   constexpr int N = Vec16<T>::N;
@@ -239,7 +239,7 @@ rope_kv8_write_kernel(const Kv8WriteParams p) {
 }
 
 // Keys and values of the first length[r] tokens of the requests as numbers, request after request: out [tokens][2][heads][d].  A block of
-// threads takes 16 positions of a request, which lie in one page, packets of 16 codes in the order in which they lie there.
+// threads takes packets of 16 codes, four a thread, of 16 positions of a request, which lie in one page, in the order in which they lie there.
 constexpr int kKv8ReadAhead = 4;
 template <int REQUESTS> struct Kv8ReadArgs {
   long long first_row;                     // of the output
@@ -255,15 +255,16 @@ read_kv8_kernel(T* __restrict__ out, const unsigned char* __restrict__ codes, co
   const int r = blockIdx.y, pos0 = blockIdx.x * kKv8Block;
   const int t0 = r ? args.end[r - 1] : 0, tokens = min(kKv8Block, args.end[r] - t0 - pos0);
   if (tokens <= 0) return;
+  // (the table is an input, not a result of the kernel before this one)
+  const int page = __ldg(block_table + (size_t)(args.first_request + r) * bt_stride + pos0 / page_size), sub = pos0 % page_size / kKv8Block;
   pdl_wait();
   pdl_launch_dependents();
-  const int page = __ldg(block_table + (size_t)(args.first_request + r) * bt_stride + pos0 / page_size), sub = pos0 % page_size / kKv8Block;
   const bool here = page >= 0 && page < num_pages;           // (a position that has no page reads as 0)
   const unsigned per_row = d / 16, total = 2u * nkv * d;     // packets of a row, and of the 16 positions
   const unsigned char* src = codes + (size_t)(here ? page : 0) * 2 * nkv * page_size * d + (size_t)sub * kKv8Block * d;
   const uint32_t* word0 = words + (size_t)(here ? page : 0) * nkv * (page_size / kKv8Block) * 2 + sub * 2;
   T* dst0 = out + (args.first_row + t0 + pos0) * 2 * nkv * d;
-  for (unsigned x0 = threadIdx.x; x0 < total; x0 += kKv8Threads * kKv8ReadAhead) {
+  for (unsigned x0 = blockIdx.z * kKv8Threads * kKv8ReadAhead + threadIdx.x; x0 < total; x0 += gridDim.z * kKv8Threads * kKv8ReadAhead) {
     uint4 c[kKv8ReadAhead];
     uint32_t w[kKv8ReadAhead];
 #pragma unroll
@@ -421,7 +422,9 @@ static int launch_read_kv8(T* out, const void* codes, const void* words, const i
       args.end[i] = (int)sum;
     }
     if (sum > 0) {
-      if (int rc = launch_kernel("read_kv8", read_kv8_kernel<T, REQUESTS>, dim3((longest + kKv8Block - 1) / kKv8Block, args.requests), dim3(kKv8Threads), 0,
+      const int chunks = (2 * nkv * d + kKv8Threads * kKv8ReadAhead - 1) / (kKv8Threads * kKv8ReadAhead);
+      if (int rc = launch_kernel("read_kv8", read_kv8_kernel<T, REQUESTS>,
+                                 dim3((longest + kKv8Block - 1) / kKv8Block, args.requests, chunks < 64 ? chunks : 64), dim3(kKv8Threads), 0,
                                  as_stream(stream), out, (const unsigned char*)codes, (const uint32_t*)words, block_table, args, bt_stride, nkv, d,
                                  page_size, num_pages))
         return rc;
