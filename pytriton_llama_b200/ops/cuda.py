@@ -942,8 +942,11 @@ class CudaOps:
         has to, and the codes that are there go by it: what is held does not depend on the steps that the tokens came in.
         Rows of the same 16 positions stand next to each other, no slot twice (a request's tokens do); rows with a slot that is
         negative or behind the pool write nothing."""
-        self._want(qkv, "qkv")
-        self._want_all(torch.int32, positions=positions, slots=slots)
+        device, i32 = self.device, torch.int32
+        if not (qkv.is_contiguous() and qkv.device == device and positions.dtype is i32 and positions.is_contiguous() and positions.device == device
+                and slots.dtype is i32 and slots.is_contiguous() and slots.device == device):
+            self._want(qkv, "qkv")
+            self._want_all(i32, positions=positions, slots=slots)
         pages, shape = self._want_kv8(codes, words, nkv, d, page_size), qkv.shape
         if len(shape) != 2 or shape[1] != (nq + 2 * nkv) * d:
             raise KernelError(f"qkv is {tuple(shape)}, expected rows of {(nq + 2 * nkv) * d} elements")
@@ -977,7 +980,7 @@ class CudaOps:
             raise KernelError(f"read_kv8: a request of {min(contexts) if min(contexts) < 0 else max(contexts)} tokens does not fit its row of the table")
         total = sum(contexts)
         lengths = array("i", contexts)
-        out = self.empty((total, 2, nkv, d), dtype)
+        out = torch.empty(total, 2, nkv, d, dtype=dtype, device=self.device)
         fn = getattr(self.lib, "ptl_read_kv8" + _suffix(dtype))
         self._check(fn(out.data_ptr(), codes.data_ptr(), words.data_ptr(), block_table.data_ptr(), lengths.buffer_info()[0], n, width, nkv, d,
                        page_size, pages, self._stream()), kernels=1 if total else 0)
@@ -989,9 +992,13 @@ class CudaOps:
         """``paged_attention`` over an 8-bit cache (``rope_kv8_write``).  q is [T, >= nq*d] (the q part of a qkv buffer is fine);
         returns [T, nq*d].  A token that was written with a number that is not finite gives NaN to the rows that see it and
         to no other; a position without a page is not seen; a row without a request or without keys is zeros."""
-        self._want(q, "q")
-        self._want_kv8(codes, words, nkv, d, page_size)
-        self._want_all(torch.int32, block_table=block_table, tok_req=tok_req, positions=positions)
+        device, i32 = self.device, torch.int32
+        if not (q.is_contiguous() and q.device == device and block_table.dtype is i32 and block_table.is_contiguous() and block_table.device == device
+                and tok_req.dtype is i32 and tok_req.is_contiguous() and tok_req.device == device and positions.dtype is i32
+                and positions.is_contiguous() and positions.device == device):
+            self._want(q, "q")
+            self._want_all(i32, block_table=block_table, tok_req=tok_req, positions=positions)
+        pages = self._want_kv8(codes, words, nkv, d, page_size)
         shape, width = q.shape, block_table.shape
         if len(shape) != 2 or shape[1] < nq * d or nq <= 0 or nq % nkv:
             raise KernelError(f"paged_attention8: q {tuple(shape)} for {nq} heads of {d} over {nkv} kv heads")
@@ -1004,14 +1011,16 @@ class CudaOps:
             raise KernelError(f"paged_attention8: a window of {window} positions")
         if not 0 <= scale < math.inf:
             raise KernelError(f"paged_attention8: scores times {scale}")
-        out = q.new_empty((tokens, nq * d))
+        out = q.new_empty(tokens, nq * d)                    # (numbers take the host half the time that a tuple does)
         longest = getattr(hints, "max_ctx_len", 0) or width[1] * page_size
         if window:
             longest = min(longest, window)
-        dec, tiles = self._work(hints, "decode_items"), self._work(hints, "prefill_tiles")
-        if (d == 64 or d == 128) and nq // nkv <= 16 and dec is not None and tiles is not None and shape[1] % 8 == 0:
-            if self._attention8_tensor_cores(out, q, codes, words, block_table, tok_req, positions, nq, nkv, d, page_size, float(scale),
-                                             int(window), longest, dec, tiles, hints):
+        work = getattr(hints, "work", None)
+        if work and (d == 64 or d == 128) and nq // nkv <= 16 and shape[1] % 8 == 0:
+            dec, tiles = work.get("decode_items"), work.get("prefill_tiles")
+            if dec is not None and tiles is not None and self._attention8_tensor_cores(
+                    out, q, shape[1], codes, words, pages, block_table, width[1], tok_req, positions, nq, nkv, d, page_size, float(scale), int(window),
+                    longest, dec, tiles, hints):
                 return out
         # blocks of 128 keys' turns: split until they fill the machine a few times
         splits = max(1, min(-(-longest // 256), 148 * 8 // max(1, tokens * nq), 64))
@@ -1062,8 +1071,8 @@ class CudaOps:
             return 0, 4
         return best[1], best[2]
 
-    def _attention8_tensor_cores(self, out, q, codes, words, block_table, tok_req, positions, nq, nkv, d, page_size, scale, window, longest,
-                                 dec, tiles, hints) -> bool:
+    def _attention8_tensor_cores(self, out, q, stride, codes, words, pages, block_table, width, tok_req, positions, nq, nkv, d, page_size, scale, window,
+                                 longest, dec, tiles, hints) -> bool:
         """Single tokens and portions by the tensor-core kernels; False where they do not take the sizes (nothing has run then).  ``hints`` may
         name the form of single tokens, ``single_form``, and of portions, ``split_portions``."""
         force, split_portions = getattr(hints, "single_form", None), getattr(hints, "split_portions", None)
@@ -1074,9 +1083,10 @@ class CudaOps:
             pairs = n * nkv
             group = nq // nkv
             per_head, units, counters, part_acc, part_ml = 0, None, None, None, None
-            parts, warps = force or self._kv8_single_form(n, nkv, -(-longest // 256), d, q.dtype == torch.float32, group > 8)
+            f32 = q.dtype is torch.float32
+            parts, warps = force or self._kv8_single_form(n, nkv, -(-longest // 256), d, f32, group > 8)
             if not parts:
-                per_head = max(self._kv8_fit(d, q.dtype == torch.float32, group > 8) // nkv, n)
+                per_head = max(self._kv8_fit(d, f32, group > 8) // nkv, n)
                 units = self._decode8_unit_list(dec, tok_req, positions, q.shape[0], nq, nkv, d, window, per_head)
                 per_head = per_head if units is not None else 0
                 parts, warps = 1, 4
@@ -1087,8 +1097,9 @@ class CudaOps:
                 counters = units.data_ptr() + nkv * per_head * 32
             rc = getattr(self.lib, "ptl_attention8_single" + suffix)(
                 out.data_ptr(), part_acc, part_ml, q.data_ptr(), codes.data_ptr(), words.data_ptr(), block_table.data_ptr(),
-                None if dec.in_order else dec.tensor.data_ptr(), tok_req.data_ptr(), positions.data_ptr(), n, q.shape[1], nq * d,
-                block_table.shape[1], nq, nkv, d, page_size, scale, window, parts, warps, per_head, _p(units), counters, codes.shape[0], _p(self._tc_status_word()), stream)
+                None if dec.in_order else dec.tensor.data_ptr(), tok_req.data_ptr(), positions.data_ptr(), n, stride, nq * d,
+                width, nq, nkv, d, page_size, scale, window, parts, warps, per_head, None if units is None else units.data_ptr(), counters, pages,
+                self._tc_status_word().data_ptr(), stream)
             if rc == -2:
                 return False
             self._check(rc)
@@ -2748,19 +2759,22 @@ class CudaOps:
         ``top`` most likely tokens [rows, k] and the tokens, int32 [rows, k]), k = min(top, vocabulary), best first, of
         equal logits the lowest index first; ``top`` up to 32.  A token outside the vocabulary has -inf.  A row without a
         distribution (a NaN, +inf, or -inf only) has NaN log-probabilities and entropy; its alternatives are the largest logits, NaN last."""
-        self._want_all(torch.float32, logits=logits)
-        self._want_all(torch.int32, tokens=tokens)
-        if logits.dim() != 2 or logits.shape[1] == 0:
-            raise KernelError(f"token_scores: logits are {tuple(logits.shape)}, expected [rows, vocabulary]")
-        rows, vocab = logits.shape
+        device, shape = self.device, logits.shape
+        if not (logits.dtype is torch.float32 and logits.is_contiguous() and logits.device == device and tokens.dtype is torch.int32
+                and tokens.is_contiguous() and tokens.device == device):
+            self._want_all(torch.float32, logits=logits)
+            self._want_all(torch.int32, tokens=tokens)
+        if len(shape) != 2 or shape[1] == 0:
+            raise KernelError(f"token_scores: logits are {tuple(shape)}, expected [rows, vocabulary]")
+        rows, vocab = shape
         if tokens.numel() != rows:
             raise KernelError(f"token_scores: {tokens.numel()} tokens for {rows} rows")
         if not 0 <= top <= self.SCORES_MAX_TOP:
             raise KernelError(f"token_scores: {top} alternatives, at most {self.SCORES_MAX_TOP}")
         k = min(int(top), vocab)
-        logprob = logits.new_empty(rows)                     # (half the host's time of torch.empty with a type and a device)
+        logprob = logits.new_empty(rows)                     # (half the host's time of torch.empty with a type and a device, or a tuple of sizes)
         entropy = torch.empty_like(logprob)
-        best, ids = logits.new_empty((rows, k)), tokens.new_empty((rows, k))
+        best, ids = logits.new_empty(rows, k), tokens.new_empty(rows, k)
         self._check(self.lib.ptl_token_scores(logprob.data_ptr(), entropy.data_ptr(), best.data_ptr(), ids.data_ptr(), logits.data_ptr(),
                                               tokens.data_ptr(), rows, vocab, k, self._stream()), kernels=1 if rows else 0)
         return logprob, entropy, best, ids
