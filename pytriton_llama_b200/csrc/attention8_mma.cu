@@ -424,7 +424,12 @@ template <int D, int NT, int WARPS> struct A8Single {
 // Single tokens: the warps of a block take turns through the keys of one (token, kv head), or of a part of them, and join
 // through shared memory.  The parts of a (token, kv head) join in a cluster, or, where the contexts are cut into parts of equal
 // length (the list of attention8_units_kernel), in the block that ends last.  Every warp fetches its own keys, kRing blocks ahead.  Eight warps
-// where there are fewer blocks than SMs: half the turns.
+// halve the turns; four leave more blocks side by side (the choice and its figures: CudaOps._kv8_single_form).
+//
+// What bounds it: the instructions that make operands out of codes (two a pair of codes), and their latencies: 0.53 of the issue slots at 24 % of
+// the warps an SM holds, tensor pipe 0.11.  32 heads over 8, bfloat16: one token of 4,000 7.8 us (bytes: 0.64), 64 of 256 to 2,560 27.4
+// (14.4; 3.4 TB/s), eight of 20,011 to 30,011 with heads of 128 84 (64; 4.9 TB/s); float32, eight of 1,000 to 4,096 16.8 (3.3).  Fewer
+// registers for half as many blocks more were slower everywhere (64 tokens 33.5 us: 80 registers, spills).
 template <int D, typename T, int NT, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, NT == 1 && sizeof(T) == 2 && WARPS == 4 ? (D == 64 ? 4 : 3) : 1)
 attention8_single_kernel(const A8Params p) {
@@ -641,7 +646,9 @@ attention8_single_kernel(const A8Params p) {
 }
 
 // Portions: a warp has rows of its own, the heads of the group for as many neighbouring tokens as fit 8 NT rows; the block's warps have
-// neighbouring ones and read the same keys out of one ring of slots, a turn's kA8Turn blocks each.  The warps take turns at fetching: turn i's
+// neighbouring ones and read the same keys out of one ring of slots, a turn's kA8Turn blocks each.  For float32, and for bfloat16 where
+// the fifth-generation tensor cores do not pay (CudaOps._attention8_tensor_cores has the figures); mma.sync bounds it: a prompt of 2,048 tokens
+// takes 133 us here and 51 there.  The warps take turns at fetching: turn i's
 // one refills the slot that turn i - kLag left, which the others are through with by then (but for the slowest, which it waits for).
 template <int D, typename T> struct A8Portion {
   static constexpr int kTiles = D == 64 ? (sizeof(T) == 2 ? 4 : 2) : 2;

@@ -5,6 +5,9 @@
 // The tensors and the pairs are arguments of the launch (up to 32 KB of them), so nothing is sent to the device
 // beforehand and a captured copy holds its own.  No dst row is a src row of the same call and none comes twice, so the
 // copies have no order.  A block takes 16 KB of a row: four packets of 16 bytes a thread, all asked for before one is stored.
+//
+// What bounds it: the bytes, read and written once.  1,500 pages of 16 KB in 16 tensors: 130 us, 6.06 TB/s (a copy of the device's own kind
+// measured 6.45); one page of 32 KB to seven others in 16 tensors: 2.2 us, of which the bytes take 1.1.
 #include "common.cuh"
 
 namespace ptl {

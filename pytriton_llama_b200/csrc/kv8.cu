@@ -6,7 +6,12 @@
 // run.  One warp does a run's work for one head's k or v: it reads the values once, into registers, for the largest magnitude
 // and the marks; then, where the block's exponent grows, the codes that are there are made coarser; then come the new codes.  A run
 // that holds the block's first position starts the block anew.  A block of threads looks at one row of the step, or, in steps
-// of more rows than fill the machine, at 16, and takes the runs that begin there.
+// of many rows, at 16, and takes the runs that begin there.
+//
+// What bounds it: three loads that wait for one another (slots, then the run's values and the word, then, where the exponent grows, the codes) and
+// the launch; one rounding a code, by fma.rd.  Four prompts of 301 to 1,021 tokens (8 heads of 128) are written and read back in 15.4 us,
+// of which the bytes take 5.2; 64 single tokens in 9.5 of 1.5.  Five blocks an SM (up to 96 registers) where the compiler would take 128: 2,644
+// rows are one wave of blocks, 18.0 us otherwise.
 #include "kv8.cuh"
 
 namespace ptl {
@@ -393,8 +398,10 @@ static int rope_kv8_write(T* qkv, const int* positions, const float* inv_freq, c
   if (tokens == 0) return 0;
   if (rot == 0) inv_freq = nullptr;
   Kv8WriteParams p{qkv, positions, inv_freq, slots, (unsigned char*)codes, (uint32_t*)words, tokens, nq, nkv, d, rot, page_size, 1, num_slots};
-  // a block a row while that does not fill the machine many times over; 64 tokens of 8 heads of 64: 6.5 us by one row, 16 rows of one block 20
-  p.rows_per_block = tokens > 1024 ? kKv8Block : 1;
+  // Steps of many rows are mostly prompts, whose runs are long: a block a row asks for every row's slot many times over there.  Written and read
+  // back, us, by one row and by 16 a block: 64 single tokens (8 heads of 64) 9.5 and 25.8; one prompt (8 heads of 128) of 500 8.7 and 9.0, of
+  // 1,024 10.4 and 8.5, of 1,500 13.0 and 9.6.
+  p.rows_per_block = tokens > 512 ? kKv8Block : 1;
   const size_t smem = inv_freq ? (size_t)(p.rows_per_block + kKv8Block - 1) * rot * sizeof(float) : 0;
   auto kernel = inv_freq ? (d == 64 ? rope_kv8_write_kernel<T, 64, true> : d == 128 ? rope_kv8_write_kernel<T, 128, true> : rope_kv8_write_kernel<T, 0, true>)
                          : (d == 64 ? rope_kv8_write_kernel<T, 64, false> : d == 128 ? rope_kv8_write_kernel<T, 128, false> : rope_kv8_write_kernel<T, 0, false>);
