@@ -684,22 +684,43 @@ PTL_EXPORT int ptl_prefill_attention_tc_bf16(void* out, const void* q, const voi
 }
 
 namespace ptl {
-// defined in attention8_mma.cu
+// defined in attention8_mma.cu and kv8.cu
 int attention8_join_bf16(void* out, const float* part_acc, const float* part_ml, const int* tiles, int n_tiles, int out_stride, int nq, int d, int splits,
                          void* stream);
+int kv8_expand_bf16(void* pages, int* table, const void* codes, const void* words, const int* block_table, const int* tiles, int n_tiles, int slots,
+                    int width, int nkv, int d, int page_size, int num_pages, int window, void* stream);
 }  // namespace ptl
 
-// The same where pages may be missing (-1) in the middle of a request; the cache's last page is zeros.  splits > 1: of the keys, split_tiles tiles of
-// them each, with part_acc [n_tokens, nq, splits, d] and part_ml [n_tokens, nq, splits, 2] float32.
-PTL_EXPORT int ptl_prefill_attention_tc_holes_bf16(void* out, const void* q, const void* cache, const int* block_table,
-                                                   const int* tiles, int n_tiles, int n_tokens, int q_stride, int out_stride,
-                                                   int bt_stride, int nq, int nkv, int d, int page_size, float scale,
-                                                   int window, int num_pages, int splits, int split_tiles, float* part_acc, float* part_ml,
-                                                   int* status, void* stream) {
-  PTL_REQUIRE(splits >= 1 && splits <= 65535 && (splits == 1 || (part_acc && part_ml && ptl::aligned16(part_acc))),
+// Portions over an 8-bit cache (kv8.cuh): the pages they see are made bfloat16 in `place` [slots * width + 1, 2, nkv, page_size, d], slots at least the
+// requests with portions, with a block table of their own, `table` as `block_table` [requests, width]; then the kernel above with HOLES.  splits > 1: of the
+// keys, split_tiles tiles of them each, with part_acc [n_tokens, nq, splits, d] and part_ml [n_tokens, nq, splits, 2] float32, and a join.  The
+// arguments come packed (the host converts that many of a call's own in microseconds).
+struct Prefill8Args {
+  void* out;
+  const void* q;
+  void* place;
+  int* table;
+  const void *codes, *words;
+  const int *block_table, *tiles;
+  float *part_acc, *part_ml;
+  int* status;
+  void* stream;
+  int n_tiles, n_tokens, q_stride, out_stride, width, slots, nq, nkv, d, page_size, num_pages, window, splits, split_tiles;
+  float scale;
+  int zero;
+};
+static_assert(sizeof(Prefill8Args) == 12 * 8 + 16 * 4, "as it is packed");
+
+PTL_EXPORT int ptl_attention8_prefill_tc_bf16(const void* args) {
+  Prefill8Args a;
+  memcpy(&a, args, sizeof a);
+  PTL_REQUIRE(a.splits >= 1 && a.splits <= 65535 && (a.splits == 1 || (a.part_acc && a.part_ml && ptl::aligned16(a.part_acc))),
               "prefill_attention_tc: splits > 1 need scratch buffers");
-  const int rc = prefill_attention_tc_entry(out, q, cache, block_table, tiles, n_tiles, n_tokens, q_stride, out_stride, bt_stride, nq, nkv, d,
-                                            page_size, scale, window, num_pages, true, splits, split_tiles, part_acc, part_ml, status, stream);
-  if (rc || splits == 1 || n_tiles == 0) return rc;
-  return ptl::attention8_join_bf16(out, part_acc, part_ml, tiles, n_tiles, out_stride, nq, d, splits, stream);
+  if (int rc = ptl::kv8_expand_bf16(a.place, a.table, a.codes, a.words, a.block_table, a.tiles, a.n_tiles, a.slots, a.width, a.nkv, a.d, a.page_size,
+                                    a.num_pages, a.window, a.stream)) return rc;
+  const int rc = prefill_attention_tc_entry(a.out, a.q, a.place, a.table, a.tiles, a.n_tiles, a.n_tokens, a.q_stride, a.out_stride, a.width, a.nq, a.nkv, a.d,
+                                            a.page_size, a.scale, a.window, a.slots * a.width + 1, true, a.splits, a.split_tiles, a.part_acc, a.part_ml,
+                                            a.status, a.stream);
+  if (rc || a.splits == 1 || a.n_tiles == 0) return rc;
+  return ptl::attention8_join_bf16(a.out, a.part_acc, a.part_ml, a.tiles, a.n_tiles, a.out_stride, a.nq, a.d, a.splits, a.stream);
 }

@@ -313,7 +313,7 @@ struct Kv8ExpandParams {
   const uint32_t* words;
   const int* block_table;
   const int* tiles;
-  int pairs, slots, width, bt_stride, nkv, d, page_size, num_pages, window;
+  int pairs, slots, width, nkv, d, page_size, num_pages, window;
 };
 
 constexpr int kKv8ExpandChunk = kKv8Threads * kKv8ReadAhead;      // packets of a page a block takes
@@ -341,7 +341,7 @@ kv8_expand_kernel(const Kv8ExpandParams p) {
     lo = p.window > 0 && pos0 + 1 > p.window ? (pos0 + 1 - p.window) / p.page_size : 0;
     hi = before < p.slots ? min((end + p.page_size - 1) / p.page_size, p.width) : 0;      // (there are as many slots as such requests)
   }
-  auto page_at = [&](int b) { return b < hi && b < p.bt_stride ? __ldg(p.block_table + (size_t)r * p.bt_stride + b) : -1; };
+  auto page_at = [&](int b) { return b < hi ? __ldg(p.block_table + (size_t)r * p.width + b) : -1; };
   int b = lo + blockIdx.x, page = page_at(b);
   pdl_wait();
   pdl_launch_dependents();
@@ -452,6 +452,20 @@ static int read_kv8(T* out, const void* codes, const void* words, const int* blo
                                                                              num_pages, stream);
 }
 
+// pages: bfloat16 [slots * width + 1, 2, nkv, page_size, d]; table: int32 [requests, width]; slots: at least the requests with portions.
+int kv8_expand_bf16(void* pages, int* table, const void* codes, const void* words, const int* block_table, const int* tiles, int n_tiles, int slots,
+                    int width, int nkv, int d, int page_size, int num_pages, int window, void* stream) {
+  PTL_REQUIRE(n_tiles >= 0 && n_tiles % 2 == 0 && slots > 0 && width > 0 && nkv > 0 && page_size > 0 && num_pages > 0, "kv8_expand: bad sizes");
+  PTL_REQUIRE(d % 16 == 0 && d > 0 && page_size % kKv8Block == 0, "kv8_expand: head size %d and pages of %d must be multiples of 16", d, page_size);
+  PTL_REQUIRE(aligned16(pages) && aligned16(codes) && (reinterpret_cast<uintptr_t>(words) & 7u) == 0 && n_tiles / 2 <= 65535, "kv8_expand: alignment");
+  if (n_tiles == 0) return 0;
+  const int x = width < 1024 ? width : 1024, chunks = (nkv * page_size * d / 8 + kKv8ExpandChunk - 1) / kKv8ExpandChunk;
+  PTL_REQUIRE(chunks <= 65535, "kv8_expand: pages are too large");
+  return launch_kernel("kv8_expand", kv8_expand_kernel, dim3(x, n_tiles / 2, chunks), dim3(kKv8Threads), 0, as_stream(stream),
+                       Kv8ExpandParams{(__nv_bfloat16*)pages, table, (const unsigned char*)codes, (const uint32_t*)words, block_table, tiles,
+                                       n_tiles / 2, slots, width, nkv, d, page_size, num_pages, window});
+}
+
 }  // namespace ptl
 
 // See the top of the file.  `inv_freq` null or `rot` 0: nothing is turned.  A slot that is negative or not below num_slots is not written.
@@ -467,19 +481,3 @@ static int read_kv8(T* out, const void* codes, const void* words, const int* blo
   }
 PTL_KV8_ENTRIES(f32, float)
 PTL_KV8_ENTRIES(bf16, __nv_bfloat16)
-
-// pages: bfloat16 [slots * width + 1, 2, nkv, page_size, d]; table: int32 [requests, width]; slots: at least the requests with portions.
-PTL_EXPORT int ptl_kv8_expand_bf16(void* pages, int* table, const void* codes, const void* words, const int* block_table, const int* tiles,
-                                   int n_tiles, int slots, int width, int bt_stride, int nkv, int d, int page_size, int num_pages, int window,
-                                   void* stream) {
-  using namespace ptl;
-  PTL_REQUIRE(n_tiles >= 0 && n_tiles % 2 == 0 && slots > 0 && width > 0 && bt_stride > 0 && nkv > 0 && page_size > 0 && num_pages > 0, "kv8_expand: bad sizes");
-  PTL_REQUIRE(d % 16 == 0 && d > 0 && page_size % kKv8Block == 0, "kv8_expand: head size %d and pages of %d must be multiples of 16", d, page_size);
-  PTL_REQUIRE(aligned16(pages) && aligned16(codes) && (reinterpret_cast<uintptr_t>(words) & 7u) == 0 && n_tiles / 2 <= 65535, "kv8_expand: alignment");
-  if (n_tiles == 0) return 0;
-  const int x = width < 1024 ? width : 1024, chunks = (nkv * page_size * d / 8 + kKv8ExpandChunk - 1) / kKv8ExpandChunk;
-  PTL_REQUIRE(chunks <= 65535, "kv8_expand: pages are too large");
-  return launch_kernel("kv8_expand", kv8_expand_kernel, dim3(x, n_tiles / 2, chunks), dim3(kKv8Threads), 0, as_stream(stream),
-                       Kv8ExpandParams{(__nv_bfloat16*)pages, table, (const unsigned char*)codes, (const uint32_t*)words, block_table, tiles,
-                                       n_tiles / 2, slots, width, bt_stride, nkv, d, page_size, num_pages, window});
-}

@@ -13,6 +13,7 @@ import ctypes
 import functools
 import math
 import os
+import struct
 from array import array
 from typing import Optional, Tuple
 
@@ -95,10 +96,7 @@ _SIGNATURES = {
     "ptl_moe_combine": [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _ptr],
     "ptl_rope_kv8_write": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ll, _ptr],
     "ptl_read_kv8": [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr],
-    "ptl_attention8_single": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
-                              _c_int, _c_f, _c_int, _c_int, _c_int, _c_int, _ptr, _ptr, _c_int, _ptr, _ptr],
-    "ptl_attention8_portion": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f,
-                               _c_int, _c_int, _c_int, _ptr, _ptr],
+    "ptl_attention8_single": [ctypes.c_char_p], "ptl_attention8_portion": [ctypes.c_char_p],
     "ptl_attention8_simt": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                             _c_int, _c_f, _c_int, _c_int, _c_int, _ptr],
     "ptl_paged_attention_simt": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int,
@@ -203,10 +201,8 @@ def load_library() -> ctypes.CDLL:
     lib.ptl_prefill_attention_tc_bf16.argtypes = [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                                   _c_int, _c_int, _c_int, _c_f, _c_int, _c_int, _ptr, _ptr]
     lib.ptl_prefill_attention_tc_bf16.restype = _c_int
-    lib.ptl_prefill_attention_tc_holes_bf16.argtypes = lib.ptl_prefill_attention_tc_bf16.argtypes[:-2] + [_c_int, _c_int, _ptr, _ptr, _ptr, _ptr]
-    lib.ptl_prefill_attention_tc_holes_bf16.restype = _c_int
-    lib.ptl_kv8_expand_bf16.argtypes = [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr]
-    lib.ptl_kv8_expand_bf16.restype = _c_int
+    lib.ptl_attention8_prefill_tc_bf16.argtypes = [ctypes.c_char_p]
+    lib.ptl_attention8_prefill_tc_bf16.restype = _c_int
     lib.ptl_argmax.argtypes = [_ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_ll, _ptr]
     lib.ptl_argmax.restype = _c_int
     lib.ptl_take_tokens.argtypes = [_ptr, _ptr, _ptr, _c_int, _c_int, _ptr]
@@ -909,6 +905,9 @@ class CudaOps:
         return out
 
     # ------------------------------------------------------------------ keys and values in 8 bits
+    # Arguments that go to the library in one piece: pointers, integers, the scale (0 for no pointer)
+    _ATTENTION8_ARGS = struct.Struct("=14Q13if")
+    _PREFILL8_ARGS = struct.Struct("=12Q14ifi")
     KV8_BLOCK = 16         # positions that share a scale
 
     def _want_kv8(self, codes: torch.Tensor, words: torch.Tensor, nkv: int, d: int, page_size: int) -> int:
@@ -1007,7 +1006,7 @@ class CudaOps:
             raise KernelError(f"paged_attention8: the block table is {tuple(width)}, expected a row per request")
         if tok_req.numel() < tokens or positions.numel() < tokens:
             raise KernelError("paged_attention8: fewer requests or positions than rows")
-        if window < 0:
+        if not 0 <= window <= 0x7fffffff:
             raise KernelError(f"paged_attention8: a window of {window} positions")
         if not 0 <= scale < math.inf:
             raise KernelError(f"paged_attention8: scores times {scale}")
@@ -1082,7 +1081,7 @@ class CudaOps:
         if n:
             pairs = n * nkv
             group = nq // nkv
-            per_head, units, counters, part_acc, part_ml = 0, None, None, None, None
+            per_head, units, counters, part_acc, part_ml = 0, None, 0, 0, 0
             f32 = q.dtype is torch.float32
             parts, warps = force or self._kv8_single_form(n, nkv, -(-longest // 256), d, f32, group > 8)
             if not parts:
@@ -1095,11 +1094,10 @@ class CudaOps:
                 part_acc = scratch.data_ptr()
                 part_ml = part_acc + nkv * per_head * group * d * 4
                 counters = units.data_ptr() + nkv * per_head * 32
-            rc = getattr(self.lib, "ptl_attention8_single" + suffix)(
+            rc = getattr(self.lib, "ptl_attention8_single" + suffix)(self._ATTENTION8_ARGS.pack(
                 out.data_ptr(), part_acc, part_ml, q.data_ptr(), codes.data_ptr(), words.data_ptr(), block_table.data_ptr(),
-                None if dec.in_order else dec.tensor.data_ptr(), tok_req.data_ptr(), positions.data_ptr(), n, stride, nq * d,
-                width, nq, nkv, d, page_size, scale, window, parts, warps, per_head, None if units is None else units.data_ptr(), counters, pages,
-                self._tc_status_word().data_ptr(), stream)
+                0 if dec.in_order else dec.tensor.data_ptr(), tok_req.data_ptr(), positions.data_ptr(), 0 if units is None else units.data_ptr(), counters,
+                self._tc_status_word().data_ptr(), stream, n, stride, nq * d, width, nq, nkv, d, page_size, window, parts, warps, per_head, pages, scale))
             if rc == -2:
                 return False
             self._check(rc)
@@ -1109,10 +1107,10 @@ class CudaOps:
             # rows of a tile are multiplied whatever they hold (heads of 128: 16 tokens behind 6,000 41 and 46 us, behind 30,000 96 and 195).
             rows = (q.shape[0] - n) / (tiles.items // 2)             # of a pair of tiles, on average
             few = longest <= 192 or (rows <= 32 and longest >= 3000) if split_portions is None else bool(split_portions)
-            if q.dtype == torch.bfloat16 and not few and self._attention8_portions(out, q, codes, words, block_table, nq, nkv, d, page_size, scale,
-                                                                                   window, longest, tiles, hints, stream):
+            if q.dtype == torch.bfloat16 and not few and self._attention8_portions(out, q, stride, codes, words, pages, block_table, nq, nkv, d, page_size,
+                                                                                   scale, window, longest, tiles, hints, stream):
                 return True
-            splits, part_acc, part_ml = 1, None, None
+            splits, part_acc, part_ml = 1, 0, 0
             if few or q.dtype == torch.float32:
                 blocks = max(1, (q.shape[0] - n) * nq // (64 if q.dtype == torch.float32 or d == 128 else 128))
                 splits = max(1, min(self._sm_count * 3 // blocks, -(-longest // 256), 32))
@@ -1120,16 +1118,17 @@ class CudaOps:
                 scratch = tok_req.new_empty(q.shape[0] * nq * splits * (d + 2))      # float32
                 part_acc = scratch.data_ptr()
                 part_ml = part_acc + q.shape[0] * nq * splits * d * 4
-            rc = getattr(self.lib, "ptl_attention8_portion" + suffix)(
-                out.data_ptr(), part_acc, part_ml, q.data_ptr(), codes.data_ptr(), words.data_ptr(), block_table.data_ptr(), tiles.tensor.data_ptr(),
-                tiles.items, q.shape[1], nq * d, block_table.shape[1], nq, nkv, d, page_size, scale, window, splits, codes.shape[0],
-                self._tc_status_word().data_ptr(), stream)
+            rc = getattr(self.lib, "ptl_attention8_portion" + suffix)(self._ATTENTION8_ARGS.pack(
+                out.data_ptr(), part_acc, part_ml, q.data_ptr(), codes.data_ptr(), words.data_ptr(), block_table.data_ptr(), tiles.tensor.data_ptr(), 0, 0,
+                0, 0, self._tc_status_word().data_ptr(), stream, tiles.items, stride, nq * d, width, nq, nkv, d, page_size, window, splits, 4, 0, pages,
+                scale))
             self._check(rc, kernels=2 if splits > 1 else 1)
         return True
 
     KV8_EXPAND_BYTES = 1 << 30       # of pages made bfloat16 for one call, at most
 
-    def _attention8_portions(self, out, q, codes, words, block_table, nq, nkv, d, page_size, scale, window, longest, tiles, hints, stream) -> bool:
+    def _attention8_portions(self, out, q, stride, codes, words, pages, block_table, nq, nkv, d, page_size, scale, window, longest, tiles, hints,
+                             stream) -> bool:
         """bfloat16 portions on the fifth-generation tensor cores, over the pages they see made bfloat16 first; False where they are too many
         (a captured step counts its longest contexts) or of a size that those tiles do not take."""
         keys = 128 if d == 64 else 64
@@ -1137,26 +1136,24 @@ class CudaOps:
             return False
         requests, width = block_table.shape
         slots = min(requests, tiles.items // 2)
-        pages = slots * width + 1
-        if pages * 4 * nkv * page_size * d > self.KV8_EXPAND_BYTES:
+        made = slots * width + 1
+        if made * 4 * nkv * page_size * d > self.KV8_EXPAND_BYTES:
             return False
         pairs = self._portion_pairs(hints, keys, page_size, window)
         if pairs is None or len(pairs) != tiles.items // 2:      # (a captured step: as if all were the longest)
             pairs = ((-(-(longest + page_size) // keys), 256),) * (tiles.items // 2)
         splits, split_tiles = self._kv8_split_plan(pairs, nq, d, self._sm_count)
-        part_acc = part_ml = None
+        part_acc = part_ml = 0
         if splits > 1:
             scratch = block_table.new_empty(q.shape[0] * nq * splits * (d + 2))      # float32
             part_acc = scratch.data_ptr()
             part_ml = part_acc + q.shape[0] * nq * splits * d * 4
-        place, table = q.new_empty(pages * 2 * nkv * page_size * d), block_table.new_empty((requests, width))
-        self._check(self.lib.ptl_kv8_expand_bf16(place.data_ptr(), table.data_ptr(), codes.data_ptr(), words.data_ptr(), block_table.data_ptr(),
-                                                 tiles.tensor.data_ptr(), tiles.items, slots, width, width, nkv, d, page_size, codes.shape[0],
-                                                 window, stream))
-        self._check(self.lib.ptl_prefill_attention_tc_holes_bf16(out.data_ptr(), q.data_ptr(), place.data_ptr(), table.data_ptr(), tiles.tensor.data_ptr(),
-                                                                 tiles.items, q.shape[0], q.shape[1], nq * d, width, nq, nkv, d, page_size, scale,
-                                                                 window, pages, splits, split_tiles, part_acc, part_ml, self._tc_status_word().data_ptr(), stream),
-                    kernels=2 if splits > 1 else 1)
+        place, table = q.new_empty(made * 2 * nkv * page_size * d), block_table.new_empty(requests, width)
+        self._check(self.lib.ptl_attention8_prefill_tc_bf16(self._PREFILL8_ARGS.pack(
+            out.data_ptr(), q.data_ptr(), place.data_ptr(), table.data_ptr(), codes.data_ptr(), words.data_ptr(), block_table.data_ptr(),
+            tiles.tensor.data_ptr(), part_acc, part_ml, self._tc_status_word().data_ptr(), stream, tiles.items, q.shape[0], stride, nq * d, width, slots, nq,
+            nkv, d, page_size, pages, window, splits, split_tiles, scale, 0)),
+                    kernels=3 if splits > 1 else 2)
         return True
 
     def _portion_pairs(self, hints, keys: int, page_size: int, window: int):

@@ -78,6 +78,7 @@ def test_tensors_of_another_device(ops):
     (dict(page_size=24), "no whole blocks"),
     (dict(d=512), "up to 256"),
     (dict(window=-1), "window"),
+    (dict(window=1 << 31), "window"),
     (dict(scale=-0.125), "scores times"),
     (dict(scale=float("nan")), "scores times"),
 ])
@@ -169,3 +170,17 @@ def test_the_library_refuses_before_it_launches():
     launches = ctypes.c_int(7)
     ptrs, rows = (ctypes.c_void_p * 1)(at), (ctypes.c_longlong * 1)(0)
     assert lib.ptl_copy_pages(ptrs, rows, 1, ctypes.addressof(n), ctypes.addressof(n), 1, ctypes.byref(launches), None) == -1 and "no rows" in err()
+
+
+def test_every_entry_that_the_operators_call_has_its_signature():
+    """Without one, addresses would be cut to 32 bits."""
+    import re
+    from pathlib import Path
+
+    import pytriton_llama_b200.ops.cuda as module
+    lib = load_library()
+    text = Path(module.__file__).read_text()
+    names = set(re.findall(r"lib\.(ptl_\w+)\((?!\))", text)) | {n + t for n in re.findall(r'"(ptl_\w+)" \+ ', text) for t in ("_f32", "_bf16")}
+    assert len(names) > 50
+    without = [n for n in sorted(names) if hasattr(lib, n) and getattr(lib, n).argtypes is None]
+    assert without == []
