@@ -21,6 +21,7 @@
 // Logits of -inf have no probability.  A row with a NaN, with +inf, or with -inf only has no distribution: its
 // log-probabilities and its entropy are NaN.  Its alternatives are the largest logits all the same, NaN behind all others.
 #include "common.cuh"
+#include <cstring>
 
 namespace ptl {
 
@@ -341,9 +342,21 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
 }  // namespace ptl
 
 // logits [rows, vocab] float32, tokens int32 [rows]; logprob and entropy float32 [rows], top_logprob float32 and top_id int32 [rows, top].
-// top <= min(vocab, 32).  A token outside the vocabulary has log-probability -inf.
-PTL_EXPORT int ptl_token_scores(float* logprob, float* entropy, float* top_logprob, int* top_id, const float* logits, const int* tokens,
-                                int rows, int vocab, int top, void* stream) {
+// top <= min(vocab, 32).  A token outside the vocabulary has log-probability -inf.  The arguments are packed by the caller.
+struct TokenScoresArgs {
+  float *logprob, *entropy, *top_logprob;
+  int* top_id;
+  const float* logits;
+  const int* tokens;
+  void* stream;
+  int rows, vocab, top, zero;
+};
+static_assert(sizeof(TokenScoresArgs) == 7 * 8 + 4 * 4, "as it is packed");
+PTL_EXPORT int ptl_token_scores(const void* args) {
+  TokenScoresArgs a;
+  memcpy(&a, args, sizeof a);
+  const int rows = a.rows, vocab = a.vocab, top = a.top;
+  const float* logits = a.logits;
   using namespace ptl;
   PTL_REQUIRE(rows >= 0 && vocab > 0 && top >= 0, "token_scores: bad sizes");
   PTL_REQUIRE(top <= kTsMaxTop && top <= vocab, "token_scores: %d alternatives; at most %d, and no more than tokens", top, kTsMaxTop);
@@ -357,6 +370,6 @@ PTL_EXPORT int ptl_token_scores(float* logprob, float* entropy, float* top_logpr
   constexpr int kSmem = (int)sizeof(TsShared);
   auto kernel = top ? token_scores_kernel<true> : token_scores_kernel<false>;
   if (int rc = raise_shared_memory("token_scores", kernel, kSmem, raised[top ? 1 : 0])) return rc;
-  return launch_kernel_cluster("token_scores", kernel, dim3((unsigned)(rows * slices)), dim3(kTsThreads), kSmem, as_stream(stream), slices, logprob,
-                               entropy, top_logprob, top_id, logits, tokens, vocab, top, slices);
+  return launch_kernel_cluster("token_scores", kernel, dim3((unsigned)(rows * slices)), dim3(kTsThreads), kSmem, as_stream(a.stream), slices, a.logprob,
+                               a.entropy, a.top_logprob, a.top_id, logits, a.tokens, vocab, top, slices);
 }

@@ -94,8 +94,7 @@ _SIGNATURES = {
     "ptl_moe_grouped": [_ptr, _c_int, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f, _c_f, _c_f, _ptr],
     "ptl_moe_combine_norm": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_f, _ptr],
     "ptl_moe_combine": [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _ptr],
-    "ptl_rope_kv8_write": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ll, _ptr],
-    "ptl_read_kv8": [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr],
+    "ptl_rope_kv8_write": [ctypes.c_char_p], "ptl_read_kv8": [ctypes.c_char_p],
     "ptl_attention8_single": [ctypes.c_char_p], "ptl_attention8_portion": [ctypes.c_char_p],
     "ptl_attention8_simt": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                             _c_int, _c_f, _c_int, _c_int, _c_int, _ptr],
@@ -215,7 +214,7 @@ def load_library() -> ctypes.CDLL:
     lib.ptl_sample_cluster.restype = _c_int
     lib.ptl_sample_work_words.argtypes = []
     lib.ptl_sample_work_words.restype = _c_int
-    lib.ptl_token_scores.argtypes = [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _ptr]
+    lib.ptl_token_scores.argtypes = [ctypes.c_char_p]
     lib.ptl_token_scores.restype = _c_int
     lib.ptl_copy_pages.argtypes = [_ptr, _ptr, _c_int, _ptr, _ptr, _c_int, _ptr, _ptr]
     lib.ptl_copy_pages.restype = _c_int
@@ -905,7 +904,10 @@ class CudaOps:
         return out
 
     # ------------------------------------------------------------------ keys and values in 8 bits
-    # Arguments that go to the library in one piece: pointers, integers, the scale (0 for no pointer)
+    # Arguments that go to the library in one piece: pointers (0 for none), integers, the scale
+    _KV8_WRITE_ARGS = struct.Struct("=7Qq6i")
+    _KV8_READ_ARGS = struct.Struct("=6Q6i")
+    _TOKEN_SCORES_ARGS = struct.Struct("=7Q4i")
     _ATTENTION8_ARGS = struct.Struct("=14Q13if")
     _PREFILL8_ARGS = struct.Struct("=12Q14ifi")
     KV8_BLOCK = 16         # positions that share a scale
@@ -957,8 +959,9 @@ class CudaOps:
             if inv_freq.numel() < rot // 2:
                 raise KernelError("inv_freq shorter than half the rotary width")
         fn = getattr(self.lib, "ptl_rope_kv8_write" + _suffix(qkv.dtype))
-        self._check(fn(qkv.data_ptr(), positions.data_ptr(), _p(inv_freq), slots.data_ptr(), codes.data_ptr(), words.data_ptr(), rows, nq, nkv, d, rot,
-                       page_size, pages * page_size, self._stream()), kernels=1 if rows else 0)
+        self._check(fn(self._KV8_WRITE_ARGS.pack(
+            qkv.data_ptr(), positions.data_ptr(), 0 if inv_freq is None else inv_freq.data_ptr(), slots.data_ptr(), codes.data_ptr(), words.data_ptr(),
+            self._stream(), pages * page_size, rows, nq, nkv, d, rot, page_size)), kernels=1 if rows else 0)
 
     def read_kv8(self, codes: torch.Tensor, words: torch.Tensor, block_table: torch.Tensor, contexts, dtype: torch.dtype) -> torch.Tensor:
         """What an 8-bit cache holds of the first ``contexts[r]`` (host integers) positions of the requests in the table's rows,
@@ -981,8 +984,8 @@ class CudaOps:
         lengths = array("i", contexts)
         out = torch.empty(total, 2, nkv, d, dtype=dtype, device=self.device)
         fn = getattr(self.lib, "ptl_read_kv8" + _suffix(dtype))
-        self._check(fn(out.data_ptr(), codes.data_ptr(), words.data_ptr(), block_table.data_ptr(), lengths.buffer_info()[0], n, width, nkv, d,
-                       page_size, pages, self._stream()), kernels=1 if total else 0)
+        self._check(fn(self._KV8_READ_ARGS.pack(out.data_ptr(), codes.data_ptr(), words.data_ptr(), block_table.data_ptr(), lengths.buffer_info()[0],
+                                                self._stream(), n, width, nkv, d, page_size, pages)), kernels=1 if total else 0)
         return out
 
     def paged_attention8(self, q: torch.Tensor, codes: torch.Tensor, words: torch.Tensor, block_table: torch.Tensor, tok_req: torch.Tensor,
@@ -2772,8 +2775,9 @@ class CudaOps:
         logprob = logits.new_empty(rows)                     # (half the host's time of torch.empty with a type and a device, or a tuple of sizes)
         entropy = torch.empty_like(logprob)
         best, ids = logits.new_empty(rows, k), tokens.new_empty(rows, k)
-        self._check(self.lib.ptl_token_scores(logprob.data_ptr(), entropy.data_ptr(), best.data_ptr(), ids.data_ptr(), logits.data_ptr(),
-                                              tokens.data_ptr(), rows, vocab, k, self._stream()), kernels=1 if rows else 0)
+        self._check(self.lib.ptl_token_scores(self._TOKEN_SCORES_ARGS.pack(
+            logprob.data_ptr(), entropy.data_ptr(), best.data_ptr(), ids.data_ptr(), logits.data_ptr(), tokens.data_ptr(), self._stream(), rows, vocab, k,
+            0)), kernels=1 if rows else 0)
         return logprob, entropy, best, ids
 
     def sample_tokens(self, logits: torch.Tensor, temperature: Optional[torch.Tensor], top_p: Optional[torch.Tensor],

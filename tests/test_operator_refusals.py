@@ -150,7 +150,8 @@ def test_the_library_refuses_before_it_launches():
     err = lambda: lib.ptl_last_error().decode()
     buf = ctypes.create_string_buffer(4096)
     at = (ctypes.addressof(buf) + 63) // 64 * 64
-    w = lambda **o: lib.ptl_rope_kv8_write_bf16(at, at, None, at, o.get("codes", at), at, 1, 1, 1, o.get("d", 64), o.get("rot", 0), o.get("ps", 16), 64, None)
+    w = lambda **o: lib.ptl_rope_kv8_write_bf16(CudaOps._KV8_WRITE_ARGS.pack(at, at, 0, at, o.get("codes", at), at, 0, 64, 1, 1, 1, o.get("d", 64),
+                                                                             o.get("rot", 0), o.get("ps", 16)))
     assert w(d=40) == -1 and "head size 40" in err()
     assert w(ps=20) == -1 and "pages of 20" in err()
     assert w(rot=65) == -1 and "rotary width" in err()
@@ -163,10 +164,12 @@ def test_the_library_refuses_before_it_launches():
     assert a(words=at + 4) == -1 and "aligned" in err()
     assert a(splits=2) == -1 and "scratch" in err()
     n = (ctypes.c_int * 1)(17)
-    assert lib.ptl_read_kv8_f32(at, at, at, at, ctypes.addressof(n), 1, 1, 1, 64, 16, 4, None) == -1 and "17 tokens" in err()
-    assert lib.ptl_token_scores(at, at, at, at, at, at, 1, 40, 33, None) == -1 and "at most 32" in err()
-    assert lib.ptl_token_scores(at, at, at, at, at, at, 1, 4, 5, None) == -1 and "at most 32" in err()
-    assert lib.ptl_token_scores(at, at, at, at, at + 2, at, 1, 4, 1, None) == -1 and "aligned" in err()
+    read = CudaOps._KV8_READ_ARGS.pack(at, at, at, at, ctypes.addressof(n), 0, 1, 1, 1, 64, 16, 4)
+    assert lib.ptl_read_kv8_f32(read) == -1 and "17 tokens" in err()
+    scores = lambda logits, vocab, top: lib.ptl_token_scores(CudaOps._TOKEN_SCORES_ARGS.pack(at, at, at, at, logits, at, 0, 1, vocab, top, 0))
+    assert scores(at, 40, 33) == -1 and "at most 32" in err()
+    assert scores(at, 4, 5) == -1 and "at most 32" in err()
+    assert scores(at + 2, 4, 1) == -1 and "aligned" in err()
     launches = ctypes.c_int(7)
     ptrs, rows = (ctypes.c_void_p * 1)(at), (ctypes.c_longlong * 1)(0)
     assert lib.ptl_copy_pages(ptrs, rows, 1, ctypes.addressof(n), ctypes.addressof(n), 1, ctypes.byref(launches), None) == -1 and "no rows" in err()
