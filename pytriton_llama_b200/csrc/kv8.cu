@@ -254,7 +254,7 @@ template <int REQUESTS> struct Kv8ReadArgs {
 };
 
 template <typename T, int REQUESTS>
-__global__ void __launch_bounds__(kKv8Threads)
+__global__ void __launch_bounds__(kKv8Threads, 3)
 read_kv8_kernel(T* __restrict__ out, const unsigned char* __restrict__ codes, const uint32_t* __restrict__ words,
                 const int* __restrict__ block_table, const __grid_constant__ Kv8ReadArgs<REQUESTS> args, int bt_stride, int nkv, int d, int page_size,
                 int num_pages) {
@@ -319,7 +319,7 @@ struct Kv8ExpandParams {
 
 constexpr int kKv8ExpandChunk = kKv8Threads * kKv8ReadAhead;      // packets of a page a block takes
 
-__global__ void __launch_bounds__(kKv8Threads)
+__global__ void __launch_bounds__(kKv8Threads, 3)
 kv8_expand_kernel(const Kv8ExpandParams p) {
   // tiles and the block table are inputs of the step, not results of the kernel before this one
   const int page_codes = 2 * p.nkv * p.page_size * p.d, lane = threadIdx.x & 31;
