@@ -79,6 +79,17 @@ struct TsShared {
 
 // Places the `top` largest of n keys (unique but for zeros, which are none) in order in best[0 .. top): a key's place is the number of larger ones.
 __device__ __forceinline__ void ts_select(const TsKey* keys, int n, int top, TsKey* best) {
+  if (n <= kTsThreads / 2) {                           // two or four threads a key
+    const int parts = n <= kTsThreads / 4 ? 4 : 2, i = threadIdx.x / parts;
+    const TsKey k = i < n ? keys[i] : 0;
+    int place = 0;
+#pragma unroll 8
+    for (int j = threadIdx.x % parts; j < n; j += parts) place += keys[j] > k;
+    place += __shfl_xor_sync(0xffffffffu, place, 1);
+    if (parts == 4) place += __shfl_xor_sync(0xffffffffu, place, 2);
+    if (k != 0 && place < top && threadIdx.x % parts == 0) best[place] = k;
+    return;
+  }
   for (int i = threadIdx.x; i < n; i += kTsThreads) {
     const TsKey k = keys[i];
     if (k == 0) continue;
@@ -210,19 +221,31 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
     float least = ts_logit(threshold);                 // (NaN, a threshold that is no number or none: everything comes in)
     const int lanes_with = __popc(__ballot_sync(0xffffffffu, !(mx < least)));
     if (lanes_with == 0) return;
-    auto key_at = [&](int i) {
+    auto pick = [&](int i) {                           // at(i), i no constant
+      float x8[8], x4[4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x8[j] = i & 1 ? v[j].y : v[j].x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x4[j] = i & 2 ? x8[2 * j + 1] : x8[2 * j];
+      const float lo = i & 4 ? x4[1] : x4[0], hi = i & 4 ? x4[3] : x4[2];
+      return i & 8 ? hi : lo;
+    };
+    static_assert(kTsPerThread == 16, "four choices between two");
+    auto key_of = [&](int i, float x_i) {
       const int p = packet(base, i / 4), e = 4 * p - skew + i % 4;
-      return p < p1 && e >= 0 && e < vocab ? ts_key(at(i), e) : (TsKey)0;
+      return p < p1 && e >= 0 && e < vocab ? ts_key(x_i, e) : (TsKey)0;
     };
     if (lanes_with > 16) {
       TsKey mine = 0;
       if (mx > -INFINITY) {                            // the first of the lane's largest (what is behind the row is -inf)
+        int first = 0;
 #pragma unroll
         for (int i = kTsPerThread - 1; i >= 0; --i)
-          if (at(i) == mx) mine = key_at(i);
+          if (at(i) == mx) first = i;
+        mine = key_of(first, mx);
       } else {
-#pragma unroll
-        for (int i = 0; i < kTsPerThread; ++i) mine = max(mine, key_at(i));
+#pragma unroll 1
+        for (int i = 0; i < kTsPerThread; ++i) mine = max(mine, key_of(i, pick(i)));
       }
       int place = 0;
       for (int j = 0; j < 32; ++j) place += __shfl_sync(0xffffffffu, mine, j) > mine;
@@ -233,10 +256,16 @@ token_scores_kernel(float* __restrict__ logprob, float* __restrict__ entropy, fl
         if (raised > threshold) { threshold = raised; least = ts_logit(raised); }
       }
     }
+    // a bit for each logit that some lane may keep; few, and what they cost is theirs, not the sixteen's (2,300 cycles a turn that had one when
+    // every logit of a thread was voted on, 100 rows with 20 alternatives 31 us)
+    uint32_t bits = 0;
 #pragma unroll
-    for (int i = 0; i < kTsPerThread; ++i) {
-      if (!__any_sync(0xffffffffu, !(at(i) < least))) continue;
-      const TsKey k = key_at(i);
+    for (int i = 0; i < kTsPerThread; ++i)
+      if (!(at(i) < least)) bits |= 1u << i;
+#pragma unroll 1
+    for (uint32_t left = __reduce_or_sync(0xffffffffu, bits); left; left &= left - 1) {
+      const int i = __ffs(left) - 1;
+      const TsKey k = key_of(i, pick(i));
       const unsigned who = __ballot_sync(0xffffffffu, k > threshold);
       if (k > threshold) sh.list[warp][have + __popc(who & ((1u << lane) - 1u))] = k;
       have += __popc(who);
