@@ -649,7 +649,7 @@ attention8_single_kernel(const A8Params p) {
 // Portions: a warp has rows of its own, the heads of the group for as many neighbouring tokens as fit 8 NT rows; the block's warps have
 // neighbouring ones and read the same keys out of one ring of slots, a turn's kA8Turn blocks each.  For float32, and for bfloat16 where
 // the fifth-generation tensor cores do not pay (CudaOps._attention8_tensor_cores has the figures); mma.sync bounds it: a prompt of 2,048 tokens
-// takes 133 us here and 51 there.  The warps take turns at fetching: turn i's
+// takes 133 us here and 50 there.  The warps take turns at fetching: turn i's
 // one refills the slot that turn i - kLag left, which the others are through with by then (but for the slowest, which it waits for).
 template <int D, typename T> struct A8Portion {
   static constexpr int kTiles = D == 64 ? (sizeof(T) == 2 ? 4 : 2) : 2;

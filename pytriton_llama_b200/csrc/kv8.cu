@@ -9,9 +9,10 @@
 // of many rows, at 16, and takes the runs that begin there.
 //
 // What bounds it: three loads that wait for one another (slots, then the run's values and the word, then, where the exponent grows, the codes) and
-// the launch; one rounding a code, by fma.rd.  Four prompts of 301 to 1,021 tokens (8 heads of 128) are written and read back in 15.4 us,
-// of which the bytes take 5.2; 64 single tokens in 9.5 of 1.5.  Five blocks an SM (up to 96 registers) where the compiler would take 128: 2,644
-// rows are one wave of blocks, 18.0 us otherwise.
+// the launch; one rounding a code, by fma.rd.  Four prompts of 301 to 1,021 tokens (8 heads of 128) are written and read back in 13.0 us,
+// of which the bytes take 5.2; 64 single tokens in 8.0 of 1.5.  Five blocks an SM (up to 96 registers) where the compiler would take 128: 2,644
+// rows are one wave of blocks (by three, four, five and six an SM 14.9, 14.7, 13.0 and 13.6 us).  Reading back and making pages bfloat16 are given up to 80
+// registers, so that a thread's four packets are asked for at once (the compiler keeps to 64: 9.4 and 15.4 us).
 #include "kv8.cuh"
 #include <cstring>
 
@@ -400,7 +401,7 @@ static int rope_kv8_write(T* qkv, const int* positions, const float* inv_freq, c
   if (rot == 0) inv_freq = nullptr;
   Kv8WriteParams p{qkv, positions, inv_freq, slots, (unsigned char*)codes, (uint32_t*)words, tokens, nq, nkv, d, rot, page_size, 1, num_slots};
   // Steps of many rows are mostly prompts, whose runs are long: a block a row asks for every row's slot many times over there.  Written and read
-  // back, us, by one row and by 16 a block: 64 single tokens (8 heads of 64) 9.5 and 25.8; one prompt (8 heads of 128) of 500 8.7 and 9.0, of
+  // back (before reading was faster), us, by one row and by 16 a block: 64 single tokens (8 heads of 64) 9.5 and 25.8; one prompt (8 heads of 128) of 500 8.7 and 9.0, of
   // 1,024 10.4 and 8.5, of 1,500 13.0 and 9.6.
   p.rows_per_block = tokens > 512 ? kKv8Block : 1;
   const size_t smem = inv_freq ? (size_t)(p.rows_per_block + kKv8Block - 1) * rot * sizeof(float) : 0;

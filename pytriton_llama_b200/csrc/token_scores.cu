@@ -14,9 +14,9 @@
 // order, or equal ones), it is raised for them to the `top`-th largest of the lanes' own.  At the end what the warps have, then what
 // the blocks have, is ranked the same way.
 //
-// What bounds it: the bytes where no alternatives are asked for (500 rows of 128,256: 42.7 us, 6.0 TB/s); with 20 of them 55.9, the looks at the
-// threshold, the lists and the ranking at the end, 0.47 of the issue slots; 8 rows with five 11.1 us, a cluster of eight blocks a row, of which the bytes
-// take 0.64: three trips through its start, one wave of loads and two cluster barriers.
+// What bounds it: the bytes where no alternatives are asked for (500 rows of 128,256: 42.8 us, 6.0 TB/s); with 20 of them 49.6, the turns that have
+// logits above the threshold and the ranking at the end; 8 rows with five 9.3 us, a cluster of eight blocks a row, of which the bytes
+// take 0.64: its start, two turns of loads, the ranking and two cluster barriers.
 //
 // Logits of -inf have no probability.  A row with a NaN, with +inf, or with -inf only has no distribution: its
 // log-probabilities and its entropy are NaN.  Its alternatives are the largest logits all the same, NaN behind all others.
@@ -392,8 +392,12 @@ PTL_EXPORT int ptl_token_scores(const void* args) {
   PTL_REQUIRE(vocab <= 0x7fffff00 - kTsTurn, "token_scores: too many tokens");
   PTL_REQUIRE((reinterpret_cast<uintptr_t>(logits) & 3u) == 0, "token_scores: logits must be 4-byte aligned");
   if (rows == 0) return 0;
+  // As many slices as are resident at once; with alternatives and more rows than SMs one, because a slice's first turns, before its threshold is
+  // near, cost more than its last (128,256 logits, 20 alternatives: 100 rows in 1, 2 and 4 slices 30.7, 29.2 and 27.3 us, 200 rows in 1 and
+  // 2 34.4 and 42.8, 290 36.3 and 43.9).
   int slices = 1;
-  while (slices < kTsMaxCluster && (long long)rows * slices * 2 <= 592 && vocab / (slices * 2) >= 4096) slices *= 2;
+  if (top == 0 || rows <= 148)
+    while (slices < kTsMaxCluster && (long long)rows * slices * 2 <= 592 && vocab / (slices * 2) >= 4096) slices *= 2;
   PTL_REQUIRE((long long)rows * slices <= 0x7fffffffLL, "token_scores: too many rows");
   static SmemRaised raised[2] = {};
   constexpr int kSmem = (int)sizeof(TsShared);
