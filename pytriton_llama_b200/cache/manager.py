@@ -468,24 +468,51 @@ class CacheManager:
                 pages[held] = rename[pages[held]]
         return out
 
-    def resize(self, num_pages: int, copy) -> None:
-        """Gives every pool ``num_pages`` pages (pools of block means what goes with them), entry by entry in new memory.  Raises
-        where more are in use."""
+    def pages_after_resize(self, num_pages: int) -> Dict[int, int]:
+        """Group -> pages that ``resize`` gives its pool (pools of block means: what goes with ``num_pages``).  Raises where more are
+        in use."""
         want = {gi: self.summary_pages(num_pages, grp.need.window) if grp.need.kind == "summary" else num_pages
                 for gi, grp in enumerate(self.groups) if grp.paged}
         for gi, n in want.items():
             if n <= 0 or n < self.groups[gi].pool.used_pages:
                 raise OutOfPages(f"group {gi}: {self.groups[gi].pool.used_pages} pages are in use, {n} are to stay")
+        return want
+
+    def resize(self, num_pages: int, copy) -> None:
+        """Gives every pool another number of pages (``pages_after_resize``), tensor by tensor in new memory, so that only one of them is
+        there twice at a time.  Where memory runs out half way, every pool gets its old number of pages again, or, where that does not fit
+        either, the smaller of the two, and the exception goes on; requests keep what they hold."""
+        want = self.pages_after_resize(num_pages)
+        before = {gi: self.groups[gi].pool.num_pages for gi in want}
         self.compact(copy)
-        for gi, n in want.items():
-            grp = self.groups[gi]
-            used = grp.pool.used_pages
-            for held in (grp.kv, grp.words):
-                for e in list(held):
-                    old = held[e]
-                    held[e] = torch.zeros((n, *old.shape[1:]), dtype=old.dtype, device=old.device)
-                    held[e][:used].copy_(old[:used])
-            grp.pool.resize(n)
+        try:
+            for gi, n in want.items():
+                self._give_rows(self.groups[gi], n)
+        except BaseException:
+            for gi, n in before.items():
+                grp = self.groups[gi]
+                try:
+                    self._give_rows(grp, n)
+                except Exception:                  # no memory for that: the rows that every tensor has
+                    n = min([n] + [t.shape[0] for t in grp.page_tensors()])
+                    for held in (grp.kv, grp.words):
+                        for e in held:
+                            held[e] = held[e][:n]
+                    grp.pool.resize(n)
+            raise
+
+    @staticmethod
+    def _give_rows(grp: CacheGroup, pages: int) -> None:
+        """The group's tensors and pool with that many pages, those in use first and kept."""
+        used = grp.pool.used_pages
+        for held in (grp.kv, grp.words):
+            for e, old in held.items():
+                if old.shape[0] != pages:
+                    new = torch.zeros((pages, *old.shape[1:]), dtype=old.dtype, device=old.device)
+                    new[:used].copy_(old[:used])
+                    held[e] = new
+                    del new
+        grp.pool.resize(pages)
 
     def release_all(self) -> None:
         for req in list(self._requests):

@@ -629,15 +629,23 @@ class Engine:
 
     def resize_cache(self, num_pages: int) -> None:
         """Gives the cache another number of pages per group while requests are live, so that memory can be given to something
-        else, or taken back.  Captured steps are captured again: they hold the old pages' addresses."""
+        else, or taken back.  Captured steps are captured again: they hold the old pages' addresses.  Where memory runs out half way the
+        cache goes back to what it was, or to the smaller of the two sizes, and the exception goes on (``CacheManager.resize``)."""
         if num_pages <= 0:
             raise ValueError("num_pages must be positive")
-        self.cache.resize(int(num_pages), self.ops.copy_pages)
+        self.cache.pages_after_resize(int(num_pages))      # refused before anything is given up
+        self._drop_captured_steps()
+        try:
+            self.cache.resize(int(num_pages), self.ops.copy_pages)
+        finally:
+            if self.device.type == "cuda":
+                torch.cuda.empty_cache()       # what the old pages took goes back to the device
+
+    def _drop_captured_steps(self) -> None:
+        """Captured steps and their memory; a shape that comes again is captured again."""
         if self._graphs and self.device.type == "cuda":
             torch.cuda.synchronize(self.device)
         self._graphs.clear()
-        if self.device.type == "cuda":
-            torch.cuda.empty_cache()           # what the old pages took goes back to the device
 
     def cached_kv(self, request: Hashable, entry: int = 0) -> torch.Tensor:
         """The keys and values of ``request`` in a cache entry as attention reads them, [tokens, 2 (k, v), kv_heads, head_dim] in the compute

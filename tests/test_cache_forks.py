@@ -226,3 +226,55 @@ def test_resize_refuses_less_than_is_held():
     c.m.resize(4, copy)
     assert c.m.groups[0].kv[0].shape[0] == c.m.groups[0].words[0].shape[0] == 4
     c.check()
+
+
+class NoMemory(RuntimeError):
+    pass
+
+
+def no_memory(monkeypatch, good, after=10 ** 9):
+    """Of the next allocations the first ``good`` succeed, those behind them do not, from ``after`` on they do again."""
+    real, count = torch.zeros, [0]
+
+    def zeros(*args, **kwargs):
+        count[0] += 1
+        if good < count[0] <= after:
+            raise NoMemory(f"allocation {count[0]}")
+        return real(*args, **kwargs)
+    monkeypatch.setattr(torch, "zeros", zeros)
+
+
+@pytest.mark.parametrize("recovers", [False, True])
+@pytest.mark.parametrize("pages", [12, 90])
+@pytest.mark.parametrize("good", range(6))
+@pytest.mark.parametrize("kind", ["full", "bits8", "window", "pooled"])
+def test_a_resize_without_memory_leaves_a_whole_cache(kind, good, pages, recovers):
+    """Whichever tensor there is no memory for: pools and tensors agree, requests hold what they held and go on, and a later resize works.  Where
+    there is memory to go back, the number of pages is the old one."""
+    c = Content(ENTRIES[kind] | ({2: FULL8} if kind == "full" else {}))
+    c.append("x", 20)
+    c.append("a", 60)
+    c.append("b", 33)
+    c.release("x")
+    before = {gi: grp.pool.num_pages for gi, grp in enumerate(c.m.groups) if grp.paged}
+    want = c.m.pages_after_resize(pages)
+    with pytest.MonkeyPatch.context() as patch:
+        no_memory(patch, good, good + 1 if recovers else 10 ** 9)
+        if good >= sum(len(g.page_tensors()) for gi, g in enumerate(c.m.groups) if g.paged and want[gi] != before[gi]):
+            c.m.resize(pages, copy)
+            before = want
+        else:
+            with pytest.raises(NoMemory):
+                c.m.resize(pages, copy)
+    for gi, n in before.items():
+        grp = c.m.groups[gi]
+        assert grp.pool.num_pages in ((n,) if recovers else (n, min(n, want[gi])))
+        assert {t.shape[0] for t in grp.page_tensors()} == {grp.pool.num_pages} and all(t.is_contiguous() for t in grp.page_tensors())
+    c.check()
+    c.append("a", 40)
+    c.fork("a", ["d"])
+    c.append("d", 3)
+    c.check()
+    c.m.resize(40, copy)
+    c.check()
+    assert all(grp.pool.num_pages == t.shape[0] for grp in c.m.groups if grp.paged for t in grp.page_tensors())

@@ -175,3 +175,35 @@ def test_what_an_8_bit_cache_refuses(model_folders):
     with pytest.raises(ValueError, match="compute type"):
         Engine(None, EngineConfig(cache_bits=8, max_gpu_num_blocks=4), device="cpu", ops=TorchOps8(), model_config=plain_tibepel.TINY[name], random_seed=0)
     assert TINY["A"]["head_dim"] == 16
+
+
+def test_captured_steps_go_before_the_pages_do(model_folders, monkeypatch):
+    """Whether the new pages can be had or not: a captured step holds the old ones' addresses.  What is refused beforehand costs nothing."""
+    cfg = EngineConfig(dtype="float32", page_size=16, max_gpu_num_blocks=10, max_seq_len=96, max_num_seqs=4, cache_bits=8)
+    eng = Engine(model_folders("B"), cfg, device="cpu", ops=TorchOps8())
+    eng.step([StepEntry("a", random_tokens(40, 384, 1))])
+    held = eng.cached_kv("a")
+    captured = {4: object(), (64, 4, 1, ()): object(), (128, 4, 1, ()): object()}
+    real = torch.zeros
+
+    def second_fails(*args, **kwargs):
+        assert not eng._graphs
+        calls.append(args)
+        if len(calls) > 1:
+            raise MemoryError
+        return real(*args, **kwargs)
+    for pages in (5, 30):
+        eng._graphs.update(captured)
+        calls = []
+        with pytest.raises(OutOfPages):
+            eng.resize_cache(2)
+        assert len(eng._graphs) == 3
+        with monkeypatch.context() as patch:
+            patch.setattr(torch, "zeros", second_fails)
+            with pytest.raises(MemoryError):
+                eng.resize_cache(pages)
+        assert not eng._graphs
+        assert torch.equal(eng.cached_kv("a"), held)
+        eng.step([StepEntry("a", [1], want=[0])])
+        held = eng.cached_kv("a")
+        eng.cache.check_invariants()
