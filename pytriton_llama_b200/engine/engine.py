@@ -642,10 +642,12 @@ class Engine:
                 torch.cuda.empty_cache()       # what the old pages took goes back to the device
 
     def _drop_captured_steps(self) -> None:
-        """Captured steps and their memory; a shape that comes again is captured again."""
+        """Captured steps and their memory; a shape that comes again is captured again, and counts once."""
         if self._graphs and self.device.type == "cuda":
             torch.cuda.synchronize(self.device)
+        self._shape_captures -= sum(isinstance(k, tuple) for k in self._graphs)
         self._graphs.clear()
+        self._graph_pool = None                # (a pool whose graphs are gone takes no capture while a caller holds logits in it)
 
     def cached_kv(self, request: Hashable, entry: int = 0) -> torch.Tensor:
         """The keys and values of ``request`` in a cache entry as attention reads them, [tokens, 2 (k, v), kv_heads, head_dim] in the compute

@@ -207,3 +207,16 @@ def test_captured_steps_go_before_the_pages_do(model_folders, monkeypatch):
         eng.step([StepEntry("a", [1], want=[0])])
         held = eng.cached_kv("a")
         eng.cache.check_invariants()
+
+
+def test_steps_captured_again_after_a_resize_count_once(model_folders):
+    """However often the cache changes its size, shapes do not use up the captures that an engine makes; those dropped for others still do.  The
+    memory of the dropped graphs is not captured into again."""
+    cfg = EngineConfig(dtype="float32", page_size=16, max_gpu_num_blocks=10, max_seq_len=96, max_num_seqs=4)
+    eng = Engine(model_folders("B"), cfg, device="cpu", ops=TorchOps8())
+    eng._shape_captures = 5                                # of shapes that others have driven out
+    for pages in [12, 9] * 60:
+        eng._graphs.update({4: object(), (64, 4, 1, ()): object(), (128, 4, 1, ()): object()})
+        eng._shape_captures, eng._graph_pool = eng._shape_captures + 2, object()
+        eng.resize_cache(pages)
+        assert eng._shape_captures == 5 and eng._graph_pool is None

@@ -149,3 +149,20 @@ def test_command_line(model_folders, capsys):
                      "--top_logprobs", "2", "--max_gpu_num_blocks", "64", "--max_seq_len", "128"]) == 0
     lines = capsys.readouterr().out.strip().splitlines()
     assert len([x for x in lines if not x.startswith("  ")]) == 3
+
+
+def test_mixed_steps_are_captured_after_any_number_of_resizes(model_folders):
+    """Beside logits that the caller still holds in the memory of the graphs that went."""
+    eng = Engine(model_folders("D", torch.bfloat16), _config("D", "bfloat16", cache_bits=8, compiled_model=True, capture_mixed_steps=True), device="cuda:0")
+    eng.GRAPH_MAX_CAPTURES = 4
+    prompt, held, want = random_tokens(60, TINY["D"]["vocab_size"], 1), [], None
+    for i in range(12):
+        for _ in range(3):                                 # seen, captured, replayed
+            held.append(eng.step([StepEntry("a", prompt, want=[59])], own_logits=False).logits)
+            eng.finish("a")
+            if len(held) > 1:                              # (the first was not captured: other key splits)
+                want = held[-1].clone() if want is None else want
+                assert torch.equal(held[-1], want)
+        assert any(isinstance(k, tuple) for k in eng._graphs)
+        eng.resize_cache(60 + i)
+    eng.check_device_status()
