@@ -171,7 +171,10 @@ class _Table:
 
     def held_below(self, block: int, first: int, pool: PagePool) -> int:
         """Pages that blocks ``first`` .. ``block`` - 1 hold alone."""
-        return sum(p >= 0 and pool.holders(p) == 1 for p in self.pages[first:min(block, self.n)].tolist()) if block > first else 0
+        if block <= first:
+            return 0
+        pages = self.pages[first:min(block, self.n)]       # nearly all given back: a step's look at a long request goes by numpy
+        return sum(pool.holders(p) == 1 for p in pages[pages >= 0].tolist())
 
 
 @dataclass

@@ -1,6 +1,7 @@
 """Forked requests, pages that move, pools that change their size: no page lost, nothing written by one request seen by another."""
 import random
 
+import numpy as np
 import pytest
 import torch
 
@@ -278,3 +279,27 @@ def test_a_resize_without_memory_leaves_a_whole_cache(kind, good, pages, recover
     c.m.resize(40, copy)
     c.check()
     assert all(grp.pool.num_pages == t.shape[0] for grp in c.m.groups if grp.paged for t in grp.page_tensors())
+
+
+def test_pages_that_a_window_has_passed_are_counted_without_a_look_at_each():
+    """A long request's blocks below the window are nearly all given back; planning a step asks the pool about those that are still held."""
+    m = CacheManager({0: CacheNeed(kind="window", kv_heads=1, head_dim=16, window=40)}, 16, 30, 3, 20000, "cpu", torch.float32, allocate=False)
+    m.admit("a")
+    for _ in range(19000 // 38):
+        m.append("a", 38)
+    looked_at = []
+
+    class Blocks(np.ndarray):
+        def tolist(self):
+            looked_at.append(self.size)
+            return super().tolist()
+    have = m.tokens_of("a")
+    first = max(0, have - 39) // 16
+    alone = sum(p >= 0 for p in m.block_table("a", 0)[:first])
+    table = m._requests["a"].tables[0]
+    table.pages = table.pages.view(Blocks)
+    assert m.pages_needed("a", 38)[0] == -(-(have + 38) // 16) - -(-have // 16) - alone
+    assert sum(looked_at) == alone > 0 and first > 1000
+    m.fork("a", ["b"], copy)
+    assert m.pages_needed("a", 38)[0] == -(-(have + 38) // 16) - -(-have // 16)
+    m.check_invariants()
