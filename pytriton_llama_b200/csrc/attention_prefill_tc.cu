@@ -36,9 +36,10 @@
 // the block drains.
 //
 // HOLES: pages may be missing in the middle of a request (an 8-bit cache's portions, kv8.cu, come here with their pages made bfloat16
-// in a place of their own).  A missing page's keys are masked, and the last page of the cache, zeros, is fetched in its place.  There too the
-// keys may be split over blockIdx.z where pairs and heads are fewer than SMs (a key tile takes a block 1.3 to 2 us, however few
-// blocks there are): a block leaves its accumulator, maximum and sum, and a kernel of its own joins them.
+// in a place of their own), and the table may end before a request's last position.  A missing page's keys are masked, and the last page of
+// the cache, zeros, is fetched in its place.  There too the keys may be split over blockIdx.z where pairs and heads are fewer than SMs (a key
+// tile takes a block 1.3 to 2 us, however few blocks there are): a block leaves its accumulator, maximum and sum, and a kernel of its
+// own joins them.
 //
 // tiles[2j], tiles[2j+1] = {request row, first token index, rows, position of the first token};
 // the second entry either continues the first (same request, first token and position + 128) or
@@ -216,7 +217,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
   const bool staged = n_blocks <= kTcStagedPages;
   if (staged)
     for (int i = threadIdx.x; i < n_blocks; i += Cfg::kThreads) s_pages[i] = i < have_blocks ? bt_global[first_block + i] : -1;
-  int holes = 0;
+  int holes = last_key / p.page_size >= p.bt_stride;       // (positions behind the table's row have no page either)
   if (HOLES)
     for (int i = threadIdx.x; i < have_blocks; i += Cfg::kThreads) holes |= bt_global[first_block + i] < 0;
   for (int i = threadIdx.x; i < Cfg::kExchangeBytes / 8; i += Cfg::kThreads) s_xchg[i] = 0ull;      // sequence numbers start at 0
@@ -437,7 +438,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
 #pragma unroll 1
         for (int b = 0; b < kTcKeys / 16; ++b) {
           const int bi = (t * kTcKeys + b * 16) / p.page_size;
-          if (bi < have_blocks && bt_global[first_block + bi] < 0) missing |= 1 << b;
+          if (bi >= have_blocks || bt_global[first_block + bi] < 0) missing |= 1 << b;      // (behind the request: masked anyway)
         }
       }
       const bool need_mask = key0 + kTcKeys - 1 > tile_pos0 || key0 < lo_raw[g] ||

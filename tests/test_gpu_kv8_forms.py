@@ -213,3 +213,40 @@ def test_a_captured_mixed_step(ops, split, dtype):
         between = call()
         torch.cuda.current_stream().wait_stream(side)
         assert torch.equal(out, first) and torch.equal(between, first)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("d,ps", [(64, 16), (64, 64), (128, 32)])
+@pytest.mark.parametrize("held", [0, 90, 640])
+def test_portions_whose_table_ends_before_their_positions(ops, held, d, ps, split, dtype):
+    """Positions behind the table's width have no page: they are not seen, whichever kernel runs, by parts of the keys too, and a row
+    that sees no other is zeros."""
+    nq, G, t, total = 4, 2, DTYPES[dtype], 1400
+    pool = Pool(ops, G, d, ps, [total], seed=3)
+    pool.append([total], values(total, G, d, seed=4, spread=1), dtype=t)
+    v, bad = pool.plain.read(pool.tables[0], total)
+    width = max(1, held // ps)
+    keys = width * ps if held else 0
+    narrow, wide = pool.table[:, :width].contiguous(), pool.table.clone()
+    wide[:, width:] = -1
+    if not held:
+        narrow, wide = torch.full_like(narrow, -1), torch.full_like(wide, -1)
+    for n, window in ((24, 0), (150, 0), (300, 0), (24, 33), (300, 900)):
+        q = torch.randn((n, nq * d), generator=torch.Generator().manual_seed(n)).to(t)
+        pos = torch.arange(total - n, total, dtype=torch.int32, device="cuda")
+        got = []
+        for table in (narrow, wide):
+            hints = Forced(ops, split_portions=split).hints_for([n], [total])
+            got.append(ops.paged_attention8(q.cuda(), pool.codes, pool.words, table, torch.zeros(n, dtype=torch.int32, device="cuda"), pos, nq, G, d, ps,
+                                            d ** -0.5, window=window, hints=hints))
+        assert torch.equal(*got)
+        mine = got[0].double().cpu().view(n, nq, d)
+        for i in range(0, n, 23):
+            first = max(0, total - n + i - window + 1) if window else 0
+            seen = slice(first, keys)
+            if first >= keys:
+                assert not mine[i].any()
+                continue
+            out, size, score = attend(q[i:i + 1].double().view(1, nq, d), v[seen], bad[seen], [keys - first - 1], d ** -0.5)
+            assert ((mine[i] - out[0]).abs() <= tolerance(t, out, size, score, d, total, torch.bfloat16)[0]).all()
