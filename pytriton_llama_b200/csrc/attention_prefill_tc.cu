@@ -669,6 +669,7 @@ static int prefill_attention_tc_entry(void* out, const void* q, const void* cach
   p.out_stride = out_stride; p.bt_stride = bt_stride; p.nq = nq; p.nkv = nkv; p.page_size = page_size;
   p.window = window; p.num_pages = num_pages; p.scale_log2 = scale * 1.4426950408889634f;
   p.splits = splits; p.split_tiles = split_tiles; p.part_acc = part_acc; p.part_ml = part_ml;
+  if (holes) p.scale_log2 = p.scale_log2 > 1e-37f ? p.scale_log2 : 1e-37f;      // an 8-bit cache's scale may be 0, and 0 times the -inf of a masked key is none
   if (holes)
     return d == 64 ? launch_prefill_tc<64, true>(q, cache, n_tiles, n_tokens, q_stride, nq, nkv, page_size, num_pages, p, as_stream(stream))
                    : launch_prefill_tc<128, true>(q, cache, n_tiles, n_tokens, q_stride, nq, nkv, page_size, num_pages, p, as_stream(stream));

@@ -993,7 +993,8 @@ class CudaOps:
                          hints=None) -> torch.Tensor:
         """``paged_attention`` over an 8-bit cache (``rope_kv8_write``).  q is [T, >= nq*d] (the q part of a qkv buffer is fine);
         returns [T, nq*d].  A token that was written with a number that is not finite gives NaN to the rows that see it and
-        to no other; a position without a page is not seen; a row without a request or without keys is zeros."""
+        to no other; a position without a page is not seen; a row without a request or without keys is zeros.  With ``scale`` 0 a
+        row is the mean of the values it sees."""
         device, i32 = self.device, torch.int32
         if not (q.is_contiguous() and q.device == device and block_table.dtype is i32 and block_table.is_contiguous() and block_table.device == device
                 and tok_req.dtype is i32 and tok_req.is_contiguous() and tok_req.device == device and positions.dtype is i32

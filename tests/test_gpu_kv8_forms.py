@@ -250,3 +250,38 @@ def test_portions_whose_table_ends_before_their_positions(ops, held, d, ps, spli
                 continue
             out, size, score = attend(q[i:i + 1].double().view(1, nq, d), v[seen], bad[seen], [keys - first - 1], d ** -0.5)
             assert ((mine[i] - out[0]).abs() <= tolerance(t, out, size, score, d, total, torch.bfloat16)[0]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("form", [{}, {"single_form": (0, 4)}, {"single_form": (4, 8)}, {"split_portions": True}, {"split_portions": False}],
+                         ids=["chosen", "units", "cluster", "mma", "tensor memory"])
+@pytest.mark.parametrize("nq,G,d,ps", [(4, 2, 64, 16), (3, 1, 128, 32), (5, 5, 48, 16)])
+def test_a_scale_of_zero_is_the_mean_of_the_values_in_sight(ops, nq, G, d, ps, form, dtype):
+    """Masked keys among them: 0 times their -inf is no number.  With a missing page and a window too."""
+    t, step = DTYPES[dtype], [(1, 700), (40, 600), (1, 3), (130, 0), (300, 5)]
+    lens = [n + c for n, c in step]
+    pool = Pool(ops, G, d, ps, lens, seed=d)
+    kv = [values(n, G, d, seed=i, spread=1) for i, n in enumerate(lens)]
+    pool.append(lens, torch.cat(kv), dtype=t)
+    table = pool.table.clone()
+    gone = {r: 0 if n < 3 * ps else 2 for r, n in enumerate(lens)}
+    for r, b in gone.items():
+        if b:
+            table[r, b] = -1
+    T = sum(n for n, _ in step)
+    q = torch.randn((T, nq * d), generator=torch.Generator().manual_seed(1)).to(t)
+    req = torch.cat([torch.full((n,), r) for r, (n, _) in enumerate(step)]).int()
+    pos = torch.cat([torch.arange(c, c + n) for n, c in step]).int()
+    for window in (0, 77):
+        hints = Forced(ops, **form).hints_for([n for n, _ in step], lens)
+        got = ops.paged_attention8(q.cuda(), pool.codes, pool.words, table, req.cuda(), pos.cuda(), nq, G, d, ps, 0.0, window=window, hints=hints)
+        at = 0
+        for r, (n, c) in enumerate(step):
+            v, bad = pool.plain.read(pool.tables[r], n + c)
+            for i in range(0, n, 13):
+                p = c + i
+                keys = [k for k in range(max(0, p - window + 1) if window else 0, p + 1) if not gone[r] or k // ps != gone[r]]
+                mine = got[at + i].double().cpu().view(nq, d)
+                out, size, score = attend(torch.zeros((1, nq, d), dtype=torch.float64), v[keys], bad[keys], [len(keys) - 1], 0.0)
+                assert ((mine - out[0]).abs() <= tolerance(t, out, size, score, d, n + c, torch.float16 if n == 1 else torch.bfloat16)[0]).all(), (r, i, window)
+            at += n
