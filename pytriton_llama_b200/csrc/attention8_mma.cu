@@ -798,7 +798,7 @@ template <int D, typename T>
 __global__ void __launch_bounds__(kA8JoinThreads)
 attention8_join_kernel(const A8Params p) {
   const int* tl = p.items + 4 * blockIdx.y;
-  const int first = __ldg(tl + 1), rows = __ldg(tl + 2);       // (inputs of the step)
+  const int first = __ldg(tl + 1), rows = __ldg(tl + 2);       // (the kernels before this one have waited for whoever wrote them)
   pdl_wait();
   pdl_launch_dependents();
   const int i = blockIdx.x * (kA8JoinThreads / (D / 4)) + threadIdx.x / (D / 4), col = threadIdx.x % (D / 4) * 4;

@@ -142,7 +142,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
   // Blocks are handed out with x running fastest: heads along x and pairs along y, last pair
   // first, start the pairs that see the most keys first on every SM (longest work first).
   const int pair = gridDim.y - 1 - blockIdx.y;
-  const int* tl = p.tiles + 8 * pair;
+  const int* tl = p.tiles + 8 * pair;                          // (an input of the step; HOLES: kv8_expand comes before and has waited for whoever wrote it)
   const int req = tl[0], tok0 = tl[1], pos0 = tl[3];
   const int rows_g[2] = {tl[2], tl[6]};                        // rows of tile A and of tile B (0: absent)
   if (rows_g[0] <= 0 && rows_g[1] <= 0) return;                // an empty pair (padding of a captured step): nothing to do, nothing allocated yet
@@ -690,7 +690,7 @@ namespace ptl {
 int attention8_join_bf16(void* out, const float* part_acc, const float* part_ml, const int* tiles, int n_tiles, int out_stride, int nq, int d, int splits,
                          void* stream);
 int kv8_expand_bf16(void* pages, int* table, const void* codes, const void* words, const int* block_table, const int* tiles, int n_tiles, int slots,
-                    int width, int nkv, int d, int page_size, int num_pages, int window, void* stream);
+                    int width, int nkv, int d, int page_size, int num_pages, int window, int early, void* stream);
 }  // namespace ptl
 
 // Portions over an 8-bit cache (kv8.cuh): the pages they see are made bfloat16 in `place` [slots * width + 1, 2, nkv, page_size, d], slots at least the
@@ -709,7 +709,7 @@ struct Prefill8Args {
   void* stream;
   int n_tiles, n_tokens, q_stride, out_stride, width, slots, nq, nkv, d, page_size, num_pages, window, splits, split_tiles;
   float scale;
-  int zero;
+  int early;                       // no kernel that is still under way writes tiles or block_table
 };
 static_assert(sizeof(Prefill8Args) == 12 * 8 + 16 * 4, "as it is packed");
 
@@ -719,7 +719,7 @@ PTL_EXPORT int ptl_attention8_prefill_tc_bf16(const void* args) {
   PTL_REQUIRE(a.splits >= 1 && a.splits <= 65535 && (a.splits == 1 || (a.part_acc && a.part_ml && ptl::aligned16(a.part_acc))),
               "prefill_attention_tc: splits > 1 need scratch buffers");
   if (int rc = ptl::kv8_expand_bf16(a.place, a.table, a.codes, a.words, a.block_table, a.tiles, a.n_tiles, a.slots, a.width, a.nkv, a.d, a.page_size,
-                                    a.num_pages, a.window, a.stream)) return rc;
+                                    a.num_pages, a.window, a.early, a.stream)) return rc;
   const int rc = prefill_attention_tc_entry(a.out, a.q, a.place, a.table, a.tiles, a.n_tiles, a.n_tokens, a.q_stride, a.out_stride, a.width, a.nq, a.nkv, a.d,
                                             a.page_size, a.scale, a.window, a.slots * a.width + 1, true, a.splits, a.split_tiles, a.part_acc, a.part_ml,
                                             a.status, a.stream);

@@ -39,7 +39,7 @@ struct Kv8WriteParams {
   const int* slots;
   unsigned char* codes;
   uint32_t* words;
-  int tokens, nq, nkv, d, rot, page_size, rows_per_block;
+  int tokens, nq, nkv, d, rot, page_size, rows_per_block, early;      // early: see the kernel
   long long num_slots;
 
   // The block of 16 positions that a row goes to, -1: none.
@@ -81,7 +81,9 @@ rope_kv8_write_kernel(const Kv8WriteParams p) {
   const int row_len = (p.nq + 2 * p.nkv) * d, half = p.rot / 2;
   const int t0 = blockIdx.x * p.rows_per_block, t1 = min(p.tokens, t0 + p.rows_per_block);
   T* qkv = static_cast<T*>(p.qkv);
-  // positions, slots and frequencies are inputs of the step, not results of the kernel before this one
+  // positions, slots and frequencies may be results of the kernel before this one, unless the caller says that they are not (a model's
+  // step, whose integers were there before its first kernel)
+  if (!p.early) pdl_wait();
   const int mine = p.block_of(t0 - 1 + lane);                  // (rows t0 - 1 .. t0 + 30)
   const int before = __shfl_up_sync(0xffffffffu, mine, 1);
   const unsigned leads = __ballot_sync(0xffffffffu, lane >= 1 && t0 - 1 + lane < t1 && mine >= 0 && mine != before) >> 1;      // bit i: row t0 + i begins a run
@@ -262,10 +264,9 @@ read_kv8_kernel(T* __restrict__ out, const unsigned char* __restrict__ codes, co
   const int r = blockIdx.y, pos0 = blockIdx.x * kKv8Block;
   const int t0 = r ? args.end[r - 1] : 0, tokens = min(kKv8Block, args.end[r] - t0 - pos0);
   if (tokens <= 0) return;
-  // (the table is an input, not a result of the kernel before this one)
-  const int page = __ldg(block_table + (size_t)(args.first_request + r) * bt_stride + pos0 / page_size), sub = pos0 % page_size / kKv8Block;
-  pdl_wait();
+  pdl_wait();                              // (the table may be a result of the kernel before this one)
   pdl_launch_dependents();
+  const int page = __ldg(block_table + (size_t)(args.first_request + r) * bt_stride + pos0 / page_size), sub = pos0 % page_size / kKv8Block;
   const bool here = page >= 0 && page < num_pages;           // (a position that has no page reads as 0)
   const unsigned per_row = d / 16, total = 2u * nkv * d;     // packets of a row, and of the 16 positions
   const unsigned char* src = codes + (size_t)(here ? page : 0) * 2 * nkv * page_size * d + (size_t)sub * kKv8Block * d;
@@ -315,14 +316,14 @@ struct Kv8ExpandParams {
   const uint32_t* words;
   const int* block_table;
   const int* tiles;
-  int pairs, slots, width, nkv, d, page_size, num_pages, window;
+  int pairs, slots, width, nkv, d, page_size, num_pages, window, early;      // early: as for a write
 };
 
 constexpr int kKv8ExpandChunk = kKv8Threads * kKv8ReadAhead;      // packets of a page a block takes
 
 __global__ void __launch_bounds__(kKv8Threads, 3)
 kv8_expand_kernel(const Kv8ExpandParams p) {
-  // tiles and the block table are inputs of the step, not results of the kernel before this one
+  if (!p.early) pdl_wait();                // (tiles and the block table)
   const int page_codes = 2 * p.nkv * p.page_size * p.d, lane = threadIdx.x & 31;
   const int pair = blockIdx.y, chunk = blockIdx.z * kKv8ExpandChunk;      // of the page's packets of 16 codes
   auto request = [&](int i) { return i >= 0 && i < p.pairs && __ldg(p.tiles + 8 * i + 2) > 0 ? __ldg(p.tiles + 8 * i) : -1; };
@@ -390,7 +391,7 @@ kv8_expand_kernel(const Kv8ExpandParams p) {
 
 template <typename T>
 static int rope_kv8_write(T* qkv, const int* positions, const float* inv_freq, const int* slots, void* codes, void* words, int tokens, int nq,
-                          int nkv, int d, int rot, int page_size, long long num_slots, void* stream) {
+                          int nkv, int d, int rot, int page_size, int early, long long num_slots, void* stream) {
   PTL_REQUIRE(tokens >= 0 && nq >= 0 && nkv > 0 && d > 0 && page_size > 0 && num_slots >= 0, "rope_kv8_write: bad sizes");
   PTL_REQUIRE(d % 16 == 0 && d <= 256, "rope_kv8_write: head size %d is no multiple of 16 up to 256", d);
   PTL_REQUIRE(nkv <= 65535, "rope_kv8_write: too many heads");
@@ -399,7 +400,7 @@ static int rope_kv8_write(T* qkv, const int* positions, const float* inv_freq, c
   PTL_REQUIRE(aligned16(qkv) && aligned16(codes), "rope_kv8_write: qkv and codes must be 16-byte aligned");
   if (tokens == 0) return 0;
   if (rot == 0) inv_freq = nullptr;
-  Kv8WriteParams p{qkv, positions, inv_freq, slots, (unsigned char*)codes, (uint32_t*)words, tokens, nq, nkv, d, rot, page_size, 1, num_slots};
+  Kv8WriteParams p{qkv, positions, inv_freq, slots, (unsigned char*)codes, (uint32_t*)words, tokens, nq, nkv, d, rot, page_size, 1, early, num_slots};
   // Steps of many rows are mostly prompts, whose runs are long: a block a row asks for every row's slot many times over there.  Written and read
   // back (before reading was faster), us, by one row and by 16 a block: 64 single tokens (8 heads of 64) 9.5 and 25.8; one prompt (8 heads of 128) of 500 8.7 and 9.0, of
   // 1,024 10.4 and 8.5, of 1,500 13.0 and 9.6.
@@ -456,7 +457,7 @@ static int read_kv8(T* out, const void* codes, const void* words, const int* blo
 
 // pages: bfloat16 [slots * width + 1, 2, nkv, page_size, d]; table: int32 [requests, width]; slots: at least the requests with portions.
 int kv8_expand_bf16(void* pages, int* table, const void* codes, const void* words, const int* block_table, const int* tiles, int n_tiles, int slots,
-                    int width, int nkv, int d, int page_size, int num_pages, int window, void* stream) {
+                    int width, int nkv, int d, int page_size, int num_pages, int window, int early, void* stream) {
   PTL_REQUIRE(n_tiles >= 0 && n_tiles % 2 == 0 && slots > 0 && width > 0 && nkv > 0 && page_size > 0 && num_pages > 0, "kv8_expand: bad sizes");
   PTL_REQUIRE(d % 16 == 0 && d > 0 && page_size % kKv8Block == 0, "kv8_expand: head size %d and pages of %d must be multiples of 16", d, page_size);
   PTL_REQUIRE(aligned16(pages) && aligned16(codes) && (reinterpret_cast<uintptr_t>(words) & 7u) == 0 && n_tiles / 2 <= 65535, "kv8_expand: alignment");
@@ -465,7 +466,7 @@ int kv8_expand_bf16(void* pages, int* table, const void* codes, const void* word
   PTL_REQUIRE(chunks <= 65535, "kv8_expand: pages are too large");
   return launch_kernel("kv8_expand", kv8_expand_kernel, dim3(x, n_tiles / 2, chunks), dim3(kKv8Threads), 0, as_stream(stream),
                        Kv8ExpandParams{(__nv_bfloat16*)pages, table, (const unsigned char*)codes, (const uint32_t*)words, block_table, tiles,
-                                       n_tiles / 2, slots, width, nkv, d, page_size, num_pages, window});
+                                       n_tiles / 2, slots, width, nkv, d, page_size, num_pages, window, early});
 }
 
 }  // namespace ptl
@@ -490,15 +491,18 @@ struct Kv8ReadCall {
 };
 static_assert(sizeof(Kv8ReadCall) == 6 * 8 + 6 * 4, "as it is packed");
 
-// See the top of the file.  `inv_freq` null or `rot` 0: nothing is turned.  A slot that is negative or not below num_slots is not written.  `lengths` is a host
-// array.
-#define PTL_KV8_ENTRIES(NAME, T)                                                                                                          \
+// See the top of the file.  `inv_freq` null or `rot` 0: nothing is turned.  A slot that is negative or not below num_slots is not written.  The second entry
+// is for callers whose positions, inv_freq and slots no kernel that is still under way writes.  `lengths` is a host array.
+#define PTL_KV8_WRITE_ENTRY(NAME, T, EARLY)                                                                                               \
   PTL_EXPORT int ptl_rope_kv8_write_##NAME(const void* args) {                                                                            \
     Kv8WriteArgs a;                                                                                                                       \
     memcpy(&a, args, sizeof a);                                                                                                           \
     return ptl::rope_kv8_write<T>((T*)a.qkv, a.positions, a.inv_freq, a.slots, a.codes, a.words, a.tokens, a.nq, a.nkv, a.d, a.rot,        \
-                                  a.page_size, a.num_slots, a.stream);                                                                    \
-  }                                                                                                                                       \
+                                  a.page_size, EARLY, a.num_slots, a.stream);                                                             \
+  }
+#define PTL_KV8_ENTRIES(NAME, T)                                                                                                          \
+  PTL_KV8_WRITE_ENTRY(NAME, T, 0)                                                                                                         \
+  PTL_KV8_WRITE_ENTRY(early_##NAME, T, 1)                                                                                                 \
   PTL_EXPORT int ptl_read_kv8_##NAME(const void* args) {                                                                                  \
     Kv8ReadCall a;                                                                                                                        \
     memcpy(&a, args, sizeof a);                                                                                                           \

@@ -94,7 +94,7 @@ _SIGNATURES = {
     "ptl_moe_grouped": [_ptr, _c_int, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f, _c_f, _c_f, _ptr],
     "ptl_moe_combine_norm": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_f, _ptr],
     "ptl_moe_combine": [_ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _ptr],
-    "ptl_rope_kv8_write": [ctypes.c_char_p], "ptl_read_kv8": [ctypes.c_char_p],
+    "ptl_rope_kv8_write": [ctypes.c_char_p], "ptl_rope_kv8_write_early": [ctypes.c_char_p], "ptl_read_kv8": [ctypes.c_char_p],
     "ptl_attention8_single": [ctypes.c_char_p], "ptl_attention8_portion": [ctypes.c_char_p],
     "ptl_attention8_simt": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                             _c_int, _c_f, _c_int, _c_int, _c_int, _ptr],
@@ -958,7 +958,7 @@ class CudaOps:
             self._want(inv_freq, "inv_freq", torch.float32)
             if inv_freq.numel() < rot // 2:
                 raise KernelError("inv_freq shorter than half the rotary width")
-        fn = getattr(self.lib, "ptl_rope_kv8_write" + _suffix(qkv.dtype))
+        fn = getattr(self.lib, ("ptl_rope_kv8_write_early" if self._in_forward() else "ptl_rope_kv8_write") + _suffix(qkv.dtype))
         self._check(fn(self._KV8_WRITE_ARGS.pack(
             qkv.data_ptr(), positions.data_ptr(), 0 if inv_freq is None else inv_freq.data_ptr(), slots.data_ptr(), codes.data_ptr(), words.data_ptr(),
             self._stream(), pages * page_size, rows, nq, nkv, d, rot, page_size)), kernels=1 if rows else 0)
@@ -1156,7 +1156,7 @@ class CudaOps:
         self._check(self.lib.ptl_attention8_prefill_tc_bf16(self._PREFILL8_ARGS.pack(
             out.data_ptr(), q.data_ptr(), place.data_ptr(), table.data_ptr(), codes.data_ptr(), words.data_ptr(), block_table.data_ptr(),
             tiles.tensor.data_ptr(), part_acc, part_ml, self._tc_status_word().data_ptr(), stream, tiles.items, q.shape[0], stride, nq * d, width, slots, nq,
-            nkv, d, page_size, pages, window, splits, split_tiles, scale, 0)),
+            nkv, d, page_size, pages, window, splits, split_tiles, scale, self._in_forward())),
                     kernels=3 if splits > 1 else 2)
         return True
 
@@ -1288,6 +1288,11 @@ class CudaOps:
         """Called at the end of every forward pass: calls outside of one work their tables and units out themselves.  One kept from
         such a call to the next would be missing from a graph that captures the second of them."""
         self._rope_memo = self._pair_memo = self._units_memo = self._units8_memo = None
+
+    def _in_forward(self) -> int:
+        """1 inside of a forward pass: the step's integers were copied to the device before its first kernel, so that kernels may read them before they
+        have waited for the one before them."""
+        return int(getattr(self, "_rope_memo", None) is not None)
 
     def _pair_angles(self, positions: torch.Tensor, freq: torch.Tensor, dims: int, amplitude: float) -> torch.Tensor:
         """(cos, sin) [tokens, dims/2, 2] of position * freq, worked out once per forward pass and stream for every table of

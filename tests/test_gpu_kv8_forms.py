@@ -285,3 +285,42 @@ def test_a_scale_of_zero_is_the_mean_of_the_values_in_sight(ops, nq, G, d, ps, f
                 out, size, score = attend(torch.zeros((1, nq, d), dtype=torch.float64), v[keys], bad[keys], [len(keys) - 1], 0.0)
                 assert ((mine - out[0]).abs() <= tolerance(t, out, size, score, d, n + c, torch.float16 if n == 1 else torch.bfloat16)[0]).all(), (r, i, window)
             at += n
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("split", [False, True])
+def test_integers_worked_out_on_the_device_right_before_the_call(ops, split, dtype):
+    """Slots, positions, table and tiles are results of the kernel before: the same as with integers that were there long ago."""
+    nq, G, d, ps, t, total = 4, 2, 64, 16, DTYPES[dtype], 700
+    forced = Forced(ops, split_portions=split)
+    pool = Pool(ops, G, d, ps, [total], seed=3)
+    kv = values(total, G, d, seed=4, spread=1)
+    q = torch.randn((total, nq * d), generator=torch.Generator().manual_seed(1))
+    f = (1.0 / 10000 ** (torch.arange(0, d, 2) / d)).cuda()
+    qkv, slots, pos = pool.append([total], kv, nq=nq, q=q, inv_freq=f, rot=d, dtype=t)
+    hints = forced.hints_for([total], [total])
+    where = torch.zeros(total, dtype=torch.int32, device="cuda"), torch.tensor(pos, dtype=torch.int32, device="cuda")
+    args = (nq, G, d, ps, d ** -0.5)
+    first = ops.paged_attention8(qkv, pool.codes, pool.words, pool.table, *where, *args, hints=hints)
+    held = ops.read_kv8(pool.codes, pool.words, pool.table, [total], t)
+    codes, words = torch.zeros_like(pool.codes), torch.zeros_like(pool.words)
+    ints = {k: torch.zeros_like(v) for k, v in dict(pos=where[1], slots=where[1], table=pool.table, f=f.int()).items()}
+    f_new = torch.zeros_like(f)
+    tiles = hints.work["prefill_tiles"].tensor
+    right = tiles.clone()
+    slots = torch.tensor(slots, dtype=torch.int32, device="cuda")
+    for _ in range(10):
+        again = torch.cat([q, kv.reshape(total, -1)], 1).to(t).cuda()
+        for x in (codes, words, f_new, tiles, *ints.values()):
+            x.zero_()
+        torch.add(where[1], 0, out=ints["pos"])
+        torch.mul(f, 1, out=f_new)
+        torch.add(slots, 0, out=ints["slots"])
+        ops.rope_kv8_write(again, ints["pos"], f_new, d, ints["slots"], codes, words, *args[:4])
+        torch.add(pool.table, 0, out=ints["table"])
+        assert torch.equal(ops.read_kv8(codes, words, ints["table"], [total], t), held)
+        ints["table"].zero_()
+        torch.add(right, 0, out=tiles)
+        torch.add(pool.table, 0, out=ints["table"])
+        out = ops.paged_attention8(again, codes, words, ints["table"], where[0], ints["pos"], *args, hints=hints)
+        assert torch.equal(out, first) and torch.equal(again, qkv)

@@ -67,3 +67,16 @@ def test_dependents_start_behind_the_wait_on_the_predecessor(source, name, body)
         around = _blocks_around(body, launch.start())
         waits = [_blocks_around(body, w.start()) for w in re.finditer(r"(?<=[;{}])\s*pdl_wait\(\);", body[:launch.start()])]
         assert any(w == around[:len(w)] for w in waits), f"{source}: {name}"
+
+
+@pytest.mark.parametrize("name,reads", [("rope_kv8_write_kernel", ["p.block_of(", "p.angle(", "p.slots"]), ("read_kv8_kernel", ["block_table"]),
+                                        ("kv8_expand_kernel", ["p.tiles", "p.block_table"])])
+def test_integers_of_an_8_bit_cache_are_read_behind_a_wait(name, reads):
+    """Slots, tables and tiles may come from the kernel directly before the call; only a caller that says otherwise (``early``) has them read
+    ahead of the wait."""
+    body = next(b for _, n, b in KERNELS if n == name)
+    first_wait = re.search(r"(?:if \(!p\.early\) )?pdl_wait\(\);", body).start()
+    for array in reads:
+        assert array in body and first_wait < body.index(array), (name, array)
+    if "p.early" in body:        # and what the kernel before this one computed is read behind a wait that every caller has
+        assert re.search(r"(?<=[;{}])\s*pdl_wait\(\);\s*pdl_launch_dependents\(\);", body)

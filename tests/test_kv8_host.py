@@ -1,0 +1,48 @@
+"""What the operators of an 8-bit cache tell their kernels, read from the packed arguments; no kernel runs."""
+import pytest
+import torch
+
+from pytriton_llama_b200.ops.cuda import CudaOps
+
+I32, BF = torch.int32, torch.bfloat16
+
+
+class Library:
+    """Keeps what an entry was called with."""
+
+    def __init__(self):
+        self.calls = {}
+
+    def __getattr__(self, name):
+        def entry(packed):
+            self.calls[name] = packed
+            return 0
+        return entry
+
+
+@pytest.fixture()
+def ops():
+    o = CudaOps.__new__(CudaOps)
+    o.device, o.lib, o._raw_stream, o._device_index, o.launches, o._sm_count = torch.device("cpu"), Library(), lambda i: 0, 0, 0, 148
+    o._tc_status_word = lambda: torch.zeros(1, dtype=I32)
+    return o
+
+
+def test_integers_are_read_early_inside_of_a_forward_pass_only(ops):
+    """There the step's integers came before its first kernel; elsewhere they may come from the kernel before."""
+    codes, words = torch.zeros((9, 2, 2, 16, 64), dtype=torch.uint8), torch.zeros((9, 2, 1, 2), dtype=I32)
+
+    def early():
+        ops.lib.calls.clear()
+        ops.rope_kv8_write(torch.zeros((3, 512), dtype=BF), torch.zeros(3, dtype=I32), torch.zeros(32), 64, torch.zeros(3, dtype=I32), codes, words, 4, 2, 64, 16)
+        write = int("ptl_rope_kv8_write_early_bf16" in ops.lib.calls)
+        hints = ops.hints_for([20], [100])
+        hints.split_portions = False
+        ops.paged_attention8(torch.zeros((20, 256), dtype=BF), codes, words, torch.zeros((1, 7), dtype=I32), torch.zeros(20, dtype=I32),
+                             torch.arange(80, 100, dtype=I32), 4, 2, 64, 16, 0.125, hints=hints)
+        return write, ops._PREFILL8_ARGS.unpack(ops.lib.calls["ptl_attention8_prefill_tc_bf16"])[-1]
+    assert early() == (0, 0)
+    ops.begin_forward()
+    assert early() == (1, 1)
+    ops.end_forward()
+    assert early() == (0, 0)
