@@ -80,3 +80,17 @@ def test_integers_of_an_8_bit_cache_are_read_behind_a_wait(name, reads):
         assert array in body and first_wait < body.index(array), (name, array)
     if "p.early" in body:        # and what the kernel before this one computed is read behind a wait that every caller has
         assert re.search(r"(?<=[;{}])\s*pdl_wait\(\);\s*pdl_launch_dependents\(\);", body)
+
+
+@pytest.mark.parametrize("name", ["prefill_attention_tc_kernel", "rope_kv8_write_kernel"])
+def test_blocks_without_work_wait_too(name):
+    """A kernel whose blocks all left without a wait would be through before its predecessor, and the kernel after it, which waits for this
+    one only, would run beside what it counts on: a return ahead of the wait that every block with work has stands behind one of its own."""
+    body = next(b for _, n, b in KERNELS if n == name)
+    main = re.search(r"(?<=[;{}])\s*pdl_wait\(\);\s*pdl_launch_dependents\(\);\s*(?:__syncthreads|const)", body).start()
+    inside = lambda at: re.search(r"\[&\]\([^)]*\)\s*$", body[:_blocks_around(body, at)[-1]])        # of a function of the kernel's own
+    left = [m.start() for m in re.finditer(r"\breturn;", body[:main]) if "blockIdx" in body[:m.start()] and not inside(m.start())]
+    assert left
+    for at in left:
+        around = _blocks_around(body, at)
+        assert any(_blocks_around(body, w.start()) == around for w in re.finditer(r"(?<=[;{}])\s*pdl_wait\(\);", body[:at])), body[at - 200:at]
