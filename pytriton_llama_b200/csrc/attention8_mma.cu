@@ -427,9 +427,10 @@ template <int D, int NT, int WARPS> struct A8Single {
 // length (the list of attention8_units_kernel), in the block that ends last.  Every warp fetches its own keys, kRing blocks ahead.  Eight warps
 // halve the turns; four leave more blocks side by side (the choice and its figures: CudaOps._kv8_single_form).
 //
-// What bounds it: the instructions that make operands out of codes (two a pair of codes), and their latencies: 0.53 of the issue slots at 24 % of
-// the warps an SM holds, tensor pipe 0.11.  32 heads over 8, bfloat16: one token of 4,000 7.8 us (bytes: 0.64), 64 of 256 to 2,560 27.4
-// (14.4; 3.4 TB/s), eight of 20,011 to 30,011 with heads of 128 84 (64; 4.9 TB/s); float32, eight of 1,000 to 4,096 16.8 (3.3).  Fewer
+// What bounds it: instructions and their latencies, 0.53 of the issue slots at 24 % of the warps an SM holds, tensor pipe 0.11.  A turn has about
+// 410, of which 144 make operands out of codes (two a pair of codes), and a warp 1,400 outside of its turns: its query, its tables, the join.  32 heads
+// over 8, bfloat16: one token of 4,000 7.8 us (bytes: 0.64; two turns a warp), 64 of 256 to 2,560 27.4 (14.4; 3.4 TB/s; six turns on average), eight of
+// 20,011 to 30,011 with heads of 128 84 (64; 4.9 TB/s); float32, eight of 1,000 to 4,096 16.8 (3.3; up to eight turns of twice the products).  Fewer
 // registers for half as many blocks more were slower everywhere (64 tokens 33.5 us: 80 registers, spills).
 template <int D, typename T, int NT, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, NT == 1 && sizeof(T) == 2 && WARPS == 4 ? (D == 64 ? 4 : 3) : 1)

@@ -9,10 +9,14 @@
 // of many rows, at 16, and takes the runs that begin there.
 //
 // What bounds it: three loads that wait for one another (slots, then the run's values and the word, then, where the exponent grows, the codes) and
-// the launch; one rounding a code, by fma.rd.  Four prompts of 301 to 1,021 tokens (8 heads of 128) are written and read back in 13.0 us,
-// of which the bytes take 5.2; 64 single tokens in 8.0 of 1.5.  Five blocks an SM (up to 96 registers) where the compiler would take 128: 2,644
-// rows are one wave of blocks (by three, four, five and six an SM 14.9, 14.7, 13.0 and 13.6 us).  Reading back and making pages bfloat16 are given up to 80
-// registers, so that a thread's four packets are asked for at once (the compiler keeps to 64: 9.4 and 15.4 us).
+// the launch; one rounding a code, by fma.rd.  Four prompts of 301 to 1,021 tokens (8 heads of 128) are written and read back in 13.2 us,
+// of which the bytes take 5.2; 64 single tokens in 8.2 of 1.5.  That is without turning; a model's step turns q and k.  With 32 query heads of 64
+// and 128, bfloat16: 8 tokens 4.4 and 5.7 us, 64 4.6 and 5.9, the four prompts 36 and 75, 8,000 tokens 89 and 192.  There q bounds it, turned in place an
+// element at a time (8,000 tokens without q 26 and 58), and a write into the other cache, two elements at a time, takes 24 and 43.
+// Five blocks an SM (up to 96 registers): over steps of 8 to 8,000 rows, heads of 64 and 128, both types, turned and not, it is on average within
+// 2 to 10 % of the best of three to six for each instance; three is 3 to 24 % off, four 6 to 18, six 0 to 9 and for float32 heads of 128, unturned, which
+// then spill, 28.  (With five the heads of 128 spill 16 to 28 bytes, but bfloat16 unturned.)  Reading back and making pages bfloat16 are
+// given up to 80 registers, so that a thread's four packets are asked for at once (the compiler keeps to 64: 9.4 and 15.4 us).
 #include "kv8.cuh"
 #include <cstring>
 

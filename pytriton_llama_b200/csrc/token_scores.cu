@@ -16,7 +16,7 @@
 //
 // What bounds it: the bytes where no alternatives are asked for (500 rows of 128,256: 42.8 us, 6.0 TB/s); with 20 of them 49.6, the turns that have
 // logits above the threshold and the ranking at the end; 8 rows with five 9.3 us, a cluster of eight blocks a row, of which the bytes
-// take 0.64: its start, two turns of loads, the ranking and two cluster barriers.
+// take 0.64: its start, four turns of loads with a threshold in the first and the fourth, the ranking and two cluster barriers.
 //
 // Logits of -inf have no probability.  A row with a NaN, with +inf, or with -inf only has no distribution: its
 // log-probabilities and its entropy are NaN.  Its alternatives are the largest logits all the same, NaN behind all others.

@@ -994,7 +994,8 @@ class CudaOps:
         """``paged_attention`` over an 8-bit cache (``rope_kv8_write``).  q is [T, >= nq*d] (the q part of a qkv buffer is fine);
         returns [T, nq*d].  A token that was written with a number that is not finite gives NaN to the rows that see it and
         to no other; a position without a page is not seen; a row without a request or without keys is zeros.  With ``scale`` 0 a
-        row is the mean of the values it sees."""
+        row is the mean of the values it sees.  Weights are summed in units in which one is up to 2^15: values whose magnitude times 2^15
+        times the keys is beyond float32 may give infinities."""
         device, i32 = self.device, torch.int32
         if not (q.is_contiguous() and q.device == device and block_table.dtype is i32 and block_table.is_contiguous() and block_table.device == device
                 and tok_req.dtype is i32 and tok_req.is_contiguous() and tok_req.device == device and positions.dtype is i32
@@ -1228,8 +1229,8 @@ class CudaOps:
     # ------------------------------------------------------------------ pages
     def copy_pages(self, tensors, src, dst) -> None:
         """tensor[dst[i]] = tensor[src[i]] for every i and every one of ``tensors`` (any types, rows of any size, at least as many
-        rows as the largest index says), in one launch.  ``src`` and ``dst`` are host integers; no row is written twice, and none that is
-        read is written."""
+        rows as the largest index says), in one launch for up to 128 tensors and 3,700 pairs.  ``src`` and ``dst`` are host integers; no
+        row is written twice, and none that is read is written."""
         if not isinstance(src, list) or not isinstance(dst, list):
             src, dst = (np.asarray(x, dtype=np.int64).reshape(-1).tolist() for x in (src, dst))
         n = len(src)
