@@ -166,3 +166,31 @@ def test_mixed_steps_are_captured_after_any_number_of_resizes(model_folders):
         assert any(isinstance(k, tuple) for k in eng._graphs)
         eng.resize_cache(60 + i)
     eng.check_device_status()
+
+
+@pytest.mark.parametrize("bits", [None, 8])
+def test_a_resize_that_finds_no_memory_half_way(model_folders, bits):
+    """The first cache entry's new pages fit, the second's do not: requests go on as if nothing had been asked for, captured steps among them."""
+    folder = model_folders("D", torch.bfloat16)
+    outs = []
+    for resize in (False, True):
+        llm = LLM(folder, _config("D", "bfloat16", compiled_model=True, cache_bits=bits))
+        cache = llm.engine.cache
+        reqs = [llm.add_request(random_tokens(40, TINY["D"]["vocab_size"], i), SamplingParams(temperature=0.0, max_gen_len=60)) for i in range(4)]
+        for i, _ in enumerate(llm.run()):
+            if resize and i in (10, 30):
+                pages = 1 << 18
+                one = pages * cache.groups[0].kv[0][0].nbytes
+                torch.cuda.empty_cache()
+                total = torch.cuda.get_device_properties(0).total_memory
+                torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved(0) + 1.5 * one) / total, 0)
+                try:
+                    with pytest.raises(torch.OutOfMemoryError):
+                        llm.engine.resize_cache(pages)
+                finally:
+                    torch.cuda.set_per_process_memory_fraction(1.0, 0)
+                assert cache.groups[0].pool.num_pages == 120 and {t.shape[0] for t in cache.groups[0].page_tensors()} == {120}
+        cache.check_invariants()
+        llm.engine.check_device_status()
+        outs.append([r.output for r in reqs])
+    assert outs[0] == outs[1]
