@@ -377,7 +377,8 @@ kv8_expand_kernel(const Kv8ExpandParams p) {
     for (int k = 0; k < kKv8ReadAhead; ++k) {
       const int i = chunk + k * kKv8Threads + threadIdx.x, row = i / per_row, part = row / (p.nkv * p.page_size), off = row % p.page_size;
       if (!here || i >= page_codes / 16) continue;
-      const float step = 2.0f * kv8_half_step((part ? w[k].y : w[k].x) & 255u);
+      // (no value has exponent 255, but a block that nothing was written to may: its keys are masked, its values are multiplied by 0 and so must be numbers)
+      const float step = 2.0f * kv8_half_step(min(254u, (part ? w[k].y : w[k].x) & 255u));
       const bool marked = part == 0 && (((w[k].x | w[k].y) >> (16 + off % kKv8Block)) & 1u);
       uint32_t out[8];
 #pragma unroll

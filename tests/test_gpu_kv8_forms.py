@@ -324,3 +324,30 @@ def test_integers_worked_out_on_the_device_right_before_the_call(ops, split, dty
         torch.add(pool.table, 0, out=ints["table"])
         out = ops.paged_attention8(again, codes, words, ints["table"], where[0], ints["pos"], *args, hints=hints)
         assert torch.equal(out, first) and torch.equal(again, qkv)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("form", [{}, {"single_form": (0, 4)}, {"single_form": (4, 8)}, {"split_portions": True}, {"split_portions": False}],
+                         ids=["chosen", "units", "cluster", "mma", "tensor memory"])
+@pytest.mark.parametrize("nq,G,d,ps", [(4, 2, 64, 32), (8, 1, 128, 64), (3, 3, 64, 128), (5, 5, 48, 48)])
+def test_what_memory_held_before_reaches_no_row(ops, nq, G, d, ps, form, dtype):
+    """Words and codes of blocks that no token was written to, in pages that the last tokens lie in: exponents that no value has, marks, and codes at both
+    ends.  What comes out is the same as over zeros."""
+    t, step = DTYPES[dtype], [(1, 700), (13, 825), (40, 600), (1, 3), (256, 4), (3, 0)]
+    lens = [n + c for n, c in step]
+    T = sum(n for n, _ in step)
+    kv = torch.cat([values(n, G, d, seed=i, spread=1) for i, n in enumerate(lens)])
+    q = torch.randn((T, nq * d), generator=torch.Generator().manual_seed(1)).to(t).cuda()
+    req = torch.cat([torch.full((n,), r) for r, (n, _) in enumerate(step)]).int().cuda()
+    pos = torch.cat([torch.arange(c, c + n) for n, c in step]).int().cuda()
+    got = []
+    for word, code in ((0, 0), (-1, 255), (-1, 0), (255, 255), (254, 0)):
+        pool = Pool(ops, G, d, ps, lens, seed=5)
+        pool.words.fill_(word)
+        pool.codes.fill_(code)
+        pool.append(lens, kv, dtype=t)
+        hints = Forced(ops, **form).hints_for([n for n, _ in step], lens)
+        got.append(ops.paged_attention8(q, pool.codes, pool.words, pool.table, req, pos, nq, G, d, ps, d ** -0.5, hints=hints))
+    assert torch.isfinite(got[0]).all()
+    for other in got[1:]:
+        assert torch.equal(other, got[0])
