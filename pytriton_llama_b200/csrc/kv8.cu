@@ -377,8 +377,10 @@ kv8_expand_kernel(const Kv8ExpandParams p) {
     for (int k = 0; k < kKv8ReadAhead; ++k) {
       const int i = chunk + k * kKv8Threads + threadIdx.x, row = i / per_row, part = row / (p.nkv * p.page_size), off = row % p.page_size;
       if (!here || i >= page_codes / 16) continue;
-      // (no value has exponent 255, but a block that nothing was written to may: its keys are masked, its values are multiplied by 0 and so must be numbers)
-      const float step = 2.0f * kv8_half_step(min(254u, (part ? w[k].y : w[k].x) & 255u));
+      // Values' exponents are 0 or 16 to 254.  A block that nothing was written to may say what it likes: its keys are masked, but its values are
+      // multiplied by 0 and so must be numbers.
+      const int e = min(254, (int)((part ? w[k].y : w[k].x) & 255u));
+      const float step = 2.0f * kv8_half_step(e < kKv8MinExponent ? 0 : e);
       const bool marked = part == 0 && (((w[k].x | w[k].y) >> (16 + off % kKv8Block)) & 1u);
       uint32_t out[8];
 #pragma unroll

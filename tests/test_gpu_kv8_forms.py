@@ -341,7 +341,7 @@ def test_what_memory_held_before_reaches_no_row(ops, nq, G, d, ps, form, dtype):
     req = torch.cat([torch.full((n,), r) for r, (n, _) in enumerate(step)]).int().cuda()
     pos = torch.cat([torch.arange(c, c + n) for n, c in step]).int().cuda()
     got = []
-    for word, code in ((0, 0), (-1, 255), (-1, 0), (255, 255), (254, 0)):
+    for word, code in ((0, 0), (-1, 255), (-1, 0), (255, 255), (254, 0), (1, 255), (4, 0), (6, 255), (7, 0), (15, 255), (16, 0)):
         pool = Pool(ops, G, d, ps, lens, seed=5)
         pool.words.fill_(word)
         pool.codes.fill_(code)
