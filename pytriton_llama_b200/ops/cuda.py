@@ -994,8 +994,8 @@ class CudaOps:
         """``paged_attention`` over an 8-bit cache (``rope_kv8_write``).  q is [T, >= nq*d] (the q part of a qkv buffer is fine);
         returns [T, nq*d].  A token that was written with a number that is not finite gives NaN to the rows that see it and
         to no other; a position without a page is not seen; a row without a request or without keys is zeros.  With ``scale`` 0 a
-        row is the mean of the values it sees.  Weights are summed in units in which one is up to 2^15: values whose magnitude times 2^15
-        times the keys is beyond float32 may give infinities."""
+        row is the mean of the values it sees.  Weights are summed in units in which one is up to 2^15: values whose magnitude times 2^15 times
+        the keys is beyond float32 may give infinities."""
         device, i32 = self.device, torch.int32
         if not (q.is_contiguous() and q.device == device and block_table.dtype is i32 and block_table.is_contiguous() and block_table.device == device
                 and tok_req.dtype is i32 and tok_req.is_contiguous() and tok_req.device == device and positions.dtype is i32
@@ -1015,11 +1015,17 @@ class CudaOps:
             raise KernelError(f"paged_attention8: a window of {window} positions")
         if not 0 <= scale < math.inf:
             raise KernelError(f"paged_attention8: scores times {scale}")
+        work = getattr(hints, "work", None)
+        if work and getattr(hints, "host_lengths_exact", False):
+            listed = getattr(hints, "listed_rows", None)
+            if listed is None:
+                listed = hints.listed_rows = sum(hints.q_lens)
+            if listed > tokens or len(hints.q_lens) > width[0]:
+                raise KernelError(f"paged_attention8: the step's lists are of {listed} rows of {len(hints.q_lens)} requests, q has {tokens} rows, the table {width[0]}")
         out = q.new_empty(tokens, nq * d)                    # (numbers take the host half the time that a tuple does)
         longest = getattr(hints, "max_ctx_len", 0) or width[1] * page_size
         if window:
             longest = min(longest, window)
-        work = getattr(hints, "work", None)
         if work and (d == 64 or d == 128) and nq // nkv <= 16 and shape[1] % 8 == 0:
             dec, tiles = work.get("decode_items"), work.get("prefill_tiles")
             if dec is not None and tiles is not None and self._attention8_tensor_cores(

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from pytriton_llama_b200.ops.cuda import CudaOps
+from pytriton_llama_b200.ops.cuda import CudaOps, KernelError
 
 I32, BF = torch.int32, torch.bfloat16
 
@@ -46,3 +46,21 @@ def test_integers_are_read_early_inside_of_a_forward_pass_only(ops):
     assert early() == (1, 1)
     ops.end_forward()
     assert early() == (0, 0)
+
+
+def attend(ops, tokens, q_lens, requests=2, **forms):
+    codes, words = torch.zeros((9, 2, 2, 16, 64), dtype=torch.uint8), torch.zeros((9, 2, 1, 2), dtype=I32)
+    hints = ops.hints_for(q_lens, [n + 30 for n in q_lens])
+    for name, value in forms.items():
+        setattr(hints, name, value)
+    return ops.paged_attention8(torch.zeros((tokens, 256), dtype=BF), codes, words, torch.zeros((requests, 4), dtype=I32), torch.zeros(tokens, dtype=I32),
+                                torch.zeros(tokens, dtype=I32), 4, 2, 64, 16, 0.125, hints=hints)
+
+
+@pytest.mark.parametrize("q_lens,requests", [([1, 4], 2), ([6], 2), ([1, 1, 1], 2)])
+def test_lists_of_more_rows_or_requests_than_there_are_are_refused(ops, q_lens, requests):
+    """The kernels go by the lists: they would write behind the output, or read behind the table."""
+    with pytest.raises(KernelError, match="the step's lists are of"):
+        attend(ops, 4, q_lens, requests)
+    assert not ops.lib.calls
+
