@@ -993,8 +993,9 @@ class CudaOps:
                          hints=None) -> torch.Tensor:
         """``paged_attention`` over an 8-bit cache (``rope_kv8_write``).  q is [T, >= nq*d] (the q part of a qkv buffer is fine);
         returns [T, nq*d].  A token that was written with a number that is not finite gives NaN to the rows that see it and
-        to no other; a position without a page is not seen; a row without a request or without keys is zeros.  With ``scale`` 0 a
-        row is the mean of the values it sees.  Weights are summed in units in which one is up to 2^15: values whose magnitude times 2^15 times
+        to no other; a position without a page is not seen; a row without a request or without keys is zeros (but for a captured step's
+        padding, which nothing reads: rows that the lists of ``hints`` do not name are left unwritten there).  With ``scale`` 0 a row is
+        the mean of the values it sees.  Weights are summed in units in which one is up to 2^15: values whose magnitude times 2^15 times
         the keys is beyond float32 may give infinities."""
         device, i32 = self.device, torch.int32
         if not (q.is_contiguous() and q.device == device and block_table.dtype is i32 and block_table.is_contiguous() and block_table.device == device
@@ -1016,13 +1017,15 @@ class CudaOps:
         if not 0 <= scale < math.inf:
             raise KernelError(f"paged_attention8: scores times {scale}")
         work = getattr(hints, "work", None)
+        listed = tokens                                      # rows that the step's lists name, where the host knows it
         if work and getattr(hints, "host_lengths_exact", False):
             listed = getattr(hints, "listed_rows", None)
             if listed is None:
                 listed = hints.listed_rows = sum(hints.q_lens)
             if listed > tokens or len(hints.q_lens) > width[0]:
                 raise KernelError(f"paged_attention8: the step's lists are of {listed} rows of {len(hints.q_lens)} requests, q has {tokens} rows, the table {width[0]}")
-        out = q.new_empty(tokens, nq * d)                    # (numbers take the host half the time that a tuple does)
+        # (numbers take the host half the time that a tuple does)
+        out = q.new_empty(tokens, nq * d) if listed == tokens else q.new_zeros(tokens, nq * d)
         longest = getattr(hints, "max_ctx_len", 0) or width[1] * page_size
         if window:
             longest = min(longest, window)

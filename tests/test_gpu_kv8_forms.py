@@ -351,3 +351,14 @@ def test_what_memory_held_before_reaches_no_row(ops, nq, G, d, ps, form, dtype):
     assert torch.isfinite(got[0]).all()
     for other in got[1:]:
         assert torch.equal(other, got[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("form", [{}, {"single_form": (0, 4)}, {"single_form": (4, 8)}, {"split_portions": True}, {"split_portions": False}],
+                         ids=["chosen", "units", "cluster", "mma", "tensor memory"])
+@pytest.mark.parametrize("step", [[(1, 300)], [(40, 300)], [(1, 300), (40, 600), (1, 3), (300, 4)]], ids=["singles", "portion", "mixed"])
+def test_rows_behind_the_last_request_are_zeros(ops, step, form, dtype):
+    """Whatever the memory of the output held before."""
+    torch.full((5000, 256), math.nan, dtype=DTYPES[dtype], device="cuda")
+    got = run_attention(Forced(ops, **form), 4, 2, 64, 16, step, dtype, extra=5)[0]
+    assert not got[sum(n for n, _ in step):].any()

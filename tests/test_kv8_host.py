@@ -64,3 +64,17 @@ def test_lists_of_more_rows_or_requests_than_there_are_are_refused(ops, q_lens, 
         attend(ops, 4, q_lens, requests)
     assert not ops.lib.calls
 
+
+def test_rows_behind_those_of_the_lists_are_zeros(ops):
+    """No kernel writes them; those of a captured step's padding are nobody's."""
+    ops.lib.calls["ptl_attention8_units"] = None
+    torch.utils.deterministic.fill_uninitialized_memory, was = True, torch.are_deterministic_algorithms_enabled()
+    torch.use_deterministic_algorithms(True)               # (memory that is not written is NaN)
+    try:
+        for q_lens in ([3], [1, 4], [1, 1], [40]):
+            T = sum(q_lens)
+            assert torch.isnan(attend(ops, T, q_lens, single_form=(1, 4)).float()).all()
+            assert not attend(ops, T + 3, q_lens, single_form=(1, 4))[T:].any()
+            assert torch.isnan(attend(ops, T + 3, q_lens, single_form=(1, 4), host_lengths_exact=False).float()).all()
+    finally:
+        torch.use_deterministic_algorithms(was)
